@@ -119,5 +119,14 @@ def current_stream(device_index) -> int:
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
+def current_device(expected: int) -> int:
+    """Index of the current CUDA device; ``expected`` (``tensor.get_device()``) must be one.  A launch goes to the current
+    device, so an op on tensors of another one makes that current first."""
+    import torch
+    if expected < 0:
+        raise ValueError("expected tensors on a CUDA device")
+    return torch._C._cuda_getDevice()
+
+
 def kernels_available() -> bool:
     return lib_path("kernels").exists()

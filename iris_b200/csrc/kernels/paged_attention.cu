@@ -1,0 +1,794 @@
+// paged_attention.cu — attention of one new token per sequence over a paged key-value cache.
+//
+//   out[b, h, :] = sum_j w_j V[j] / sum_j w_j,   w_j = exp(scale * q[b, h] . K[j]),   lse[b, h] = log(sum_j w_j)
+//
+// over the keys j that the newest token sees: all of the sequence's lens[b], or, with a window, the last `window` of them and
+// the first `sinks`.  Key j lies in slot j % page_size of page block_table[b, j / page_size]; query head h reads key head
+// h / (heads / kv_heads).  16-bit elements, fp32 sums, head dimension 64, 128 or 256.  No counterpart in the reference.
+//
+// Every key and value is read once and used for 2 * group products: HBM bounds it, and the work goes into an even share of
+// the bytes for every SM and enough of them in flight.
+//   * The keys that are seen are counted through (sinks first, then the window), so a mask costs nothing: a position in that
+//     count gives the key, the key its page.
+//   * A warp is a worker of its own: it takes 16 of the 64 keys of a tile, copies their rows into a ring of its own with
+//     cp.async (16 bytes a lane, rows found through the block table one step ahead), and keeps its own running maximum, sum
+//     and output in registers (one pass).  No barrier inside a sequence; the four warps meet when a sequence's tiles end.
+//   * Products go through mma.sync m16n8k16: up to 16 query heads that share a key head are the 16 rows.  (The rate that a
+//     group of 16 asks of them is 2 % of what the tensor cores do; a tcgen05 tile is 128 rows.)
+//   * The weights enter the second product as two 16-bit numbers, the rounded value and what it lost, so that the output has
+//     one rounding to 16 bits, its own.
+// Two ways to share out the keys:
+//   cluster  the CTAs of a cluster take equal parts of one sequence and key head and add up through distributed shared
+//            memory: one launch, no workspace.  For sequences of few tiles.
+//   stream   every CTA takes an equal part of all tiles of all sequences in a row, wherever that part begins and ends; parts
+//            of a sequence that spans CTAs go to a workspace and a second kernel, started early, adds them up in their order.
+// Both give the same bits in every run: no atomics, and parts are added in a fixed order.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <atomic>
+
+#include "iris/iris.cuh"
+#include "iris/ptx_sm100.cuh"
+
+namespace iris {
+namespace paged {
+
+using namespace iris::ptx;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kWarpKeys = 16;                    // keys of a warp in a tile
+constexpr int kTile = kWarps * kWarpKeys;        // keys of a tile
+constexpr int kRows = 16;                        // query heads of a tile
+constexpr int kJoinThreads = 256;
+constexpr uint32_t kSitePage = 95;
+
+template <int D>
+struct Shape {
+  static constexpr int kStages = D == 64 ? 6 : 3;              // ring of a warp
+  static constexpr int kQBufs = D == 64 ? 8 : 4;               // queries of the sequences that the ring reaches: stages + 1, a power of two
+  static constexpr int kHalf = kWarpKeys * D * 2;              // keys (or values) of a stage
+  static constexpr int kStageBytes = 2 * kHalf;                // = the fp32 output of a warp, which takes its place at the end
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kStats = 2 * kWarps * kRows * 4;        // maxima and sums of the warps
+  static constexpr int kMasks = kWarps * 8 * 4;                // which keys of a stage count
+  static constexpr int kSmem = kRing + kQBufs * kQBytes + kStats + kMasks + 64;
+  static constexpr int kPerSm = D == 256 ? 1 : 2;
+  static_assert(kStages <= 8 && kStages < kQBufs, "ring");
+  static_assert(kPerSm * (kSmem + 1024) <= 228 * 1024 && kSmem <= 227 * 1024, "shared-memory budget");
+};
+
+struct Params {
+  const uint8_t* q;          // strides in bytes
+  const uint8_t* k;
+  const uint8_t* v;
+  const int* table;
+  const int* lens;
+  uint8_t* out;
+  float* lse;                // may be null
+  StatusBlock* status;       // may be null
+  float* parts;              // stream: [ctas][2][rows][D], then maxima and sums [ctas][2][rows][2]
+  int4* jobs;                // stream: what the second kernel adds up
+  int64_t q_batch, q_head, page_pitch, slot_pitch, head_pitch, table_pitch, out_batch, out_head, lse_batch;
+  int batch, group, row_tiles, segments_per_seq, pages, page_shift, wide, window, sinks;
+  int ctas, rows;            // stream: CTAs of the first kernel; rows of a part
+  float scale_log2;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {   // ex2.approx: 2 ulp, 2^-inf = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {   // zeros where not taken
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  if (F16) {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&b);
+}
+template <bool F16>
+__device__ __forceinline__ float2 unpack(uint32_t v) {
+  return F16 ? __half22float2(*reinterpret_cast<__half2*>(&v)) : __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+}
+
+// The keys that a sequence's newest token sees, counted through: position v is key v below `sinks`, key v + skip above.
+struct Seen {
+  int n, sinks, skip;
+};
+__device__ __forceinline__ Seen seen_of(const Params& p, int len) {
+  const int64_t cap = (int64_t)p.wide << p.page_shift;
+  len = len < 0 ? 0 : (int64_t)len > cap ? (int)cap : len;
+  const int start = p.window > 0 && len > p.window ? len - p.window : 0;
+  Seen s;
+  s.sinks = p.sinks < start ? p.sinks : start;
+  s.skip = start - s.sinks;
+  s.n = len - s.skip;
+  return s;
+}
+__device__ __forceinline__ int tiles_of(const Seen& s) {   // a sequence without keys has one tile too: its output is zeros
+  const int t = s.n / kTile + (s.n % kTile != 0);
+  return t ? t : 1;
+}
+
+// Where a worker is: tile `tile` of `tiles` of segment `seg` (key head and row tile) of sequence b.
+struct Cursor {
+  Seen s;
+  int b, seg, tile, tiles, next_len;
+};
+__device__ __forceinline__ void enter(const Params& p, Cursor& c, int len) {
+  c.s = seen_of(p, len);
+  c.tiles = tiles_of(c.s);
+  c.next_len = c.b + 1 < p.batch ? p.lens[c.b + 1] : 0;
+}
+// Whether a new segment begins.
+__device__ __forceinline__ bool advance(const Params& p, Cursor& c) {
+  if (++c.tile < c.tiles) return false;
+  c.tile = 0;
+  if (++c.seg == p.segments_per_seq) {
+    c.seg = 0;
+    if (++c.b < p.batch) enter(p, c, c.next_len);
+  }
+  return true;
+}
+
+// Joins a part with maximum m2 and sum l2 (not 0) to (m, l); f and f2: what the outputs of the two are multiplied by.
+__device__ __forceinline__ void join(float& m, float& l, float m2, float l2, float& f, float& f2) {
+  const float top = fmaxf(m, m2);
+  f = m == top ? 1.f : exp2_fast(m - top);
+  f2 = m2 == top ? 1.f : exp2_fast(m2 - top);
+  l = l * f + l2 * f2;
+  m = top;
+}
+__device__ __forceinline__ void add(float4& a, float f, const float4& x, float f2) {
+  a.x = a.x * f + x.x * f2, a.y = a.y * f + x.y * f2, a.z = a.z * f + x.z * f2, a.w = a.w * f + x.w * f2;
+}
+__device__ __forceinline__ float log_sum(float m, float l) {   // m in powers of two
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+// One output row of 4 columns: rounded to 16 bits.
+template <bool F16>
+__device__ __forceinline__ void store4(uint8_t* dst, float4 a, float f) {
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack<F16>(a.x * f, a.y * f), pack<F16>(a.z * f, a.w * f));
+}
+
+template <int D, bool F16, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_kernel(const __grid_constant__ Params p) {
+  using S = Shape<D>;
+  constexpr int kChunks = D / 8;             // 16-byte pieces of a row
+  constexpr int kRowsPer = 32 / kChunks;     // rows that a warp copies at a time
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* stat_m = reinterpret_cast<float*>(smem + S::kRing + S::kQBufs * S::kQBytes);
+  float* stat_l = stat_m + kWarps * kRows;
+  volatile uint32_t* masks = reinterpret_cast<uint32_t*>(stat_l + kWarps * kRows);
+  volatile int* words = reinterpret_cast<int*>(const_cast<uint32_t*>(masks) + kWarps * 8);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;     // an accumulator's row (and row + 8), and column pair
+  const uint32_t q_s = smem_u32(smem) + S::kRing;
+  const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStageBytes;
+  const float* ring_f = reinterpret_cast<const float*>(smem);
+
+  grid_dependency_wait();
+  grid_dependency_launch();
+
+  // ---- this CTA's tiles: from cursor c on, `count` of them ----
+  Cursor c;
+  int64_t first = 0, total = 0;              // stream: its first tile among all
+  int count, ctas = 1;
+  if (CLUSTER) {
+    c.b = blockIdx.z;
+    c.seg = blockIdx.y;
+    enter(p, c, p.lens[c.b]);
+    const int parts = gridDim.x, r = blockIdx.x;
+    c.tile = (int)((int64_t)c.tiles * r / parts);
+    count = (int)((int64_t)c.tiles * (r + 1) / parts) - c.tile;
+  } else {
+    // tiles of the sequences before each thread's share of them
+    const int per = (p.batch + kThreads - 1) / kThreads;
+    const int b0 = min(p.batch, (int)threadIdx.x * per), b1 = min(p.batch, b0 + per);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += tiles_of(seen_of(p, p.lens[b]));
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    int64_t* sums = reinterpret_cast<int64_t*>(stat_m);
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int64_t before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sums[w];
+      total += sums[w];
+    }
+    total *= p.segments_per_seq;
+    before *= p.segments_per_seq;
+    mine *= p.segments_per_seq;
+    ctas = (int)min((int64_t)p.ctas, total);   // with a tile each at least: a part from every CTA that a segment spans
+    if ((int)blockIdx.x >= ctas) return;       // (then the jobs are listed by segment)
+    first = total * blockIdx.x / ctas;
+    count = (int)(total * (blockIdx.x + 1) / ctas - first);
+    if (mine > 0 && before <= first && first < before + mine) {
+      int64_t left = first - before;
+      int b = b0, n;
+      for (;; ++b) {
+        n = tiles_of(seen_of(p, p.lens[b]));
+        if (left < (int64_t)n * p.segments_per_seq) break;
+        left -= (int64_t)n * p.segments_per_seq;
+      }
+      words[0] = b;
+      words[1] = (int)(left / n);
+      words[2] = (int)(left % n);
+    }
+    __syncthreads();
+    c.b = words[0];
+    c.seg = words[1];
+    enter(p, c, p.lens[c.b]);
+    c.tile = words[2];
+  }
+
+  // ---- copies: the cursor of the loads runs a ring ahead of that of the products ----
+  Cursor l = c;
+  int l_left = count, l_stage = 0, l_seg = 0;
+  bool l_new = true;                          // the next step is its segment's first here
+  int l_page = 0;                             // page of this lane's row of the next step
+  auto find_page = [&]() {
+    const int at = l.tile * kTile + warp * kWarpKeys + (lane & 15);
+    const int key = at < l.s.sinks ? at : at + l.s.skip;
+    l_page = l_left > 0 && at < l.s.n ? p.table[l.b * p.table_pitch + (key >> p.page_shift)] : 0;
+  };
+  auto issue = [&]() {
+    if (l_left > 0) {
+      const int kv = p.row_tiles == 1 ? l.seg : l.seg / p.row_tiles;
+      if (l_new) {                            // the queries: four rows a warp
+        const int r0 = (l.seg - kv * p.row_tiles) * kRows;
+        const uint8_t* src = p.q + l.b * p.q_batch + (int64_t)(kv * p.group + r0) * p.q_head;
+        const uint32_t dst = q_s + (l_seg & (S::kQBufs - 1)) * S::kQBytes;
+#pragma unroll
+        for (int i = 0; i < 4 / kRowsPer; ++i) {
+          const int row = warp * 4 + i * kRowsPer + lane / kChunks, ch = lane % kChunks;
+          if (r0 + row < p.group) cp_async16(dst + row * D * 2 + ((ch ^ (row & 7)) << 4), src + row * p.q_head + ch * 16, true);
+        }
+      }
+      const int at = l.tile * kTile + warp * kWarpKeys + (lane & 15);
+      const int key = at < l.s.sinks ? at : at + l.s.skip;
+      const bool inside = at < l.s.n;
+      const bool ok = inside && (uint32_t)l_page < (uint32_t)p.pages;
+      if (inside && !ok) record_status(p.status, kBadPointer, kSitePage, l.b, key, (uint64_t)(int64_t)l_page);
+      const int64_t off =
+          ok ? l_page * p.page_pitch + (key & ((1 << p.page_shift) - 1)) * p.slot_pitch + kv * p.head_pitch : 0;
+      const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+      if (lane == 0) masks[warp * 8 + l_stage] = mask;
+      const uint32_t dst = ring + l_stage * S::kStageBytes;
+#pragma unroll
+      for (int i = 0; i < kWarpKeys / kRowsPer; ++i) {
+        const int row = i * kRowsPer + lane / kChunks, ch = lane % kChunks;
+        const int64_t o = __shfl_sync(0xffffffffu, off, row) + ch * 16;
+        const bool take = mask >> row & 1;
+        const uint32_t d = dst + row * D * 2 + ((ch ^ (row & 7)) << 4);
+        cp_async16(d, p.k + o, take);
+        cp_async16(d + S::kHalf, p.v + o, take);
+      }
+      l_stage = l_stage + 1 == S::kStages ? 0 : l_stage + 1;
+      --l_left;
+      l_new = advance(p, l);
+      if (l_new) ++l_seg;
+      find_page();
+    }
+    cp_commit();
+  };
+  find_page();
+#pragma unroll 1
+  for (int i = 0; i < S::kStages; ++i) issue();
+
+  // ---- products ----
+  float o[D / 8][4], m[2], sum[2];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    sum[0] = sum[1] = 0.f;
+  };
+  clear();
+  const int mat = lane >> 3, mrow = lane & 7;   // ldmatrix: which of the four 8 x 8 pieces this lane addresses, and its row
+  int stage = 0, c_seg = 0;
+  bool fresh = true, whole = c.tile == 0;       // whole: the segment began in this CTA
+  int64_t seg_first = first - c.tile;           // stream: its first tile among all
+
+  // The four warps' results of a segment (whose last stage here is `stage`): sum over them of this thread's four columns
+  // of a row.
+  auto merged = [&](int item, float& mx, float& l) {
+    const int row = item / (D / 4), col = item % (D / 4);
+    mx = fmaxf(fmaxf(stat_m[row], stat_m[kRows + row]), fmaxf(stat_m[2 * kRows + row], stat_m[3 * kRows + row]));
+    l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = stat_m[w * kRows + row], lw = stat_l[w * kRows + row];
+      const float f = mw == mx ? 1.f : exp2_fast(mw - mx);
+      const float4 x = *reinterpret_cast<const float4*>(ring_f + (w * S::kStages + stage) * (S::kStageBytes / 4) + row * D +
+                                                        ((((col >> 1) ^ (row & 7)) << 3) | ((col & 1) << 2)));
+      if (lw != 0.f) {    // (a warp without keys, or with keys of minus infinity only, adds nothing; one with a NaN adds that)
+        l += lw * f;
+        a.x += x.x * f, a.y += x.y * f, a.z += x.z * f, a.w += x.w * f;
+      }
+    }
+    return a;
+  };
+  // A row's finished values: output, and the logarithm of the sum
+  auto finish = [&](int b, int head, int col, float4 a, float mx, float l) {
+    store4<F16>(p.out + b * p.out_batch + head * p.out_head + col * 8, a, l == 0.f ? 0.f : 1.f / l);
+    if (p.lse && col == 0) p.lse[b * p.lse_batch + head] = log_sum(mx, l);
+  };
+  // this warp's results into the ring stage it has just used up
+  auto deposit = [&]() {
+    float* dst = reinterpret_cast<float*>(smem) + (warp * S::kStages + stage) * (S::kStageBytes / 4);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x = sum[h];
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      if (t == 0) {
+        stat_m[warp * kRows + g + 8 * h] = m[h];
+        stat_l[warp * kRows + g + 8 * h] = x;
+      }
+      if (h == 0 || p.group > 8) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          *reinterpret_cast<float2*>(dst + (g + 8 * h) * D + ((i ^ g) << 3) + 2 * t) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+      }
+    }
+  };
+
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    cp_wait<S::kStages - 1>();
+    __syncwarp();
+    if (fresh) {
+      __syncthreads();   // all four warps' rows of the queries are there
+      fresh = false;
+    }
+    const uint32_t ks = ring + stage * S::kStageBytes, vs = ks + S::kHalf;
+    const uint32_t qs = q_s + (c_seg & (S::kQBufs - 1)) * S::kQBytes;
+    const uint32_t mask = masks[warp * 8 + stage] & 0xffffu;
+    if (mask) {
+      float sc[2][2][4];                        // two chains each: even and odd steps of the dimension
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) sc[x][n][0] = sc[x][n][1] = sc[x][n][2] = sc[x][n][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t a[4], b[4];
+        const int ra = (mat & 1) * 8 + mrow, rb = (mat >> 1) * 8 + mrow;
+        ldsm4(a, qs + ra * D * 2 + (((kk * 2 + (mat >> 1)) ^ mrow) << 4));
+        ldsm4(b, ks + rb * D * 2 + (((kk * 2 + (mat & 1)) ^ mrow) << 4));
+        mma<F16>(sc[kk & 1][0], a, b[0], b[1]);
+        mma<F16>(sc[kk & 1][1], a, b[2], b[3]);
+      }
+      float s[2][4];                            // [row half][key 2t, 2t + 1, 2t + 8, 2t + 9]
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = e >> 1, r = 2 * h + (e & 1);
+          const bool ok = mask >> (8 * n + 2 * t + (e & 1)) & 1;
+          s[h][e] = ok ? sc[0][n][r] + sc[1][n][r] : -INFINITY;
+        }
+      const int halves = p.group > 8 ? 2 : 1;
+      uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h < halves) {
+          float mx = fmaxf(fmaxf(s[h][0], s[h][1]), fmaxf(s[h][2], s[h][3]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * p.scale_log2;
+          if (__any_sync(0xffffffffu, mx > m[h])) {
+            const float m_new = fmaxf(m[h], mx);
+            const float f = m_new == m[h] ? 1.f : exp2_fast(m[h] - m_new);
+            m[h] = m_new;
+            sum[h] *= f;
+#pragma unroll
+            for (int d = 0; d < D / 8; ++d) o[d][2 * h] *= f, o[d][2 * h + 1] *= f;
+          }
+          const float shift = m[h] == -INFINITY ? 0.f : -m[h];
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = exp2_fast(fmaf(s[h][e], p.scale_log2, shift));
+          sum[h] += (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            hi[h + 2 * n] = pack<F16>(w[2 * n], w[2 * n + 1]);
+            const float2 r = unpack<F16>(hi[h + 2 * n]);
+            lo[h + 2 * n] = pack<F16>(w[2 * n] - r.x, w[2 * n + 1] - r.y);
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        uint32_t b[4];
+        ldsm4_t(b, vs + ((mat & 1) * 8 + mrow) * D * 2 + (((d * 2 + (mat >> 1)) ^ mrow) << 4));
+        mma<F16>(o[2 * d], hi, b[0], b[1]);
+        mma<F16>(o[2 * d + 1], hi, b[2], b[3]);
+        mma<F16>(o[2 * d], lo, b[0], b[1]);
+        mma<F16>(o[2 * d + 1], lo, b[2], b[3]);
+      }
+    }
+    __syncwarp();        // every lane has read the stage
+
+    const bool ends = c.tile + 1 == c.tiles;
+    if (!CLUSTER && (ends || i + 1 == count)) {
+      deposit();
+      __syncthreads();
+      const int kv = p.row_tiles == 1 ? c.seg : c.seg / p.row_tiles, r0 = (c.seg - kv * p.row_tiles) * kRows;
+      const int rows = min(kRows, p.group - r0);
+      const bool direct = whole && ends;
+      float* part = p.parts + ((int64_t)blockIdx.x * 2 + (whole ? 1 : 0)) * p.rows * D;
+      float* ml = p.parts + (int64_t)p.ctas * 2 * p.rows * D + ((int64_t)blockIdx.x * 2 + (whole ? 1 : 0)) * p.rows * 2;
+#pragma unroll 1
+      for (int item = threadIdx.x; item < rows * (D / 4); item += kThreads) {
+        float mx, l;
+        const float4 a = merged(item, mx, l);
+        const int row = item / (D / 4), col = item % (D / 4);
+        if (direct) {
+          finish(c.b, kv * p.group + r0 + row, col, a, mx, l);
+        } else {
+          *reinterpret_cast<float4*>(part + row * D + col * 4) = a;
+          if (col == 0) *reinterpret_cast<float2*>(ml + row * 2) = make_float2(mx, l);
+        }
+      }
+      if (threadIdx.x == 0 && whole) {
+        // what the second kernel adds up: a segment's parts from this CTA to that of its last tile; listed by segment
+        // where there are fewer of them than CTAs, else by the CTA in which it begins
+        const int64_t segments = (int64_t)p.batch * p.segments_per_seq, id = (int64_t)c.b * p.segments_per_seq + c.seg;
+        const int last = ends ? (int)blockIdx.x : (int)(((seg_first + c.tiles) * ctas - 1) / total);
+        const int4 job = make_int4(blockIdx.x, last, ends ? -1 : c.b, c.seg);
+        if (segments <= p.ctas) p.jobs[id] = job;
+        else if (!ends || i + 1 == count) p.jobs[blockIdx.x] = job;
+      }
+      if (threadIdx.x == 0 && !whole && i + 1 == count && p.batch * (int64_t)p.segments_per_seq > p.ctas)
+        p.jobs[blockIdx.x] = make_int4(0, 0, -1, 0);
+      __syncthreads();   // the stage and the statistics are free again
+      clear();
+      fresh = whole = true;
+      seg_first += c.tiles;
+      ++c_seg;
+    }
+    if (!CLUSTER || i + 1 < count) advance(p, c);
+    issue();
+    if (CLUSTER && i + 1 == count) break;
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+  }
+
+  if (CLUSTER) {
+    cp_wait<0>();
+    if (count == 0) __syncthreads();   // (the queries' barrier)
+    deposit();
+    __syncthreads();
+    const int kv = p.row_tiles == 1 ? (int)blockIdx.y : (int)blockIdx.y / p.row_tiles, r0 = ((int)blockIdx.y - kv * p.row_tiles) * kRows;
+    const int rows = min(kRows, p.group - r0);
+    const int parts = gridDim.x;
+    if (parts == 1) {
+      for (int item = threadIdx.x; item < rows * (D / 4); item += kThreads) {
+        float mx, l;
+        const float4 a = merged(item, mx, l);
+        finish(blockIdx.z, kv * p.group + r0 + item / (D / 4), item % (D / 4), a, mx, l);
+      }
+      return;
+    }
+    // where the queries were: this CTA's part, for the others to read
+    float* part = reinterpret_cast<float*>(smem + S::kRing);
+    float2* ml = reinterpret_cast<float2*>(part + kRows * D);
+    static_assert(kRows * D * 4 + kRows * 8 <= S::kQBufs * S::kQBytes, "the part fits");
+    for (int item = threadIdx.x; item < rows * (D / 4); item += kThreads) {
+      float mx, l;
+      const float4 a = merged(item, mx, l);
+      *reinterpret_cast<float4*>(part + item * 4) = a;
+      if (item % (D / 4) == 0) ml[item / (D / 4)] = make_float2(mx, l);
+    }
+    cluster_sync_all();
+    const uint32_t part_s = smem_u32(part), ml_s = smem_u32(ml);
+    for (int item = blockIdx.x * kThreads + threadIdx.x; item < rows * (D / 4); item += parts * kThreads) {
+      const int row = item / (D / 4);
+      float mx = -INFINITY, l = 0.f;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int r = 0; r < parts; ++r) {
+        float mr, lr;
+        float4 x;
+        asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(mr), "=f"(lr) : "r"(mapa_shared(ml_s + row * 8, r)) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                     : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(mapa_shared(part_s + item * 16, r)) : "memory");
+        if (lr == 0.f) continue;
+        float fo, fr;
+        join(mx, l, mr, lr, fo, fr);
+        add(a, fo, x, fr);
+      }
+      finish(blockIdx.z, kv * p.group + r0 + row, item % (D / 4), a, mx, l);
+    }
+    cluster_sync_all();   // no CTA leaves before the others have read its part
+  }
+}
+
+// Second kernel of the stream form: the parts of a segment that spans CTAs, in their order.  A warp takes 128 columns of a
+// row (`rows_per` rows a block); the block's warps share out the parts of a row where there are fewer rows than warps.
+template <int D, bool F16>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ Params p, int rows_per) {
+  constexpr int kW = kJoinThreads / 32;
+  constexpr int kV = D / 128 ? D / 128 : 1;          // 16-byte pieces of a row per lane
+  __shared__ float4 acc[kW][D / 4];
+  __shared__ float2 stats[kW];
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int4 job = p.jobs[blockIdx.x];
+  if (job.z < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int share = kW / rows_per;                   // warps of a row
+  const int row = blockIdx.y * rows_per + warp / share, w = warp % share;
+  const int kv = job.w / p.row_tiles, r0 = (job.w - kv * p.row_tiles) * kRows;
+  const bool live = row < min(kRows, p.group - r0);
+  const float* ml = p.parts + (int64_t)p.ctas * 2 * p.rows * D;
+  float mx = -INFINITY, l = 0.f;
+  float4 a[kV];
+#pragma unroll
+  for (int v = 0; v < kV; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int n = job.y - job.x + 1;
+  if (live) {
+    constexpr int U = 4;
+#pragma unroll 1
+    for (int i0 = w; i0 < n; i0 += share * U) {
+      float2 s[U];
+      float4 x[U][kV];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * share;
+        s[u] = make_float2(-INFINITY, 0.f);
+        if (i < n) {
+          const int64_t slot = ((int64_t)(job.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row;
+          s[u] = *reinterpret_cast<const float2*>(ml + slot * 2);
+#pragma unroll
+          for (int v = 0; v < kV; ++v)
+            if (lane + v * 32 < D / 4) x[u][v] = *reinterpret_cast<const float4*>(p.parts + slot * D + (lane + v * 32) * 4);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (s[u].y == 0.f) continue;
+        float fo, fr;
+        join(mx, l, s[u].x, s[u].y, fo, fr);
+#pragma unroll
+        for (int v = 0; v < kV; ++v) add(a[v], fo, x[u][v], fr);
+      }
+    }
+  }
+  if (share > 1) {
+#pragma unroll
+    for (int v = 0; v < kV; ++v)
+      if (lane + v * 32 < D / 4) acc[warp][lane + v * 32] = a[v];
+    if (lane == 0) stats[warp] = make_float2(mx, l);
+    __syncthreads();
+    if (w != 0) return;
+    for (int r = 1; r < share; ++r) {
+      const float2 s = stats[warp + r];
+      if (s.y == 0.f) continue;
+      float fo, fr;
+      join(mx, l, s.x, s.y, fo, fr);
+#pragma unroll
+      for (int v = 0; v < kV; ++v)
+        if (lane + v * 32 < D / 4) add(a[v], fo, acc[warp + r][lane + v * 32], fr);
+    }
+  }
+  if (!live) return;
+  const int head = kv * p.group + r0 + row;
+  const float f = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int v = 0; v < kV; ++v)
+    if (lane + v * 32 < D / 4) store4<F16>(p.out + job.z * p.out_batch + head * p.out_head + (lane + v * 32) * 8, a[v], f);
+  if (p.lse && lane == 0) p.lse[job.z * p.lse_batch + head] = log_sum(mx, l);
+}
+
+}  // namespace paged
+}  // namespace iris
+
+// ================================================================================================
+// Host side
+// ================================================================================================
+namespace {
+
+using namespace iris::paged;
+thread_local char g_paged_err[256] = "";
+
+int refuse(const char* what) {
+  snprintf(g_paged_err, sizeof(g_paged_err), "paged attention: %s", what);
+  return -1;
+}
+
+int sms_of(int device) {
+  static std::atomic<int> known[64];
+  if (device >= 0 && device < 64 && known[device].load(std::memory_order_relaxed)) return known[device].load(std::memory_order_relaxed);
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  if (device >= 0 && device < 64) known[device].store(sms, std::memory_order_relaxed);
+  return sms;
+}
+
+// The limit of dynamic shared memory is a property of the kernel on one device.
+template <class K>
+cudaError_t allow_smem(K kernel, int bytes, int device, std::atomic<uint64_t>& done) {
+  if (device < 64 && (done.load(std::memory_order_acquire) >> device & 1)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && device < 64) done.fetch_or(1ull << device, std::memory_order_release);
+  return e;
+}
+
+template <int D, bool F16>
+int launch_paged(Params& p, int cluster, int device, cudaStream_t stream) {
+  static std::atomic<uint64_t> done[2];
+  const auto kern = cluster ? paged_attention_kernel<D, F16, true> : paged_attention_kernel<D, F16, false>;
+  cudaError_t e = allow_smem(kern, Shape<D>::kSmem, device, done[cluster ? 1 : 0]);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster ? cluster : 1;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = cluster ? dim3(cluster, p.segments_per_seq, p.batch) : dim3(p.ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Shape<D>::kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kern, (const Params)p);
+  if (e == cudaSuccess && !cluster) {
+    // jobs times rows: a block for every row while there are few, else several rows a block
+    const int64_t segments = (int64_t)p.batch * p.segments_per_seq;
+    const int jobs = (int)(segments < p.ctas ? segments : p.ctas);
+    int per = 8;
+    while (per > 1 && jobs * ((p.rows + per - 1) / per) < 296) per /= 2;
+    cfg.gridDim = dim3(jobs, (p.rows + per - 1) / per);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<D, F16>, (const Params)p, per);
+  }
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();   // reported here: it must not turn up at someone else's launch
+    snprintf(g_paged_err, sizeof(g_paged_err), "paged attention: launch: %s", cudaGetErrorString(e));
+    return -3;
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* iris_paged_attention_last_error() { return g_paged_err; }
+
+// q [batch, heads, dim], k and v [pages, page_size, kv_heads, dim], out like q: pitches in elements, 16-byte aligned rows.
+// table [batch, wide] and lens [batch]: int32.  lse [batch, heads] fp32 or null.  longest: what the lengths are expected not to
+// exceed (0: the table's width); it chooses the form and nothing else.  cluster: CTAs of a cluster, 0 the stream form, -1 by rule.
+// Returns 0, a positive number of bytes if the form needs a workspace of that size (16-byte aligned) and got a smaller one, or
+// a negative code with a message in iris_paged_attention_last_error().  The device must be the current one.
+int iris_k_paged_attention(const void* q, int64_t q_batch, int64_t q_head, const void* k, const void* v, int64_t page_pitch,
+                           int64_t slot_pitch, int64_t head_pitch, int64_t pages, int page_size, int kv_heads,
+                           const void* table, int64_t table_pitch, int64_t wide, const void* lens, void* out,
+                           int64_t out_batch, int64_t out_head, void* lse, int64_t lse_batch, int64_t batch, int heads,
+                           int dim, int dtype, int window, int sinks, float scale, int64_t longest, int cluster, void* work,
+                           int64_t work_bytes, void* status, int device, void* stream) {
+  g_paged_err[0] = 0;
+  if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads) return refuse("query heads must be a multiple of key heads");
+  if (dim != 64 && dim != 128 && dim != 256) return refuse("head dimension 64, 128 or 256");
+  if (dtype != 0 && dtype != 1) return refuse("dtype must be 0 (bf16) or 1 (fp16)");
+  if (page_size < 1 || (page_size & (page_size - 1))) return refuse("page size must be a power of two");
+  if (pages < 1 || wide < 1 || pages > 0x7fffffff || wide > 0x7fffffff || batch > 0x7fffffff) return refuse("no pages, or too many");
+  if (window < 0 || sinks < 0 || !(scale > 0.f) || isinf(scale)) return refuse("window and sinks must not be negative, scale above 0");
+  // a pitch along one element says nothing
+  if (batch == 1) q_batch = out_batch = table_pitch = lse_batch = 0;
+  if (heads == 1) q_head = out_head = 0;
+  if (pages == 1) page_pitch = 0;
+  if (page_size == 1) slot_pitch = 0;
+  if (kv_heads == 1) head_pitch = 0;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+       reinterpret_cast<uintptr_t>(out)) % 16 || (q_batch | q_head | page_pitch | slot_pitch | head_pitch | out_batch | out_head) % 8)
+    return refuse("rows of q, k, v and out must start on 16 bytes");
+  const int sms = sms_of(device);
+  if (sms < 1) return refuse("no device");
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.q = static_cast<const uint8_t*>(q);
+  p.k = static_cast<const uint8_t*>(k);
+  p.v = static_cast<const uint8_t*>(v);
+  p.table = static_cast<const int*>(table);
+  p.lens = static_cast<const int*>(lens);
+  p.out = static_cast<uint8_t*>(out);
+  p.lse = static_cast<float*>(lse);
+  p.status = static_cast<iris::StatusBlock*>(status);
+  p.q_batch = q_batch * 2, p.q_head = q_head * 2;
+  p.page_pitch = page_pitch * 2, p.slot_pitch = slot_pitch * 2, p.head_pitch = head_pitch * 2;
+  p.table_pitch = table_pitch;
+  p.out_batch = out_batch * 2, p.out_head = out_head * 2;
+  p.lse_batch = lse_batch;
+  p.batch = (int)batch;
+  p.group = heads / kv_heads;
+  p.row_tiles = (p.group + kRows - 1) / kRows;
+  p.segments_per_seq = kv_heads * p.row_tiles;
+  p.pages = (int)pages;
+  while ((1 << p.page_shift) < page_size) ++p.page_shift;
+  p.wide = (int)wide;
+  p.window = window;
+  p.sinks = sinks;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.rows = p.group < kRows ? p.group : kRows;
+  const int per_sm = dim == 256 ? 1 : 2;
+  p.ctas = sms * per_sm;
+  const int64_t segments = batch * p.segments_per_seq;
+  if (cluster < 0) {
+    int64_t most = wide * (int64_t)page_size;
+    if (longest > 0 && longest < most) most = longest;
+    if (window > 0 && (int64_t)window + sinks < most) most = (int64_t)window + sinks;
+    const int64_t tiles = (most + kTile - 1) / kTile;
+    cluster = 0;
+    if (tiles <= 32) {
+      cluster = 1;
+      while (cluster < 8 && cluster < tiles && segments * cluster < p.ctas) cluster *= 2;
+    }
+  }
+  if (batch > 65535 || p.segments_per_seq > 65535) cluster = 0;
+  if (cluster == 0) {
+    const int64_t need = (int64_t)p.ctas * (16 + 2 * p.rows * (dim + 2) * 4);
+    if (!work || work_bytes < need) return (int)need;
+    p.jobs = static_cast<int4*>(work);
+    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + (int64_t)p.ctas * 16);
+  } else if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) {
+    return refuse("a cluster has 1, 2, 4 or 8 CTAs");
+  }
+  const auto st = static_cast<cudaStream_t>(stream);
+  if (dim == 64) return dtype ? launch_paged<64, true>(p, cluster, device, st) : launch_paged<64, false>(p, cluster, device, st);
+  if (dim == 128) return dtype ? launch_paged<128, true>(p, cluster, device, st) : launch_paged<128, false>(p, cluster, device, st);
+  return dtype ? launch_paged<256, true>(p, cluster, device, st) : launch_paged<256, false>(p, cluster, device, st);
+}
+
+}  // extern "C"

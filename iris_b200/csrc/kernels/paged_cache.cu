@@ -1,0 +1,303 @@
+// paged_cache.cu — pages of a paged key-value cache handed out and taken back on the GPU, from the requests' lengths.
+//
+// reserve: request b holds lens[b] tokens in ceil(lens[b] / page_size) pages and gets new_lens[b] more.  In the requests' order
+// each takes the pages it lacks from the end of the list of free pages,
+//
+//   need_b = ceil((lens[b] + new_lens[b]) / page_size) - ceil(lens[b] / page_size),   first_b = need_0 + .. + need_{b-1}
+//   block_table[b, held_b + i] = free[count - 1 - (first_b + i)],   0 <= i < need_b
+//
+// as long as they last: a request with first_b + need_b > count, too long for its row of the table, or with more tokens than rows
+// were left for them, gets nothing.  Every new
+// token gets its position and its slot, page * page_size + position % page_size.  release: pages of chosen requests go back to
+// the end of the list.  No counterpart in the reference.
+//
+// A call's time is its launch and a few passes through memory in a row (lengths, prefix sums, free list or table, output), so
+// it is one launch: every CTA of one cluster makes the prefix sums for itself, in chunks of a request per thread, and the tokens
+// and pages of a chunk are shared out over the cluster's threads, whatever their lengths, by a search in the chunk's sums.
+// What may be updated in place (lengths, count) is written after a barrier of the cluster, when every CTA has read it.
+// All sums are whole numbers in 64 bits.
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include "iris/ptx_sm100.cuh"
+
+namespace iris {
+namespace pages {
+
+using namespace iris::ptx;
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+
+struct Params {
+  const int* lens;
+  const int* more;           // reserve: new tokens per request; release: not 0 for the requests to end
+  int* table;
+  int* free;
+  const int* count;
+  int* slots;
+  int* positions;
+  int* lens_out;
+  int* count_out;
+  int64_t table_pitch, tokens, row_stride;
+  int batch, wide, page_shift, capacity;
+};
+
+// A chunk of kThreads requests, one a thread, and the sums over them, for every thread to search.
+struct Chunk {
+  int64_t pages_upto[kThreads];    // of pages, this request's included
+  int64_t tokens_upto[kThreads];
+  int len[kThreads], held[kThreads], granted[kThreads];
+  int64_t warp_sum[2][kWarps];
+};
+
+// Sums of the threads before this one and this one's own.
+__device__ __forceinline__ int64_t scan(int64_t x, int64_t* warp_sum, int64_t& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sum[warp] = x;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) x += warp_sum[w];
+    all += warp_sum[w];
+  }
+  return x;
+}
+
+// The first request of the chunk with more than `at` before or in it.
+__device__ __forceinline__ int search(const int64_t* upto, int64_t at) {
+  int lo = 0;
+#pragma unroll
+  for (int step = kThreads / 2; step > 0; step >>= 1)
+    if (upto[lo + step - 1] <= at) lo += step;
+  return lo;
+}
+
+template <bool RELEASE>
+__global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__ Params p) {
+  __shared__ Chunk c;
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int mask = (1 << p.page_shift) - 1;
+  const int rank = blockIdx.x, ctas = gridDim.x;
+  const int64_t at0 = (int64_t)rank * kThreads + threadIdx.x, step = (int64_t)ctas * kThreads;
+  const int count = min(max(*p.count, 0), p.capacity);
+  int64_t pages = 0, tokens = 0;   // of the chunks before
+  int64_t used = 0;                // pages handed out, or taken back, so far
+
+  // Request base + threadIdx.x of a chunk; true if it gets its pages.  Leaves the chunk's sums in shared memory.
+  int len, more;
+  auto take_in = [&](int base, int64_t& all_pages, int64_t& all_tokens) {
+    const int b = base + threadIdx.x;
+    len = more = 0;
+    if (b < p.batch) {
+      len = max(p.lens[b], 0);
+      more = max(p.more[b], 0);
+    }
+    __syncthreads();               // the chunk before has been used
+    const int64_t t_upto = RELEASE ? 0 : scan(more, c.warp_sum[1], all_tokens);
+    int held = (int)(((int64_t)len + mask) >> p.page_shift);
+    int64_t need = 0;
+    bool fits = b < p.batch;
+    if (RELEASE) {
+      held = min(held, p.wide);
+      fits = fits && more != 0;
+      if (fits) need = held;
+    } else {
+      fits = fits && (int64_t)len + more <= ((int64_t)p.wide << p.page_shift) && (int64_t)len + more <= 0x7fffffff &&
+             (p.row_stride ? more <= p.row_stride : tokens + t_upto <= p.tokens);
+      if (fits) need = (((int64_t)len + more + mask) >> p.page_shift) - held;
+    }
+    const int64_t upto = scan(need, c.warp_sum[0], all_pages);
+    const bool granted = fits && (need == 0 || pages + upto <= (RELEASE ? p.capacity - count : count));
+    c.pages_upto[threadIdx.x] = upto;
+    c.tokens_upto[threadIdx.x] = t_upto;
+    c.len[threadIdx.x] = len;
+    c.held[threadIdx.x] = held;
+    c.granted[threadIdx.x] = granted;
+    // requests that got pages come before those that did not, so the last of them has the sum
+    __syncthreads();
+    return granted;
+  };
+  auto last_granted = [&](int64_t all) {   // pages of the chunk that were handed out
+    if (all == 0) return (int64_t)0;
+    const int64_t room = (RELEASE ? p.capacity - count : count) - pages;
+    if (all <= room) return all;
+    // the largest sum within the room
+    if (room <= 0) return (int64_t)0;
+    const int i = search(c.pages_upto, room);
+    return i > 0 ? c.pages_upto[i - 1] : (int64_t)0;
+  };
+
+  bool granted = false;
+  for (int base = 0; base < p.batch; base += kThreads) {
+    int64_t all_pages = 0, all_tokens = 0;
+    granted = take_in(base, all_pages, all_tokens);
+    const int64_t got = last_granted(all_pages);
+    used += got;
+    for (int64_t k = at0; k < got; k += step) {
+      const int r = search(c.pages_upto, k);
+      const int64_t i = k - (r ? c.pages_upto[r - 1] : 0);
+      int* entry = p.table + (base + r) * p.table_pitch;
+      if (RELEASE) {
+        p.free[count + pages + k] = entry[i];
+        entry[i] = -1;
+      } else {
+        entry[c.held[r] + i] = p.free[count - 1 - (pages + k)];
+      }
+    }
+    if (!RELEASE) {
+      // token rows of this chunk's requests: packed one request behind the other, or row_stride rows to a request
+      const int n = min(kThreads, p.batch - base);
+      const int64_t row0 = p.row_stride ? base * p.row_stride : tokens;
+      const int64_t row1 = min(p.tokens, p.row_stride ? (base + n) * p.row_stride : tokens + all_tokens);
+      for (int64_t row = row0 + at0; row < row1; row += step) {
+        int r;
+        int64_t j;
+        bool valid = true;
+        if (p.row_stride) {
+          r = (int)((row - row0) / p.row_stride);
+          j = row - row0 - r * p.row_stride;
+          valid = j < c.tokens_upto[r] - (r ? c.tokens_upto[r - 1] : 0);
+        } else {
+          r = search(c.tokens_upto, row - row0);
+          j = row - row0 - (r ? c.tokens_upto[r - 1] : 0);
+        }
+        int pos = -1, slot = -1;
+        if (valid && c.granted[r]) {
+          pos = (int)(c.len[r] + j);
+          const int i = pos >> p.page_shift, fresh = i - c.held[r];
+          const int page = fresh < 0 ? p.table[(base + r) * p.table_pitch + i]
+                                     : p.free[count - 1 - (pages + (r ? c.pages_upto[r - 1] : 0) + fresh)];
+          const int64_t s = ((int64_t)page << p.page_shift) + (pos & mask);
+          slot = page < 0 || s > 0x7fffffff ? -1 : (int)s;   // an entry that is no page: as a token that is not kept
+        }
+        p.slots[row] = slot;
+        p.positions[row] = pos;
+      }
+    }
+    pages += all_pages;
+    tokens += all_tokens;
+  }
+  if (!RELEASE) {
+    const int64_t end = p.row_stride ? p.batch * p.row_stride : tokens;
+    for (int64_t row = end + at0; row < p.tokens; row += step) p.slots[row] = p.positions[row] = -1;
+  }
+  cluster_sync_all();   // every CTA has read the lengths and the count
+  if (rank != 0) return;
+  auto put = [&](int b) {
+    if (b < p.batch) p.lens_out[b] = !granted ? p.lens[b] : RELEASE ? 0 : len + more;
+  };
+  if (p.batch <= kThreads) {
+    put(threadIdx.x);
+  } else {
+    pages = tokens = 0;
+    for (int base = 0; base < p.batch; base += kThreads) {
+      int64_t all_pages = 0, all_tokens = 0;
+      granted = take_in(base, all_pages, all_tokens);
+      put(base + threadIdx.x);
+      pages += all_pages;
+      tokens += all_tokens;
+    }
+  }
+  if (threadIdx.x == 0) *p.count_out = (int)(RELEASE ? count + used : count - used);
+}
+
+thread_local char g_err[256] = "";
+
+int refuse(const char* what) {
+  snprintf(g_err, sizeof(g_err), "%s", what);
+  return -1;
+}
+
+template <bool RELEASE>
+int launch(const Params& p, int64_t items, void* stream) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  // as many CTAs as have something to write, up to a cluster of eight
+  int ctas = 1;
+  while (ctas < 8 && items > (int64_t)ctas * kThreads) ctas *= 2;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, pages_kernel<RELEASE>, p);
+  if (e == cudaSuccess) return 0;
+  (void)cudaGetLastError();   // reported here: it must not turn up at someone else's launch
+  snprintf(g_err, sizeof(g_err), "launch: %s", cudaGetErrorString(e));
+  return -3;
+}
+
+}  // namespace pages
+}  // namespace iris
+
+extern "C" {
+
+const char* iris_pages_last_error() { return iris::pages::g_err; }
+
+// All arrays int32 on the current device.  table [batch, wide] with rows table_pitch apart; free [capacity], count [1].
+// slots, positions [tokens]: row_stride rows to a request, or, with row_stride 0, packed; rows of no token get -1.
+// lens_out and count_out may be lens and count.
+int iris_k_reserve_slots(const void* lens, const void* new_lens, void* table, int64_t table_pitch, int64_t wide, void* free,
+                         int64_t capacity, const void* count, int page_size, int64_t batch, void* slots, void* positions,
+                         int64_t tokens, int64_t row_stride, void* lens_out, void* count_out, void* stream) {
+  using namespace iris::pages;
+  g_err[0] = 0;
+  if (page_size < 1 || (page_size & (page_size - 1))) return refuse("page size must be a power of two");
+  if (batch < 1 || batch > 0x7fffffff - kThreads || wide < 1 || wide > 0x7fffffff || capacity < 0 || capacity > 0x7fffffff || tokens < 0 || row_stride < 0)
+    return refuse("sizes out of range");
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.lens = static_cast<const int*>(lens);
+  p.more = static_cast<const int*>(new_lens);
+  p.table = static_cast<int*>(table);
+  p.free = static_cast<int*>(free);
+  p.count = static_cast<const int*>(count);
+  p.slots = static_cast<int*>(slots);
+  p.positions = static_cast<int*>(positions);
+  p.lens_out = static_cast<int*>(lens_out);
+  p.count_out = static_cast<int*>(count_out);
+  p.table_pitch = table_pitch, p.tokens = tokens, p.row_stride = row_stride;
+  p.batch = (int)batch, p.wide = (int)wide, p.capacity = (int)capacity;
+  while ((1 << p.page_shift) < page_size) ++p.page_shift;
+  return launch<false>(p, tokens, stream);
+}
+
+// which [batch]: not 0 for the requests whose pages go back; their length becomes 0 and their entries of the table -1.
+int iris_k_release_slots(void* lens, const void* which, void* table, int64_t table_pitch, int64_t wide, void* free,
+                         int64_t capacity, void* count, int page_size, int64_t batch, void* stream) {
+  using namespace iris::pages;
+  g_err[0] = 0;
+  if (page_size < 1 || (page_size & (page_size - 1))) return refuse("page size must be a power of two");
+  if (batch < 1 || batch > 0x7fffffff - kThreads || wide < 1 || wide > 0x7fffffff || capacity < 0 || capacity > 0x7fffffff)
+    return refuse("sizes out of range");
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.lens = static_cast<const int*>(lens);
+  p.more = static_cast<const int*>(which);
+  p.table = static_cast<int*>(table);
+  p.free = static_cast<int*>(free);
+  p.count = static_cast<const int*>(count);
+  p.lens_out = static_cast<int*>(lens);
+  p.count_out = static_cast<int*>(count);
+  p.table_pitch = table_pitch;
+  p.batch = (int)batch, p.wide = (int)wide, p.capacity = (int)capacity;
+  while ((1 << p.page_shift) < page_size) ++p.page_shift;
+  return launch<true>(p, batch * wide, stream);
+}
+
+}  // extern "C"

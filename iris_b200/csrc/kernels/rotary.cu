@@ -1,0 +1,281 @@
+// rotary.cu — what lies between the projection of queries, keys and values and the attention, in one pass over its output:
+// a norm of every query and key head, the rotation by the token's position, and the keys' and values' way into a paged cache.
+//
+//   y = x * rsqrt(mean(x^2) + eps) * w                      (per head of q and k, w per component; or y = x)
+//   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin)    for each pair (a, b) of the first `rotary` components, with the
+//                                                           angle of the token's position and the pair
+//   cache[slot] = rotated k, v
+//
+// Pairs are (i, i + rotary / 2) or, interleaved, (2 i, 2 i + 1).  cos and sin come from a table in fp32 (a row per position:
+// rotary / 2 cosines, then the sines), so that far positions lose nothing; arithmetic is fp32 with one rounding at the end.
+// No counterpart in the reference.
+//
+// HBM bounds it: every element is read once and written once (keys and values twice, with a cache).  A lane takes 16 components
+// of a head, the two 8-component pieces whose components are each other's partners, so that neither rotation nor norm needs more
+// than the registers and a few shuffles; the lanes of a token keep their cosines and sines and take several of its heads, whose
+// loads are all under way before the first is used.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include "iris/iris.cuh"
+#include "iris/ptx_sm100.cuh"
+
+namespace iris {
+namespace rotary {
+
+using namespace iris::ptx;
+
+constexpr int kThreads = 256;
+constexpr int kHeads = 4;                // heads of a lane
+constexpr uint32_t kSitePosition = 96, kSiteSlot = 97;
+
+struct Params {
+  const uint8_t* qkv;        // pitches in bytes
+  uint8_t* out;
+  const int* positions;
+  const float* table;
+  const uint8_t* q_weight;   // null: no norm
+  const uint8_t* k_weight;
+  uint8_t* k_cache;          // null: no cache
+  uint8_t* v_cache;
+  const int* slots;
+  StatusBlock* status;
+  int64_t ld_in, ld_out, ld_table, page_pitch, slot_pitch, head_pitch, cache_slots;
+  int positions_in_table, heads, kv_heads, dim, half, page_shift;
+  int out_heads;             // heads written to out: all, those of q and k (in place), or those of q
+  float eps;
+};
+
+template <bool F16>
+__device__ __forceinline__ void unpack8(uint4 v, float* f) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = F16 ? __half22float2(*reinterpret_cast<const __half2*>(w + i))
+                         : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(w + i));
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+template <bool F16>
+__device__ __forceinline__ uint4 pack8(const float* f) {
+  uint4 o;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (F16) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return o;
+}
+
+// LANES: lanes of a head, the power of two from dim / 16 on.  Block (x, y): token x, heads y * kThreads / LANES * kHeads on.
+template <int LANES, bool F16, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ Params p) {
+  constexpr int kGroups = kThreads / LANES;
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int64_t token = blockIdx.x;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int head0 = blockIdx.y * kGroups * kHeads + group;
+  const int all = p.heads + 2 * p.kv_heads;
+  const bool live = lane * 16 < p.dim;                   // (a dimension that is no power of two)
+  const bool turns = lane * 8 < p.half;
+  // this lane's two pieces: partners of one another where it turns them, neighbours elsewhere
+  const int c0 = turns && !INTERLEAVED ? lane * 8 : lane * 16;
+  const int c1 = turns && !INTERLEAVED ? c0 + p.half : c0 + 8;
+
+  uint4 x[kHeads][2];
+  const uint8_t* src = p.qkv + token * p.ld_in;
+#pragma unroll
+  for (int u = 0; u < kHeads; ++u) {
+    const int h = head0 + u * kGroups;
+    if (live && h < all) {
+      x[u][0] = *reinterpret_cast<const uint4*>(src + (h * p.dim + c0) * 2);
+      x[u][1] = *reinterpret_cast<const uint4*>(src + (h * p.dim + c1) * 2);
+    }
+  }
+  const int pos = p.positions[token];
+  const int slot = p.k_cache ? p.slots[token] : -1;
+  if (pos < 0) return;                                    // a row of no token
+  if (pos >= p.positions_in_table) {
+    if (threadIdx.x == 0) record_status(p.status, kBadPointer, kSitePosition, 0, (uint32_t)token, (uint64_t)pos);
+    return;
+  }
+  if (slot >= p.cache_slots && threadIdx.x == 0) record_status(p.status, kBadPointer, kSiteSlot, 0, (uint32_t)token, (uint64_t)slot);
+  const bool keep = slot >= 0 && slot < p.cache_slots;
+  const int64_t cached = keep ? (slot >> p.page_shift) * p.page_pitch + (slot & ((1 << p.page_shift) - 1)) * p.slot_pitch : 0;
+
+  float cs[8], sn[8];
+  if (turns) {
+    const float* row = p.table + pos * p.ld_table + lane * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<float4*>(cs + 4 * i) = *reinterpret_cast<const float4*>(row + 4 * i);
+      *reinterpret_cast<float4*>(sn + 4 * i) = *reinterpret_cast<const float4*>(row + p.half + 4 * i);
+    }
+  }
+  uint8_t* dst = p.out + token * p.ld_out;
+#pragma unroll
+  for (int u = 0; u < kHeads; ++u) {
+    const int h = head0 + u * kGroups;
+    if (h >= all) break;                                  // (the same for all lanes of a head)
+    if (h < p.heads + p.kv_heads) {
+      float a[8], b[8];
+      if (live) {
+        unpack8<F16>(x[u][0], a);
+        unpack8<F16>(x[u][1], b);
+      }
+      const uint8_t* weight = h < p.heads ? p.q_weight : p.k_weight;
+      if (weight) {
+        float ss = 0.f;
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+        }
+        // (the groups of a warp may have left the loop at different heads)
+        const uint32_t lanes = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << (threadIdx.x & 31 & ~(LANES - 1));
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(lanes, ss, o);
+        const float scale = rsqrtf(ss / (float)p.dim + p.eps);
+        if (live) {
+          float w[8];
+          unpack8<F16>(*reinterpret_cast<const uint4*>(weight + c0 * 2), w);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a[i] *= scale * w[i];
+          unpack8<F16>(*reinterpret_cast<const uint4*>(weight + c1 * 2), w);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b[i] *= scale * w[i];
+        }
+      }
+      if (turns) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (INTERLEAVED) {
+            float* f = i < 4 ? a + 2 * i : b + 2 * i - 8;
+            const float e = f[0], d = f[1];
+            f[0] = e * cs[i] - d * sn[i];
+            f[1] = d * cs[i] + e * sn[i];
+          } else {
+            const float e = a[i], d = b[i];
+            a[i] = e * cs[i] - d * sn[i];
+            b[i] = d * cs[i] + e * sn[i];
+          }
+        }
+      }
+      if (live) {
+        x[u][0] = pack8<F16>(a);
+        x[u][1] = pack8<F16>(b);
+      }
+    }
+    if (!live) continue;
+    if (h < p.out_heads) {
+      *reinterpret_cast<uint4*>(dst + (h * p.dim + c0) * 2) = x[u][0];
+      *reinterpret_cast<uint4*>(dst + (h * p.dim + c1) * 2) = x[u][1];
+    }
+    if (keep && h >= p.heads) {
+      const bool key = h < p.heads + p.kv_heads;
+      uint8_t* to = (key ? p.k_cache : p.v_cache) + cached + (h - p.heads - (key ? 0 : p.kv_heads)) * p.head_pitch;
+      *reinterpret_cast<uint4*>(to + c0 * 2) = x[u][0];
+      *reinterpret_cast<uint4*>(to + c1 * 2) = x[u][1];
+    }
+  }
+}
+
+thread_local char g_err[256] = "";
+
+int refuse(const char* what) {
+  snprintf(g_err, sizeof(g_err), "%s", what);
+  return -1;
+}
+
+template <int LANES>
+cudaError_t launch(const Params& p, int64_t tokens, int f16, int interleaved, void* stream) {
+  constexpr int kBlockHeads = kThreads / LANES * kHeads;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)tokens, (p.heads + 2 * p.kv_heads + kBlockHeads - 1) / kBlockHeads);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return f16 ? interleaved ? cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, true, true>, p)
+                           : cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, true, false>, p)
+             : interleaved ? cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, false, true>, p)
+                           : cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, false, false>, p);
+}
+
+}  // namespace rotary
+}  // namespace iris
+
+extern "C" {
+
+const char* iris_rotary_last_error() { return iris::rotary::g_err; }
+
+// qkv [tokens, (heads + 2 kv_heads) * dim], 16-bit (dtype 0 bf16, 1 fp16); out [tokens, out_heads * dim], or qkv itself with
+// out_heads = heads + kv_heads.  table [positions_in_table, rotary] fp32; positions, slots int32 [tokens].  Pitches in elements.
+int iris_k_qk_norm_rope(const void* qkv, int64_t ld_in, void* out, int64_t ld_out, int out_heads, const void* positions,
+                        const void* table, int64_t ld_table, int64_t positions_in_table, int rotary, int interleaved,
+                        const void* q_weight, const void* k_weight, float eps, void* k_cache, void* v_cache,
+                        int64_t page_pitch, int64_t slot_pitch, int64_t head_pitch, int64_t pages, int page_size,
+                        const void* slots, int64_t tokens, int heads, int kv_heads, int dim, int dtype, void* status,
+                        void* stream) {
+  using namespace iris::rotary;
+  g_err[0] = 0;
+  if (tokens < 1 || tokens > 0x7fffffff || heads < 1 || kv_heads < 1 || heads > 65536 || kv_heads > 65536) return refuse("sizes out of range");
+  if (dim < 16 || dim > 512 || dim % 16) return refuse("head dimension must be a multiple of 16, at most 512");
+  if (rotary < 0 || rotary > dim || rotary % 16) return refuse("rotated part must be a multiple of 16 within the head");
+  if (dtype != 0 && dtype != 1) return refuse("dtype must be 0 (bf16) or 1 (fp16)");
+  if (k_cache && (page_size < 1 || (page_size & (page_size - 1)) || pages < 1)) return refuse("page size must be a power of two");
+  // a pitch along one element says nothing
+  if (tokens == 1) ld_in = ld_out = 0;
+  if (positions_in_table == 1) ld_table = 0;
+  if (pages == 1) page_pitch = 0;
+  if (page_size == 1) slot_pitch = 0;
+  if (kv_heads == 1) head_pitch = 0;
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(table) |
+                          reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight) |
+                          reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache);
+  if (bases % 16 || (ld_in | ld_out) % 8 || ld_table % 4 || (k_cache && (page_pitch | slot_pitch | head_pitch) % 8))
+    return refuse("rows must start on 16 bytes");
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.qkv = static_cast<const uint8_t*>(qkv);
+  p.out = static_cast<uint8_t*>(out);
+  p.positions = static_cast<const int*>(positions);
+  p.table = static_cast<const float*>(table);
+  p.q_weight = static_cast<const uint8_t*>(q_weight);
+  p.k_weight = static_cast<const uint8_t*>(k_weight);
+  p.k_cache = static_cast<uint8_t*>(k_cache);
+  p.v_cache = static_cast<uint8_t*>(v_cache);
+  p.slots = static_cast<const int*>(slots);
+  p.status = static_cast<iris::StatusBlock*>(status);
+  p.ld_in = ld_in * 2, p.ld_out = ld_out * 2, p.ld_table = ld_table;
+  p.page_pitch = page_pitch * 2, p.slot_pitch = slot_pitch * 2, p.head_pitch = head_pitch * 2;
+  p.cache_slots = k_cache ? pages * page_size : 0;
+  p.positions_in_table = positions_in_table > 0x7fffffff ? 0x7fffffff : (int)positions_in_table;
+  p.heads = heads, p.kv_heads = kv_heads, p.dim = dim, p.half = rotary / 2, p.out_heads = out_heads, p.eps = eps;
+  while (k_cache && (1 << p.page_shift) < page_size) ++p.page_shift;
+  const int pieces = dim / 16;
+  const cudaError_t e = pieces <= 4    ? launch<4>(p, tokens, dtype, interleaved, stream)
+                        : pieces <= 8  ? launch<8>(p, tokens, dtype, interleaved, stream)
+                        : pieces <= 16 ? launch<16>(p, tokens, dtype, interleaved, stream)
+                                       : launch<32>(p, tokens, dtype, interleaved, stream);
+  if (e == cudaSuccess) return 0;
+  (void)cudaGetLastError();   // reported here: it must not turn up at someone else's launch
+  snprintf(g_err, sizeof(g_err), "launch: %s", cudaGetErrorString(e));
+  return -3;
+}
+
+}  // extern "C"

@@ -1,0 +1,244 @@
+"""A paged key-value cache: its pages (:class:`PagedCache`), their bookkeeping on the GPU (:func:`reserve_slots`,
+:func:`release_slots`, ``csrc/kernels/paged_cache.cu``) and the attention of one new token per sequence over them
+(:func:`paged_attention`, ``csrc/kernels/paged_attention.cu``).
+
+Nothing here waits for the GPU: which pages a request holds, how long it is and how many pages are free live on the device, so
+a decode step, the taking of new pages included, can be recorded into a CUDA graph and replayed
+(``TPDecoder.capture``).  No counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from .. import _native
+
+_DT = {torch.bfloat16: 0, torch.float16: 1}
+_P, _L, _I, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+_ATTENTION = [_P, _L, _L, _P, _P, _L, _L, _L, _L, _I, _I, _P, _L, _L, _P, _P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _I, _F, _L, _I,
+              _P, _L, _P, _I, _P]
+_RESERVE = [_P, _P, _P, _L, _L, _P, _L, _P, _I, _L, _P, _P, _L, _L, _P, _P, _P]
+_RELEASE = [_P, _P, _P, _L, _L, _P, _L, _P, _I, _L, _P]
+
+
+def _ints(t: torch.Tensor, name: str, shape) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be int32 {list(shape)} with contiguous rows, got {t.dtype} {list(t.shape)}")
+    return t
+
+
+def same_strides(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one shape are laid out alike (along one element, a stride says nothing)."""
+    return a.stride() == b.stride() or all(x == y or n < 2 for x, y, n in zip(a.stride(), b.stride(), a.shape))
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    lens: torch.Tensor, out: torch.Tensor, *, window: int = 0, sinks: int = 0, scale: Optional[float] = None,
+                    lse: Optional[torch.Tensor] = None, longest: Optional[int] = None, status: Optional[torch.Tensor] = None,
+                    stream=None) -> torch.Tensor:
+    """Attention of every sequence's newest token over its cached keys and values.
+
+    ``q`` and ``out`` are ``[batch, heads, head_dim]`` (any strides with contiguous heads, e.g. the query columns of a
+    projection), ``k_cache`` / ``v_cache`` ``[pages, page_size, kv_heads, head_dim]`` with equal strides, in any order with
+    contiguous heads; ``head_dim`` 64, 128 or 256, ``page_size`` a power of two, query head ``h`` reads key head
+    ``h // (heads // kv_heads)``.  ``block_table`` int32 ``[batch, max_pages]``: key ``j`` of a sequence lies in page
+    ``block_table[b, j // page_size]``; ``lens`` int32 ``[batch]``: keys of each sequence, the newest token's included.  With
+    ``window`` the token sees the last ``window`` keys (its own among them) and the first ``sinks``.  ``scale`` defaults to
+    ``head_dim ** -0.5``.  ``lse`` fp32 ``[batch, heads]``: receives the logarithm of the softmax's sum.
+
+    A sequence of no keys gets zeros (and minus infinity in ``lse``).  Memory behind a sequence's last key is not looked at.  A
+    key whose table entry is no page is left out and recorded in ``status`` (an ``Iris`` context's status block) if that is
+    given.  ``longest``: what the lengths are expected not to exceed, where that is much less than the table's width; it is
+    for speed alone.
+    """
+    if q.dtype not in _DT or out.dtype != q.dtype or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("q, out and the cache must all be bfloat16 or all float16")
+    if q.dim() != 3 or out.shape != q.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("expected q and out [batch, heads, head_dim] and a cache [pages, page_size, kv_heads, head_dim]")
+    batch, heads, dim = q.shape
+    pages, size, kv_heads, cache_dim = k_cache.shape
+    if cache_dim != dim or kv_heads < 1 or heads < 1 or heads % kv_heads or dim not in (64, 128, 256):
+        raise ValueError(f"{heads} query heads of {dim} do not go with {kv_heads} key heads of {cache_dim} (64, 128 or 256)")
+    q_batch, q_head, q_one = q.stride()
+    out_batch, out_head, out_one = out.stride()
+    page, slot, head, one = k_cache.stride()
+    if one != 1 or q_one != 1 or out_one != 1 or not same_strides(k_cache, v_cache):
+        raise ValueError("k_cache and v_cache must have the same strides, and all heads be contiguous")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or (
+            block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError(f"block_table must be int32 [{batch}, pages of a sequence] with contiguous rows")
+    if lens.dtype != torch.int32 or lens.shape != (batch,) or (batch > 1 and lens.stride(0) != 1):
+        raise ValueError(f"lens must be contiguous int32 [{batch}]")
+    if (batch > 1 and out_batch < dim) or (heads > 1 and out_head < dim):
+        raise ValueError("rows of out must not overlap")
+    device = q.get_device()
+    same = (out.get_device() == device and k_cache.get_device() == device and v_cache.get_device() == device and
+            block_table.get_device() == device and lens.get_device() == device)
+    lse_ptr = lse_batch = 0
+    if lse is not None:
+        if lse.dtype != torch.float32 or lse.shape != (batch, heads) or (heads > 1 and lse.stride(1) != 1):
+            raise ValueError(f"lse must be fp32 [{batch}, {heads}] with contiguous rows")
+        same = same and lse.get_device() == device
+        lse_ptr, lse_batch = lse.data_ptr(), lse.stride(0)
+    if not same or (status is not None and status.get_device() != device):
+        raise ValueError("all tensors must be on one device")
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    if batch == 0:
+        return out
+    if device != _native.current_device(device):
+        with torch.cuda.device(device):
+            return paged_attention(q, k_cache, v_cache, block_table, lens, out, window=window, sinks=sinks, scale=scale, lse=lse,
+                                   longest=longest, status=status, stream=stream)
+    lib = _native.kernels()
+    fn = _native.typed(lib.iris_k_paged_attention, _ATTENTION)
+    raw = _native.current_stream(device) if stream is None else stream
+    work, bytes_ = None, 0
+    while True:
+        rc = fn(q.data_ptr(), q_batch, q_head, k_cache.data_ptr(), v_cache.data_ptr(), page, slot, head, pages, size, kv_heads,
+                block_table.data_ptr(), block_table.stride(0), block_table.shape[1], lens.data_ptr(), out.data_ptr(), out_batch,
+                out_head, lse_ptr, lse_batch, batch, heads, dim, _DT[q.dtype], window, sinks,
+                dim ** -0.5 if scale is None else scale, longest or 0, -1, 0 if work is None else work.data_ptr(), bytes_,
+                0 if status is None else status.data_ptr(), device, raw)
+        if rc <= 0 or bytes_:
+            break
+        work, bytes_ = torch.empty(rc, dtype=torch.uint8, device=q.device), rc   # sums of sequences that several CTAs share
+    if rc:
+        lib.iris_paged_attention_last_error.restype = ctypes.c_char_p
+        raise RuntimeError(lib.iris_paged_attention_last_error().decode() or f"paged attention failed ({rc})")
+    if work is not None and stream is not None and stream != _native.current_stream(device):
+        work.record_stream(torch.cuda.ExternalStream(stream, device=device))
+    return out
+
+
+def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, page_size: int, slots: torch.Tensor, positions: torch.Tensor, *,
+                  row_stride: int = 0, lens_out: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None,
+                  stream=None) -> None:
+    """Takes pages for ``new_lens[b]`` further tokens of every request ``b``, and says where those tokens go.
+
+    Request ``b`` holds ``lens[b]`` tokens in pages ``block_table[b, :]``.  In the requests' order, each takes the pages it lacks
+    from the end of the ``free_count[0]`` entries of ``free_pages``; they are written into ``block_table``.  ``slots`` and
+    ``positions`` receive, for the row of every new token, page * page_size + place in the page, and the token's position in its
+    request: with ``row_stride`` 0 the requests' tokens are packed one behind the other, else request ``b`` has rows
+    ``b * row_stride`` on.  Rows of no token get -1 in both.  ``lens_out`` / ``free_count_out`` (default: ``lens`` and
+    ``free_count``, in place) receive the new lengths and count.  ``new_lens`` below 0 count as 0.
+
+    A request for which the free pages do not last (nor for any later one that lacks a page), whose tokens do not fit its row of
+    the table, or have not enough rows, gets nothing: its length stays, its rows get -1.  All tensors int32.
+    """
+    batch = lens.shape[0] if lens.dim() == 1 else -1
+    _ints(lens, "lens", (batch,))
+    _ints(new_lens, "new_lens", (batch,))
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or (
+            block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError(f"block_table must be int32 [{batch}, pages of a request] with contiguous rows")
+    if free_pages.dim() != 1 or slots.dim() != 1:
+        raise ValueError("free_pages and slots must be 1-D")
+    _ints(free_pages, "free_pages", free_pages.shape)
+    _ints(free_count, "free_count", (1,))
+    _ints(slots, "slots", slots.shape)
+    _ints(positions, "positions", slots.shape)
+    if page_size < 1 or page_size & (page_size - 1):
+        raise ValueError("page_size must be a power of two")
+    if row_stride < 0 or slots.shape[0] < batch * row_stride:
+        raise ValueError(f"{slots.shape[0]} rows do not hold {batch} requests of {row_stride}")
+    lens_out = lens if lens_out is None else _ints(lens_out, "lens_out", (batch,))
+    free_count_out = free_count if free_count_out is None else _ints(free_count_out, "free_count_out", (1,))
+    device = lens.get_device()
+    for t in (new_lens, block_table, free_pages, free_count, slots, positions, lens_out, free_count_out):
+        if t.get_device() != device:
+            raise ValueError("all tensors must be on one device")
+    if batch == 0 or block_table.shape[1] == 0:
+        raise ValueError("no requests, or no room in the block table")
+    if device != _native.current_device(device):
+        with torch.cuda.device(device):
+            return reserve_slots(lens, new_lens, block_table, free_pages, free_count, page_size, slots, positions,
+                                 row_stride=row_stride, lens_out=lens_out, free_count_out=free_count_out, stream=stream)
+    lib = _native.kernels()
+    rc = _native.typed(lib.iris_k_reserve_slots, _RESERVE)(
+        lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, batch, slots.data_ptr(),
+        positions.data_ptr(), slots.shape[0], row_stride, lens_out.data_ptr(), free_count_out.data_ptr(),
+        _native.current_stream(device) if stream is None else stream)
+    if rc:
+        _raise(lib, "reserve_slots", rc)
+
+
+def release_slots(lens: torch.Tensor, which: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, page_size: int, *, stream=None) -> None:
+    """Gives the pages of the requests with ``which[b] != 0`` (int32) back to the end of the list of free pages; their lengths
+    become 0 and their entries of the table -1.  A request whose pages the list has no room for keeps them (that, and all later
+    ones)."""
+    batch = lens.shape[0] if lens.dim() == 1 else -1
+    _ints(lens, "lens", (batch,))
+    _ints(which, "which", (batch,))
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or (
+            block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError(f"block_table must be int32 [{batch}, pages of a request] with contiguous rows")
+    if free_pages.dim() != 1:
+        raise ValueError("free_pages must be 1-D")
+    _ints(free_pages, "free_pages", free_pages.shape)
+    _ints(free_count, "free_count", (1,))
+    if page_size < 1 or page_size & (page_size - 1):
+        raise ValueError("page_size must be a power of two")
+    device = lens.get_device()
+    for t in (which, block_table, free_pages, free_count):
+        if t.get_device() != device:
+            raise ValueError("all tensors must be on one device")
+    if batch == 0 or block_table.shape[1] == 0:
+        raise ValueError("no requests, or no room in the block table")
+    if device != _native.current_device(device):
+        with torch.cuda.device(device):
+            return release_slots(lens, which, block_table, free_pages, free_count, page_size, stream=stream)
+    lib = _native.kernels()
+    rc = _native.typed(lib.iris_k_release_slots, _RELEASE)(
+        lens.data_ptr(), which.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, batch,
+        _native.current_stream(device) if stream is None else stream)
+    if rc:
+        _raise(lib, "release_slots", rc)
+
+
+def _raise(lib, what: str, rc: int):
+    lib.iris_pages_last_error.restype = ctypes.c_char_p
+    raise RuntimeError(f"{what}: " + (lib.iris_pages_last_error().decode() or f"launch failed ({rc})"))
+
+
+class PagedCache:
+    """Keys and values of up to ``max_batch`` requests in pages that all layers share out alike: page ``i`` of the list is page
+    ``i`` in every layer.  ``k(layer)`` / ``v(layer)``: ``[pages, page_size, kv_heads, head_dim]``."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, max_batch: int, max_len: int,
+                 dtype: torch.dtype = torch.bfloat16, device=None):
+        if min(layers, pages, page_size, kv_heads, head_dim, max_batch, max_len) < 1 or page_size & (page_size - 1):
+            raise ValueError("sizes must be positive, page_size a power of two")
+        if dtype not in _DT:
+            raise TypeError("the cache holds bfloat16 or float16")
+        self.page_size = page_size
+        self.max_len = max_len
+        self.data = torch.zeros((layers, 2, pages, page_size, kv_heads, head_dim), dtype=dtype, device=device)
+        ints = dict(dtype=torch.int32, device=device)
+        self.block_table = torch.full((max_batch, math.ceil(max_len / page_size)), -1, **ints)
+        self.lens = torch.zeros(max_batch, **ints)
+        self.free_pages = torch.arange(pages - 1, -1, -1, **ints)
+        self.free_count = torch.full((1,), pages, **ints)
+
+    def k(self, layer: int) -> torch.Tensor:
+        return self.data[layer, 0]
+
+    def v(self, layer: int) -> torch.Tensor:
+        return self.data[layer, 1]
+
+    def reserve(self, new_lens: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, row_stride: int = 0,
+                stream=None) -> None:
+        """:func:`reserve_slots` on this cache's requests, lengths and free pages updated in place."""
+        reserve_slots(self.lens, new_lens, self.block_table, self.free_pages, self.free_count, self.page_size, slots, positions,
+                      row_stride=row_stride, stream=stream)
+
+    def release(self, which: torch.Tensor, stream=None) -> None:
+        """:func:`release_slots` on this cache's requests."""
+        release_slots(self.lens, which, self.block_table, self.free_pages, self.free_count, self.page_size, stream=stream)
