@@ -31,6 +31,13 @@
 // Before: one 128-row tile per CTA, two threads per row reading the scores twice, P through shared memory, O folded
 // through registers after every tile: 659 us causal, 1091 without a mask.
 //
+// Windows (WIN): a query sees the last `window` keys, its own among them, and the first `sinks` keys of its sequence.  The
+// list of key tiles of an item is then the tiles of the first keys and those from the window of its first row on; everything
+// above counts along that list, and only tiles that a border of the mask crosses are masked.  These variants also take grouped
+// heads (head h reads key head h / group) and sequences of any length: sequences are planes of a 3-D tensor map, so that rows
+// behind a sequence's end read as zeros and not as the next sequence.  Key tiles that no row sees are neither loaded nor
+// multiplied (a pair's second tile of queries multiplies one that only the first one sees).
+//
 // Every wait is bounded by timeout_ns: on expiry the CTA records a status, every role leaves its loop, tensor memory
 // is released and the kernel returns.
 #include <cuda.h>
@@ -42,6 +49,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "iris/iris.cuh"
@@ -139,6 +147,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&b);
 }
 
+// Keys that a row does not see: after `last`, or not after `before` and from `sinks` on (all counted from v[0]).
+template <int N>
+__device__ __forceinline__ void mask_window(uint32_t* v, int last, int before, int sinks) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i > last || (i <= before && i >= sinks)) v[i] = 0xff800000u;
+}
 // Scores of the keys after `row` become minus infinity.
 template <int N>
 __device__ __forceinline__ void mask_after(uint32_t* v, int row) {
@@ -159,16 +174,21 @@ struct Params {
   int group;             // heads whose items are dealt out together
   int items;
   float scale_log2;      // log2(e) / sqrt(128)
+  int kv_heads, head_group, window, sinks;   // windows only
 };
 
 // One item of the list: head `bh`, query tiles qa and qa + 1 (pair) or qa (split), n key tiles loaded, of which side A
 // uses na and side B nb (0: side B has nothing to do).
 struct Item {
   int bh, qa, n, na, nb;
+  int ns, w0;            // windows: the first ns tiles of the list are key tiles 0 .. ns - 1, then w0, w0 + 1, ...
 };
+// Key tile i of the list.
+template <bool WIN>
+__device__ __forceinline__ int listed_tile(const Item& it, int i) { return WIN && i >= it.ns ? i - it.ns + it.w0 : i; }
 
 // Item of round r of CTA c, false past the end of the list.
-template <bool SPLIT>
+template <bool SPLIT, bool WIN>
 __device__ __forceinline__ bool item_of(const Params& p, int r, Item& it) {
   const int g = gridDim.x;
   const int idx = r * g + ((r & 1) ? g - 1 - (int)blockIdx.x : (int)blockIdx.x);
@@ -180,8 +200,23 @@ __device__ __forceinline__ bool item_of(const Params& p, int r, Item& it) {
   const int rank = idx % per;
   it.bh = first + rank % hc;
   const int q = p.blocks - 1 - rank / hc;      // longest rows of work first
-  const int nq = p.seq / BQ;
-  if (SPLIT) {
+  const int nq = WIN ? (p.seq + BQ - 1) / BQ : p.seq / BQ;
+  if (WIN) {
+    it.qa = SPLIT ? q : 2 * q;
+    const int oldest = it.qa * BQ - p.window + 1;          // that the item's first row sees, but for the first keys
+    it.w0 = oldest > 0 ? oldest / BKV : 0;
+    it.ns = min((p.sinks + BKV - 1) / BKV, it.w0);
+    const int n = it.ns + it.qa - it.w0 + 1;               // up to the diagonal of the first tile of queries
+    if (SPLIT) {
+      it.n = n;
+      it.na = (n + 1) / 2;
+      it.nb = n / 2;
+    } else {
+      it.na = n;
+      it.nb = it.qa + 1 < nq ? n + 1 : 0;
+      it.n = it.nb ? n + 1 : n;
+    }
+  } else if (SPLIT) {
     it.qa = q;
     it.n = p.causal ? q + 1 : nq;
     it.na = (it.n + 1) / 2;
@@ -196,7 +231,7 @@ __device__ __forceinline__ bool item_of(const Params& p, int r, Item& it) {
   return true;
 }
 
-template <bool F16, bool SPLIT>
+template <bool F16, bool SPLIT, bool WIN>
 __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -269,10 +304,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
         *abort_flag = 1;
         ok = false;
       };
+      int plane = 0;                    // windows: the sequence
       auto load_tile = [&](uint32_t dst, int x, int y, uint32_t bar) {
         mbar_expect_tx(bar, kTileBytes);
-        tma_load_2d(dst, &p.tm, x, y, bar);
-        tma_load_2d(dst + kHalfBytes, &p.tm, x + 64, y, bar);
+        if (WIN) {
+          tma_load_3d(dst, &p.tm, x, y, plane, bar);
+          tma_load_3d(dst + kHalfBytes, &p.tm, x + 64, y, plane, bar);
+        } else {
+          tma_load_2d(dst, &p.tm, x, y, bar);
+          tma_load_2d(dst + kHalfBytes, &p.tm, x + 64, y, bar);
+        }
       };
       auto load_kv = [&](int x, int y) {
         if (!ok) return;
@@ -293,16 +334,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
       };
       Item it;
       for (int r = 0; r * (int)gridDim.x < p.items && ok; ++r) {
-        if (!item_of<SPLIT>(p, r, it)) continue;
+        if (!item_of<SPLIT, WIN>(p, r, it)) continue;
         const int b = it.bh / p.heads, h = it.bh - b * p.heads;
-        const int y0 = b * p.seq, xq = h * D, xk = (p.heads + h) * D, xv = (2 * p.heads + h) * D;
+        const int y0 = WIN ? 0 : b * p.seq, xq = h * D;
+        const int xk = WIN ? (p.heads + h / p.head_group) * D : (p.heads + h) * D;
+        const int xv = WIN ? xk + p.kv_heads * D : (2 * p.heads + h) * D;
+        plane = b;
         load_q(0, xq, y0 + it.qa * BQ);
-        load_kv(xk, y0);
+        auto key_row = [&](int i) { return y0 + listed_tile<WIN>(it, i) * BKV; };
+        load_kv(xk, key_row(0));
         if (!SPLIT && it.nb > 0) load_q(1, xq, y0 + (it.qa + 1) * BQ);
-        if (lead == 2 && it.n > 1) load_kv(xk, y0 + BKV);
+        if (lead == 2 && it.n > 1) load_kv(xk, key_row(1));
         for (int i = 0; i < it.n && ok; ++i) {
-          load_kv(xv, y0 + i * BKV);
-          if (i + lead < it.n) load_kv(xk, y0 + (i + lead) * BKV);
+          load_kv(xv, key_row(i));
+          if (i + lead < it.n) load_kv(xk, key_row(i + lead));
         }
       }
       if (*abort_flag) {   // loads in flight still write into shared memory: wait for each, bounded
@@ -365,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
       int r = 0;
       auto fetch = [&](Item& to) {
         for (; r * (int)gridDim.x < p.items; ++r)
-          if (item_of<SPLIT>(p, r, to)) {
+          if (item_of<SPLIT, WIN>(p, r, to)) {
             ++r;
             return true;
           }
@@ -458,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     Item it;
     for (int r = 0; r * (int)gridDim.x < p.items && ok; ++r) {
-      if (!item_of<SPLIT>(p, r, it)) continue;
+      if (!item_of<SPLIT, WIN>(p, r, it)) continue;
       const int n = x ? it.nb : it.na;
       if (n == 0 && !SPLIT) continue;
       const int qt = SPLIT ? it.qa : it.qa + x;
@@ -475,7 +520,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
         // its turn comes (P overwrites only the first half of the scores)
         constexpr int kKept = SPLIT ? 64 : 96;
         uint32_t v[kKept];
-        const bool diag = p.causal && (SPLIT ? 2 * j + x : j) == qt;   // keys after the query: 0 after the exponential
+        const int kt = listed_tile<WIN>(it, SPLIT ? 2 * j + x : j);
+        const bool diag = p.causal && kt == qt;                        // keys after the query: 0 after the exponential
+        // windows: a tile with the diagonal, behind it, or with the far border of some row's window; borders from its key 0
+        const int first = WIN ? (qt - kt) * BQ + row - p.window : 0, sinks = WIN ? p.sinks - kt * BKV : 0;
+        const bool border = WIN && (kt >= qt || (qt - kt + 1) * BQ - 1 >= p.window);
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};    // four chains instead of one long one
         {
           uint32_t t[128 - kKept];
@@ -484,7 +533,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
 #pragma unroll
           for (int c = 0; c < kKept; c += 32) tmem_ld_32x32b_x32(s_t + c, v + c);
           tmem_wait_ld();
-          if (diag) mask_after<128 - kKept>(t, row - kKept), mask_after<kKept>(v, row);
+          if (WIN) {
+            if (border) {
+              mask_window<128 - kKept>(t, (qt - kt) * BQ + row - kKept, first - kKept, sinks - kKept);
+              mask_window<kKept>(v, (qt - kt) * BQ + row, first, sinks);
+            }
+          } else if (diag) {
+            mask_after<128 - kKept>(t, row - kKept), mask_after<kKept>(v, row);
+          }
 #pragma unroll
           for (int i = 0; i < 128 - kKept; i += 8)
 #pragma unroll
@@ -533,7 +589,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
           if (c * 32 >= kKept) {   // into registers that are free again
             tmem_ld_32x32b_x32(s_t + c * 32, v + c * 32 % kKept);
             tmem_wait_ld();
-            if (diag) mask_after<32>(v + c * 32 % kKept, row - c * 32);
+            if (WIN) {
+              if (border) mask_window<32>(v + c * 32 % kKept, (qt - kt) * BQ + row - c * 32, first - c * 32, sinks - c * 32);
+            } else if (diag) {
+              mask_after<32>(v + c * 32 % kKept, row - c * 32);
+            }
           }
           uint32_t pk[16];
 #pragma unroll
@@ -563,7 +623,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
       const int b = it.bh / p.heads, h = it.bh - b * p.heads;
       uint8_t* orow = reinterpret_cast<uint8_t*>(p.out) +
                       ((int64_t)(b * p.seq + qt * BQ + row) * p.ldo + (int64_t)h * D) * 2;
+      const bool stored = !WIN || qt * BQ + row < p.seq;
       auto store = [&](int col, const float* f) {   // 8 columns
+        if (!stored) return;
         uint4 o;
         o.x = pack2<F16>(f[0], f[1]);
         o.y = pack2<F16>(f[2], f[3]);
@@ -711,6 +773,76 @@ bool split_keys(int batch, int seq, int heads, bool causal, int sms) {
   };
   return 1.15 * makespan(true) < makespan(false);
 }
+// The same for windows.
+bool split_window(int batch, int seq, int heads, int window, int sinks, int sms) {
+  using namespace iris::attn;
+  const long long nq = (seq + BQ - 1) / BQ, bh = (long long)batch * heads;
+  auto makespan = [&](bool split) {
+    const long long blocks = split ? nq : (nq + 1) / 2;
+    long long total = 0, longest = 0;
+    for (long long b = 0; b < blocks; ++b) {
+      const long long qa = split ? b : 2 * b, oldest = qa * BQ - window + 1, w0 = oldest > 0 ? oldest / BKV : 0;
+      const long long ns = (sinks + BKV - 1) / BKV < w0 ? (sinks + BKV - 1) / BKV : w0;
+      const long long keys = ns + qa - w0 + (split || qa + 1 == nq ? 1 : 2);
+      const long long steps = (split ? (keys + 1) / 2 : keys) + 1;
+      const long long same = w0 > (sinks + BKV - 1) / BKV && qa + 2 < nq ? (split ? nq - 1 : (nq - 1) / 2) - b : 1;   // equal blocks from here on
+      const long long n = same > 1 ? same : 1;
+      total += steps * n;
+      b += n - 1;
+      if (steps > longest) longest = steps;
+    }
+    const long long even = (total * bh + sms - 1) / sms;
+    return even > longest ? even : longest;
+  };
+  return 1.15 * makespan(true) < makespan(false);
+}
+
+// Shared-memory limits are set once per kernel and device (a bit each).
+std::atomic<uint64_t> attn_attr[8];
+
+template <class K>
+int attn_launch(iris::attn::Params& p, K kern, std::atomic<uint64_t>& allowed, int split, int query_tiles, int sms, int dev,
+                void* stream) {
+  using namespace iris::attn;
+  cudaError_t e = cudaSuccess;
+  if (dev >= 64 || !(allowed.load(std::memory_order_acquire) >> dev & 1)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    snprintf(g_attn_err, sizeof(g_attn_err), "attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    return -3;
+  }
+  p.blocks = split ? query_tiles : (query_tiles + 1) / 2;
+  // Heads dealt out together: two rounds of items, the lengths of which then add up to the same for every CTA, and whose
+  // K and V (about 300 items x 256 rows x 512 bytes = 39 MB) stay in L2 until their last item.
+  p.group = (2 * sms + p.blocks - 1) / p.blocks;
+  if ((long long)p.batch * p.heads * p.blocks > 0x7fffffffLL / 2) {
+    snprintf(g_attn_err, sizeof(g_attn_err), "attention: too many query tiles");
+    return -1;
+  }
+  p.items = p.batch * p.heads * p.blocks;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.items < sms ? p.items : sms);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see grid_dependency_wait() in the kernel
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void* args[] = {&p};
+  e = cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kern), args);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();   // reported here: it must not turn up at someone else's launch
+    snprintf(g_attn_err, sizeof(g_attn_err), "attention: launch: %s", cudaGetErrorString(e));
+    return -3;
+  }
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -772,44 +904,66 @@ int iris_k_attention_fwd(const void* qkv, int64_t ld_qkv, void* out, int64_t ldo
     return -3;
   }
   const int split = split_keys(batch, seq, heads, causal != 0, sms) ? 1 : 0;
-  auto kern = split ? (dtype ? attention_fwd_kernel<true, true> : attention_fwd_kernel<false, true>)
-                    : (dtype ? attention_fwd_kernel<true, false> : attention_fwd_kernel<false, false>);
-  static std::once_flag attr_once[4];
-  cudaError_t e = cudaSuccess;
-  std::call_once(attr_once[dtype * 2 + split], [&]() {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  });
-  if (e != cudaSuccess) {
-    snprintf(g_attn_err, sizeof(g_attn_err), "attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-    return -3;
-  }
-  p.blocks = split ? seq / BQ : (seq / BQ + 1) / 2;
-  // Heads dealt out together: two rounds of items, the lengths of which then add up to the same for every CTA, and whose
-  // K and V (about 300 items x 256 rows x 512 bytes = 39 MB) stay in L2 until their last item.
-  p.group = (2 * sms + p.blocks - 1) / p.blocks;
-  if ((long long)batch * heads * p.blocks > 0x7fffffffLL / 2) {
-    snprintf(g_attn_err, sizeof(g_attn_err), "attention: too many query tiles");
+  const auto kern = split ? (dtype ? attention_fwd_kernel<true, true, false> : attention_fwd_kernel<false, true, false>)
+                          : (dtype ? attention_fwd_kernel<true, false, false> : attention_fwd_kernel<false, false, false>);
+  return attn_launch(p, kern, attn_attr[dtype * 2 + split], split, seq / BQ, sms, dev, stream);
+}
+
+// Causal, with windows: query i of a sequence sees its keys j <= i with j > i - window or j < sinks.  qkv [batch * seq,
+// (heads + 2 * kv_heads) * 128] (Q | K | V), out [batch * seq, heads * 128]; any seq.  Otherwise as iris_k_attention_fwd.
+int iris_k_attention_window_fwd(const void* qkv, int64_t ld_qkv, void* out, int64_t ldo, int batch, int seq, int heads,
+                                int kv_heads, int window, int sinks, int dtype, void* status, uint64_t timeout_ns,
+                                void* stream) {
+  using namespace iris::attn;
+  g_attn_err[0] = 0;
+  auto refuse = [](const char* what) {
+    snprintf(g_attn_err, sizeof(g_attn_err), "attention: %s", what);
     return -1;
+  };
+  if (!qkv || !out || batch < 1 || seq < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads)
+    return refuse("need buffers, sequences, and query heads that are a multiple of the key heads");
+  if (window < 1 || sinks < 0) return refuse("a window has at least one key, the number of first keys is not negative");
+  if (batch == 1 && seq == 1) ld_qkv = (heads + 2ll * kv_heads) * D, ldo = (int64_t)heads * D;   // a pitch of one row says nothing
+  if (reinterpret_cast<uintptr_t>(qkv) % 16 || reinterpret_cast<uintptr_t>(out) % 16 || (ld_qkv * 2) % 16 || (ldo * 2) % 16 ||
+      ld_qkv < (heads + 2ll * kv_heads) * D || ldo < (int64_t)heads * D)
+    return refuse("16-byte aligned buffers and pitches of at least the row");
+  if (dtype != 0 && dtype != 1) return refuse("dtype must be 0 (bf16) or 1 (fp16)");
+  if ((heads + 2ll * kv_heads) * D > 0x7fffffffLL) return refuse("too many heads");
+  const EncodeTiledFn enc = attn_encode_fn();
+  if (!enc) return refuse("cuTensorMapEncodeTiled is not available") - 1;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  cuuint64_t dims[3] = {(cuuint64_t)(heads + 2 * kv_heads) * D, (cuuint64_t)seq, (cuuint64_t)batch};
+  cuuint64_t strides[2] = {(cuuint64_t)ld_qkv * 2, (cuuint64_t)ld_qkv * 2 * seq};
+  cuuint32_t box[3] = {64, 128, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(&p.tm, dtype ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                         const_cast<void*>(qkv), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    snprintf(g_attn_err, sizeof(g_attn_err), "attention: cuTensorMapEncodeTiled failed with %d", (int)r);
+    return -2;
   }
-  p.items = batch * heads * p.blocks;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.items < sms ? p.items : sms);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see grid_dependency_wait() in the kernel
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  void* args[] = {&p};
-  e = cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kern), args);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();   // reported here: it must not turn up at someone else's launch
-    snprintf(g_attn_err, sizeof(g_attn_err), "attention: launch: %s", cudaGetErrorString(e));
-    return -3;
+  p.out = out;
+  p.ldo = ldo;
+  p.status = static_cast<iris::StatusBlock*>(status);
+  p.timeout_ns = timeout_ns ? timeout_ns : 2000000000ull;
+  p.batch = batch, p.seq = seq, p.heads = heads;
+  p.causal = 1;
+  p.kv_heads = kv_heads, p.head_group = heads / kv_heads;
+  p.window = window < seq ? window : seq;
+  p.sinks = sinks < seq ? sinks : seq;
+  p.scale_log2 = 1.4426950408889634f / 11.313708498984761f;   // log2(e) / sqrt(128)
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) {
+    (void)cudaGetLastError();
+    return refuse("no device") - 2;
   }
-  return 0;
+  const int split = split_window(batch, seq, heads, p.window, p.sinks, sms) ? 1 : 0;
+  const auto kern = split ? (dtype ? attention_fwd_kernel<true, true, true> : attention_fwd_kernel<false, true, true>)
+                          : (dtype ? attention_fwd_kernel<true, false, true> : attention_fwd_kernel<false, false, true>);
+  return attn_launch(p, kern, attn_attr[4 + dtype * 2 + split], split, (seq + BQ - 1) / BQ, sms, dev, stream);
 }
 
 }  // extern "C"

@@ -1,4 +1,5 @@
-"""Self-attention forward on the tcgen05 kernel of ``csrc/kernels/attention.cu`` (head dimension 128, bf16 / fp16).
+"""Self-attention forward on the tcgen05 kernel of ``csrc/kernels/attention.cu`` (head dimension 128, bf16 / fp16): causal or
+full, and causal with a sliding window and first keys that stay visible.
 
 No counterpart in the reference, which has no model code; the tensor-parallel decoder block
 (``iris_b200/models/tp_block.py``) uses it for the attention core between its fused all-gather -> GEMM (which produces
@@ -40,6 +41,55 @@ def attention_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: int, he
     st = _native.current_stream(qkv.get_device()) if stream is None else stream
     rc = fn(qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), batch, seq, heads, int(bool(causal)),
             _DT[qkv.dtype], status.data_ptr() if status is not None else 0, int(timeout_ms * 1e6), st)
+    if rc != 0:
+        lib.iris_attention_last_error.restype = ctypes.c_char_p
+        raise RuntimeError(lib.iris_attention_last_error().decode() or f"attention launch failed ({rc})")
+    return out
+
+
+_WINDOW_ARGTYPES = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_int] * 7 + \
+    [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]
+
+
+def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: int, heads: int, kv_heads: Optional[int] = None, *,
+                         window: int, sinks: int = 0, status: Optional[torch.Tensor] = None, timeout_ms: float = 2000.0,
+                         stream=None) -> torch.Tensor:
+    """Causal self-attention in which query ``i`` of a sequence sees its keys ``j <= i`` with ``j > i - window`` or
+    ``j < sinks`` (``window >= seq``: all of them); :func:`iris_b200.ops.paged.paged_attention` is the form for one new token.
+
+    ``qkv`` is ``[batch * seq, (heads + 2 * kv_heads) * 128]`` with the Q, K and V column blocks side by side, query head ``h``
+    reading key head ``h // (heads // kv_heads)``; ``out`` is ``[batch * seq, heads * 128]``; rows may be strided views.
+    ``seq``: any length.  ``status``: as for :func:`attention_fwd`.  A masked key weighs exactly nothing; a masked *value* that
+    is infinite or NaN still reaches the queries of its sequence whose window shares its tile of 128 keys (zero times it), so
+    the rows of padding have to be finite.
+    """
+    kv_heads = heads if kv_heads is None else kv_heads
+    if qkv.dtype not in _DT or out.dtype != qkv.dtype:
+        raise TypeError("qkv and out must both be bfloat16 or both float16")
+    if qkv.dim() != 2 or out.dim() != 2 or qkv.stride(1) != 1 or out.stride(1) != 1:
+        raise ValueError("qkv and out must be 2-D with contiguous rows")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("query heads must be a multiple of key heads")
+    if batch < 0 or seq < 0 or qkv.shape != (batch * seq, (heads + 2 * kv_heads) * HEAD_DIM) or \
+            out.shape != (batch * seq, heads * HEAD_DIM):
+        raise ValueError(f"expected qkv [{batch * seq}, {(heads + 2 * kv_heads) * HEAD_DIM}] and out [{batch * seq}, "
+                         f"{heads * HEAD_DIM}], got {tuple(qkv.shape)} and {tuple(out.shape)}")
+    if window < 1 or sinks < 0:
+        raise ValueError("a window has at least one key, the number of first keys is not negative")
+    device = qkv.get_device()
+    if out.get_device() != device or (status is not None and status.get_device() != device):
+        raise ValueError("all tensors must be on one device")
+    if batch * seq == 0:
+        return out
+    if device != _native.current_device(device):
+        with torch.cuda.device(device):
+            return attention_window_fwd(qkv, out, batch, seq, heads, kv_heads, window=window, sinks=sinks, status=status,
+                                        timeout_ms=timeout_ms, stream=stream)
+    lib = _native.kernels()
+    fn = _native.typed(lib.iris_k_attention_window_fwd, _WINDOW_ARGTYPES)
+    rc = fn(qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), batch, seq, heads, kv_heads, min(window, seq),
+            min(sinks, seq), _DT[qkv.dtype], status.data_ptr() if status is not None else 0, int(timeout_ms * 1e6),
+            _native.current_stream(device) if stream is None else stream)
     if rc != 0:
         lib.iris_attention_last_error.restype = ctypes.c_char_p
         raise RuntimeError(lib.iris_attention_last_error().decode() or f"attention launch failed ({rc})")

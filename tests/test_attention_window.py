@@ -1,0 +1,169 @@
+"""Attention with a sliding window and first keys that stay visible against softmax(Q K^T / sqrt(d)) V in 64 bits."""
+import pytest
+import torch
+
+from iris_b200.ops import attention as A
+
+gpu = pytest.mark.gpu
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}   # half a step of a rounding, relative
+
+
+def _inputs(batch, seq, heads, kv, dtype, seed=0, device="cuda"):
+    g = torch.Generator().manual_seed(seed + seq + heads)
+    width = (heads + 2 * kv) * 128
+    qkv = torch.randn((batch * seq, width + 64), generator=g).to(device, dtype)[:, 32:32 + width]
+    whole = torch.full((batch * seq + 3, heads * 128 + 16), float("nan"), dtype=dtype, device=device)
+    return qkv, whole, whole[:batch * seq, 8:8 + heads * 128]
+
+
+def _seen(seq, window, sinks):
+    i, j = torch.arange(seq, device="cuda")[:, None], torch.arange(seq, device="cuda")
+    return (j <= i) & ((j > i - window) | (j < sinks))
+
+
+def _check(qkv, out, batch, seq, heads, kv, window, sinks):
+    """The weights and the output are rounded to 16 bits once each: a weight by half a step of its own, which the values of the
+    keys that are seen turn into at most that times their largest magnitude; ex2.approx (2 ulp), scores (129 additions in fp32
+    of magnitudes of up to |q||k|, 2^-24 each) and sums are 5 % of that for bf16, and 2^-13 of it besides for fp16."""
+    half, group = HALF[qkv.dtype], heads // kv
+    x = qkv.double().view(batch, seq, heads + 2 * kv, 128)
+    seen = _seen(seq, window, sinks)
+    for b in range(batch):
+        for h in range(heads):
+            q, k, v = x[b, :, h], x[b, :, heads + h // group], x[b, :, heads + kv + h // group]
+            s = (q @ k.T / 128 ** 0.5).masked_fill(~seen, float("-inf"))
+            ref = torch.softmax(s, 1) @ v
+            v_max = torch.stack([v[seen[i]].abs().max() for i in range(seq)]) if seq <= 200 else v.abs().max().expand(seq)
+            tol = half * ref.abs() + ((1.05 * half + 2.0 ** -13) * v_max)[:, None]
+            err = (out.view(batch, seq, heads, 128)[b, :, h].double() - ref).abs()
+            assert bool((err <= tol).all()), f"batch {b} head {h}: {(err / tol).max().item()} of the tolerance"
+
+
+def _run(batch, seq, heads, kv, window, sinks, dtype):
+    qkv, whole, out = _inputs(batch, seq, heads, kv, dtype)
+    status = torch.zeros(16, dtype=torch.int32, device="cuda")
+    A.attention_window_fwd(qkv, out, batch, seq, heads, kv, window=window, sinks=sinks, status=status)
+    torch.cuda.synchronize()
+    assert int(status[0]) == 0, f"a wait of the kernel ran out: {status[:8].tolist()}"
+    rest = whole.clone()
+    rest[:batch * seq, 8:8 + heads * 128] = float("nan")
+    assert bool(torch.isnan(rest.float()).all()), "wrote outside the output"
+    return qkv, out
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("seq", [1, 2, 77, 127, 128, 129, 256, 300, 640])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (33, 0), (128, 4), (129, 130), (200, 300), (5000, 0)])
+def test_lengths_and_windows(seq, window, sinks, dtype):
+    """Few heads: the keys of a tile of queries are shared out."""
+    _check(*_run(2, seq, 3, 1, window, sinks, dtype), 2, seq, 3, 1, window, sinks)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("batch,seq,heads,kv", [(3, 640, 40, 40), (2, 1000, 40, 8), (1, 1300, 64, 2), (9, 129, 80, 80), (70, 77, 10, 5)])
+@pytest.mark.parametrize("window,sinks", [(100, 0), (256, 4), (300, 200), (9999, 0)])
+def test_many_heads(batch, seq, heads, kv, window, sinks, dtype):
+    """Pairs of query tiles, several items per CTA, an odd number of tiles, grouped heads."""
+    qkv, out = _run(batch, seq, heads, kv, window, sinks, dtype)
+    x, o = qkv.view(batch, seq, -1), out.view(batch, seq, -1)
+    for b in {0, batch - 1}:
+        for h in {0, heads // 2, heads - 1}:                # one head at a time
+            g = h // (heads // kv)
+            part = torch.cat([x[b, :, n * 128:(n + 1) * 128] for n in (h, heads + g, heads + kv + g)], 1)
+            _check(part, o[b, :, h * 128:(h + 1) * 128], 1, seq, 1, 1, window, sinks)
+
+
+@gpu
+@pytest.mark.parametrize("batch,seq,heads", [(1, 512, 2), (2, 1024, 40)])
+def test_a_window_of_all_keys_is_causal_attention(batch, seq, heads):
+    qkv, _, out = _inputs(batch, seq, heads, heads, torch.bfloat16)
+    want = torch.empty_like(out)
+    A.attention_fwd(qkv, want, batch, seq, heads)
+    A.attention_window_fwd(qkv, out, batch, seq, heads, window=seq)
+    assert torch.equal(out, want)
+
+
+@gpu
+@pytest.mark.parametrize("batch,heads", [(1, 2), (2, 60)])   # keys of a query tile shared out; pairs of query tiles
+def test_hidden_keys_weigh_nothing(batch, heads):
+    """Keys and values that a query does not see reach it with no bit, whatever finite size they have; neither does the next
+    sequence, NaN and all."""
+    seq, window, sinks = 500, 70, 5
+    qkv, _, out = _inputs(batch, seq, heads, heads, torch.bfloat16)
+    A.attention_window_fwd(qkv, out, batch, seq, heads, window=window, sinks=sinks)
+    w = heads * 128
+    other, got = qkv.clone(), torch.empty_like(out)
+    x = other.view(batch, seq, 3 * w)
+    x[0, 100:130, 2 * w:] = 3.0e38
+    x[0, 100:130, w:2 * w] *= -50.0
+    if batch > 1:
+        x[1] = float("nan")
+    A.attention_window_fwd(other, got, batch, seq, heads, window=window, sinks=sinks)
+    a, b = (t.view(batch, seq, w)[0] for t in (out, got))
+    assert torch.equal(a[:100], b[:100]) and torch.equal(a[199:], b[199:])
+    assert not torch.equal(a[129:199], b[129:199])
+
+
+@gpu
+@pytest.mark.parametrize("batch,heads", [(1, 1), (2, 80)])
+def test_nan_of_a_key_reaches_the_queries_that_see_it(batch, heads):
+    seq, window, sinks, w = 400, 90, 3, heads * 128
+    for key, rows in ((200, list(range(200, 290))), (1, list(range(1, 400)))):
+        qkv, _, out = _inputs(batch, seq, heads, heads, torch.bfloat16)
+        qkv[key, w:w + 128] = float("nan")
+        A.attention_window_fwd(qkv, out, batch, seq, heads, window=window, sinks=sinks)
+        nan = torch.isnan(out.float())
+        want = torch.zeros_like(nan)
+        want[rows, :128] = True
+        assert torch.equal(nan, want)
+
+
+@gpu
+def test_in_a_graph_and_on_another_stream():
+    qkv, _, out = _inputs(2, 300, 4, 2, torch.bfloat16)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    A.attention_window_fwd(qkv, out, 2, 300, 4, 2, window=50, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    first = out.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        A.attention_window_fwd(qkv, out, 2, 300, 4, 2, window=50)
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
+    qkv.mul_(0.5)
+    g.replay()
+    torch.cuda.synchronize()
+    _check(qkv, out, 2, 300, 4, 2, 50, 0)
+
+
+@gpu
+def test_no_rows():
+    qkv, _, out = _inputs(1, 4, 2, 1, torch.bfloat16)
+    assert A.attention_window_fwd(qkv[:0], out[:0], 0, 4, 2, 1, window=4).shape == (0, 256)
+
+
+def test_refusals():
+    qkv, _, out = _inputs(2, 10, 4, 2, torch.bfloat16, device="cpu")
+    ok = dict(qkv=qkv, out=out, batch=2, seq=10, heads=4, kv_heads=2, window=4)
+    with pytest.raises(TypeError):
+        A.attention_window_fwd(**{**ok, "out": out.half()})
+    for bad in (dict(kv_heads=3), dict(kv_heads=0), dict(kv_heads=4), dict(seq=9), dict(batch=3), dict(window=0), dict(window=-1),
+                dict(sinks=-1), dict(qkv=qkv.t().contiguous().t()), dict(out=out[:, :128]), dict(qkv=qkv[None])):
+        with pytest.raises(ValueError):
+            A.attention_window_fwd(**{**ok, **bad})
+    with pytest.raises(ValueError, match="CUDA device"):
+        A.attention_window_fwd(**ok)
+
+
+@gpu
+def test_refusals_of_the_native_entry():
+    wide = torch.zeros((20, 2000), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="16-byte"):
+        A.attention_window_fwd(wide[:, 1:1025], wide[:, 1200:1712], 2, 10, 4, 2, window=4)
+    with pytest.raises(RuntimeError, match="16-byte"):
+        A.attention_window_fwd(wide[:1].expand(20, -1)[:, :1024], wide[:, 1200:1712], 2, 10, 4, 2, window=4)
