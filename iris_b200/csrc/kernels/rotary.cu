@@ -224,7 +224,7 @@ extern "C" {
 const char* iris_rotary_last_error() { return iris::rotary::g_err; }
 
 // qkv [tokens, (heads + 2 kv_heads) * dim], 16-bit (dtype 0 bf16, 1 fp16); out [tokens, out_heads * dim], or qkv itself with
-// out_heads = heads + kv_heads.  table [positions_in_table, rotary] fp32; positions, slots int32 [tokens].  Pitches in elements.
+// out_heads = heads + kv_heads.  table [positions_in_table, rotary] fp32, or null with rotary 0; positions, slots int32 [tokens].  Pitches in elements.
 int iris_k_qk_norm_rope(const void* qkv, int64_t ld_in, void* out, int64_t ld_out, int out_heads, const void* positions,
                         const void* table, int64_t ld_table, int64_t positions_in_table, int rotary, int interleaved,
                         const void* q_weight, const void* k_weight, float eps, void* k_cache, void* v_cache,
@@ -235,7 +235,7 @@ int iris_k_qk_norm_rope(const void* qkv, int64_t ld_in, void* out, int64_t ld_ou
   g_err[0] = 0;
   if (tokens < 1 || tokens > 0x7fffffff || heads < 1 || kv_heads < 1 || heads > 65536 || kv_heads > 65536) return refuse("sizes out of range");
   if (dim < 16 || dim > 512 || dim % 16) return refuse("head dimension must be a multiple of 16, at most 512");
-  if (rotary < 0 || rotary > dim || rotary % 16) return refuse("rotated part must be a multiple of 16 within the head");
+  if (rotary < 0 || rotary > dim || rotary % 16 || (rotary && !table)) return refuse("rotated part must be a multiple of 16 within the head");
   if (dtype != 0 && dtype != 1) return refuse("dtype must be 0 (bf16) or 1 (fp16)");
   if (k_cache && (page_size < 1 || (page_size & (page_size - 1)) || pages < 1)) return refuse("page size must be a power of two");
   // a pitch along one element says nothing
@@ -264,7 +264,7 @@ int iris_k_qk_norm_rope(const void* qkv, int64_t ld_in, void* out, int64_t ld_ou
   p.ld_in = ld_in * 2, p.ld_out = ld_out * 2, p.ld_table = ld_table;
   p.page_pitch = page_pitch * 2, p.slot_pitch = slot_pitch * 2, p.head_pitch = head_pitch * 2;
   p.cache_slots = k_cache ? pages * page_size : 0;
-  p.positions_in_table = positions_in_table > 0x7fffffff ? 0x7fffffff : (int)positions_in_table;
+  p.positions_in_table = !table || positions_in_table > 0x7fffffff ? 0x7fffffff : (int)positions_in_table;
   p.heads = heads, p.kv_heads = kv_heads, p.dim = dim, p.half = rotary / 2, p.out_heads = out_heads, p.eps = eps;
   while (k_cache && (1 << p.page_shift) < page_size) ++p.page_shift;
   const int pieces = dim / 16;

@@ -65,7 +65,7 @@ def _may_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
-def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, heads: int, kv_heads: int,
+def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, table: Optional[torch.Tensor], heads: int, kv_heads: int,
                  head_dim: int, *, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
                  eps: float = 1e-6, interleaved: bool = False, k_cache: Optional[torch.Tensor] = None,
                  v_cache: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
@@ -75,7 +75,7 @@ def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, 
 
     ``qkv`` is ``[tokens, (heads + 2 kv_heads) * head_dim]`` (Q | K | V column blocks; rows may be strided), ``positions`` int32
     ``[tokens]``, ``table`` a :func:`rotary_table` whose width says how much of a head is rotated (its first components; pairs
-    ``(i, i + width / 2)``, or ``(2 i, 2 i + 1)`` if ``interleaved``).  ``q_weight`` / ``k_weight`` ``[head_dim]``: the head is
+    ``(i, i + width / 2)``, or ``(2 i, 2 i + 1)`` if ``interleaved``; ``None``: nothing is).  ``q_weight`` / ``k_weight`` ``[head_dim]``: the head is
     first divided by the root of its mean square (plus ``eps``) and multiplied by the weight; ``None``: no norm.  ``out``: all
     columns like ``qkv``; ``qkv`` itself (in place); or the query columns alone.  ``k_cache`` / ``v_cache``: pages
     ``[pages, page_size, kv_heads, head_dim]`` with equal strides, in any order with contiguous heads; token ``t`` goes to slot
@@ -96,9 +96,13 @@ def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, 
     device = qkv.get_device()
     if positions.dtype != torch.int32 or positions.shape != (tokens,) or (tokens > 1 and positions.stride(0) != 1):
         raise ValueError(f"positions must be contiguous int32 [{tokens}]")
-    if table.dtype != torch.float32 or table.dim() != 2 or table.stride(1) != 1 or table.shape[1] > head_dim or table.shape[1] % 16:
-        raise ValueError("table must be fp32 [positions, rotary dimension], at most as wide as a head, a multiple of 16")
-    same = out.get_device() == device and positions.get_device() == device and table.get_device() == device
+    same = out.get_device() == device and positions.get_device() == device
+    turns = table_ptr = table_pitch = rotary = 0
+    if table is not None:
+        if table.dtype != torch.float32 or table.dim() != 2 or table.stride(1) != 1 or table.shape[1] > head_dim or table.shape[1] % 16:
+            raise ValueError("table must be fp32 [positions, rotary dimension], at most as wide as a head, a multiple of 16")
+        same = same and table.get_device() == device
+        (turns, rotary), table_ptr, table_pitch = table.shape, table.data_ptr(), table.stride(0)
     for w in (q_weight, k_weight):
         if w is not None:
             if w.dtype != qkv.dtype or w.shape != (head_dim,) or w.stride(0) != 1:
@@ -142,8 +146,8 @@ def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, 
     out_heads = heads + kv_heads if in_place and out.shape[1] == width else out.shape[1] // head_dim
     lib = _native.kernels()
     fn = _native.typed(lib.iris_k_qk_norm_rope, _ARGTYPES)
-    rc = fn(qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), out_heads, positions.data_ptr(), table.data_ptr(),
-            table.stride(0), table.shape[0], table.shape[1], 1 if interleaved else 0,
+    rc = fn(qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), out_heads, positions.data_ptr(), table_ptr,
+            table_pitch, turns, rotary, 1 if interleaved else 0,
             0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), eps, k_ptr, v_ptr,
             page, slot, head, pages, size, slots_ptr, tokens, heads, kv_heads, head_dim, _DT[qkv.dtype],
             0 if status is None else status.data_ptr(), _native.current_stream(device) if stream is None else stream)

@@ -185,6 +185,18 @@ def test_in_a_graph_and_on_another_stream():
 
 
 @gpu
+@pytest.mark.parametrize("norm", [True, False])
+def test_without_rotation(norm):
+    """No table: norms and cache writes alone, positions as large as they come; nothing at all to do leaves every bit."""
+    c = Case(70, 4, 2, 128, 128, torch.bfloat16, norm)
+    c.table = torch.cat([torch.ones(500, 64), torch.zeros(500, 64)], 1).cuda()      # for the comparison: angles of zero
+    pos = c.pos + 2000000000
+    R.qk_norm_rope(c.qkv, c.out, pos, None, 4, 2, 128, **c.kw(), **c.cache())
+    c.check()
+    assert norm or torch.equal(c.out, c.qkv)
+
+
+@gpu
 def test_no_tokens():
     c = Case(4, 2, 1, 64, 64, torch.bfloat16)
     out = c.out[:0]

@@ -1,0 +1,130 @@
+"""The decoder with positions, head norms, grouped heads and windows against the unsharded fp32 oracle: whole sequences, and the
+same sequences as prompts followed by single tokens over a paged cache."""
+import pytest
+import torch
+
+import iris_b200 as iris
+from iris_b200.models.tp_block import TPConfig, TPDecoder, TPDecoderBaseline, reference_forward
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+SIZES = dict(hidden=512, n_heads=4, head_dim=128, intermediate=1024, n_layers=2, seed=4)
+KINDS = {
+    "plain": dict(),
+    "grouped": dict(n_kv_heads=2, rope_theta=10000.0, qk_norm=True),
+    "window": dict(rope_theta=10000.0, window=50, sinks=3),
+    "part": dict(n_kv_heads=2, rope_theta=10000.0, rotary_dim=32, interleaved=True, window=9),
+}
+
+
+def _inputs(batch, seq, hidden=512):
+    g = torch.Generator(device="cuda").manual_seed(batch + seq)
+    return torch.randn((batch, seq, hidden), generator=g, device="cuda").to(torch.bfloat16)
+
+
+def _near(got, ref):
+    """Bounds of tests/test_gpu_tp_block.py for the same depth and width."""
+    err = (got.float() - ref).abs()
+    assert err.mean().item() < 2e-2 and err.max().item() < 0.25, (err.mean().item(), err.max().item())
+
+
+@pytest.mark.parametrize("world", [1, 2])
+@pytest.mark.parametrize("kind", ["grouped", "window", "part"])
+def test_whole_sequences(kind, world):
+    batch, seq = 4, 192 if kind != "grouped" else 256      # (with peers, a rank has a multiple of 128 rows)
+    cfg = TPConfig(batch=batch, seq=seq, **SIZES, **KINDS[kind])
+    ranks = iris.Iris.local_world(world, heap_size=192 << 20)
+    model = TPDecoder(ranks, cfg)
+    x = _inputs(batch, seq).view(batch * seq, -1)
+    ts = cfg.tokens // world
+    shards = [x[r * ts:(r + 1) * ts].clone() for r in range(world)]
+    model.forward(shards)
+    model.check()
+    _near(torch.cat(shards, 0), reference_forward(x, cfg))
+    model.close()
+    ranks[0].close()
+
+
+@pytest.mark.parametrize("world,kind,batch,seq,steps", [
+    (1, "plain", 4, 96, 40), (1, "grouped", 4, 96, 40), (1, "window", 4, 96, 40), (1, "part", 5, 77, 40), (2, "grouped", 256, 8, 30)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_prompts_then_single_tokens(kind, world, batch, seq, steps, graph):
+    """Prompts of several lengths, one of them empty, then tokens one by one, a request that pauses, one that ends and whose
+    pages another gets: every row is the oracle's for the whole sequence."""
+    more = dict(SIZES, **KINDS[kind], positions=seq + steps)
+    pre, one = TPConfig(batch=batch, seq=seq, **more), TPConfig(batch=batch, seq=1, **more)
+    whole = TPConfig(batch=batch, seq=seq + steps, **more)
+    ranks = iris.Iris.local_world(world, heap_size=192 << 20)
+    prefill = TPDecoder(ranks, pre)
+    decode = TPDecoder(ranks, one, weights=prefill)
+    cache = prefill.make_cache(pages=batch * -(-(seq + steps) // 16), page_size=16, max_batch=batch, max_len=seq + steps)
+    x = _inputs(batch, seq + steps)
+    want = reference_forward(x.view(-1, 512), whole).view(batch, seq + steps, 512)
+    lens = [(seq, 17, 0, 50)[b % 4] % (seq + 1) for b in range(batch)]
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+
+    def run(model, rows, new):
+        n = rows.shape[0] // world
+        shards = [rows[r * n:(r + 1) * n].clone() for r in range(world)]
+        model.forward(shards, cache=cache, new_lens=new)
+        model.check()
+        return torch.cat(shards, 0)
+    got = run(prefill, x[:, :seq].reshape(-1, 512), ints(lens)).view(batch, seq, 512)
+    real = torch.arange(seq) < torch.tensor(lens)[:, None]
+    _near(got[real], want[:, :seq][real])
+    new = ints([1] * batch)
+    per = batch // world
+    shards = [torch.empty((per, 512), dtype=torch.bfloat16, device="cuda") for _ in range(world)]
+    recorded = None
+    if graph:
+        before = [c.lens.clone() for c in cache], [c.free_count.clone() for c in cache], [c.block_table.clone() for c in cache]
+        for s in shards:
+            s.zero_()
+        recorded = decode.capture(shards, cache=cache, new_lens=new)
+        assert all(torch.equal(c.lens, l) and torch.equal(c.free_count, f) and torch.equal(c.block_table, t)
+                   for c, l, f, t in zip(cache, *before))
+    for step in range(steps):
+        active = [not (b % 4 == 1 and step % 5 == 2) for b in range(batch)]
+        if step == 20:                                            # request 3 ends, and begins again from its first token
+            for c in cache:
+                c.release(ints([int(b % 4 == 3) for b in range(batch)]))
+            lens = [0 if b % 4 == 3 else n for b, n in enumerate(lens)]
+        new.copy_(ints([int(a) for a in active]))
+        rows = x[torch.arange(batch), lens]
+        if graph:
+            for r, s in enumerate(shards):
+                s.copy_(rows[r * per:(r + 1) * per])
+            recorded.replay()
+            decode.check()
+            out = torch.cat(shards, 0)
+        else:
+            out = run(decode, rows, new)
+        _near(out[active], want[torch.arange(batch), lens][active])
+        lens = [n + a for n, a in zip(lens, active)]
+    assert all(c.lens.tolist() == lens for c in cache)
+    decode.close(), prefill.close()
+    ranks[0].close()
+
+
+def test_refusals():
+    ctx = iris.iris(192 << 20)
+    cfg = TPConfig(batch=2, seq=64, **SIZES, **KINDS["grouped"])
+    model = TPDecoder(ctx, cfg)
+    x = [torch.zeros((128, 512), dtype=torch.bfloat16, device="cuda")]
+    new = torch.ones(2, dtype=torch.int32, device="cuda")
+    for bad in (dict(new_lens=new), dict(cache=model.make_cache(4, 16, 2, 64)), dict(cache=model.make_cache(4, 16, 3, 64), new_lens=new),
+                dict(cache=model.make_cache(4, 16, 2, 65), new_lens=new), dict(cache=[], new_lens=new)):
+        with pytest.raises(ValueError):
+            model.forward(x, **bad)
+    with pytest.raises(ValueError):
+        TPDecoder(ctx, TPConfig(batch=2, seq=64, **SIZES, n_kv_heads=3))
+    with pytest.raises(ValueError):
+        TPDecoder(ctx, TPConfig(batch=2, seq=64, **SIZES, window=8), attention="sdpa")
+    with pytest.raises(ValueError):
+        TPDecoder(ctx, TPConfig(batch=2, seq=64, **SIZES), weights=model)
+    with pytest.raises(ValueError):
+        TPDecoderBaseline(cfg, 0, 1, "cuda")
+    model.close(), ctx.close()
