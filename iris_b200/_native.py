@@ -110,6 +110,19 @@ def typed(fn, argtypes, restype=c_int):
     return fn
 
 
+_entries = {}
+
+
+def entry(name: str):
+    """The kernel library's entry point ``name`` that takes its arguments packed (one pointer to a struct, passed as bytes)."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = getattr(kernels(), name)
+        fn.argtypes, fn.restype = [c_char_p], c_int
+        _entries[name] = fn
+    return fn
+
+
 def current_stream(device_index) -> int:
     """The handle of PyTorch's current stream on CUDA device ``device_index`` (``tensor.get_device()``): what
     ``torch.cuda.current_stream(...).cuda_stream`` gives, without making the stream object (2 us, as much as a launch)."""

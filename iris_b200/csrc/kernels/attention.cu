@@ -911,16 +911,23 @@ int iris_k_attention_fwd(const void* qkv, int64_t ld_qkv, void* out, int64_t ldo
 
 // Causal, with windows: query i of a sequence sees its keys j <= i with j > i - window or j < sinks.  qkv [batch * seq,
 // (heads + 2 * kv_heads) * 128] (Q | K | V), out [batch * seq, heads * 128]; any seq.  Otherwise as iris_k_attention_fwd.
-int iris_k_attention_window_fwd(const void* qkv, int64_t ld_qkv, void* out, int64_t ldo, int batch, int seq, int heads,
-                                int kv_heads, int window, int sinks, int dtype, void* status, uint64_t timeout_ns,
-                                void* stream) {
+// The arguments of a call, packed (see paged_attention.cu).
+struct IrisAttentionWindowArgs {
+  const void* qkv;
+  void *out, *status, *stream;
+  int64_t ld_qkv, ldo, batch, seq, heads, kv_heads, window, sinks, dtype, timeout_ns;
+};
+int iris_k_attention_window_fwd(const IrisAttentionWindowArgs* args) {
   using namespace iris::attn;
   g_attn_err[0] = 0;
+  const auto [qkv, out, status, stream, ld_qkv0, ldo0, batch, seq, heads, kv_heads, window, sinks, dtype, timeout_ns] = *args;
+  int64_t ld_qkv = ld_qkv0, ldo = ldo0;
   auto refuse = [](const char* what) {
     snprintf(g_attn_err, sizeof(g_attn_err), "attention: %s", what);
     return -1;
   };
-  if (!qkv || !out || batch < 1 || seq < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads)
+  if (!qkv || !out || batch < 1 || seq < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || batch > 0x7fffffff ||
+      seq > 0x7fffffff - 256)
     return refuse("need buffers, sequences, and query heads that are a multiple of the key heads");
   if (window < 1 || sinks < 0) return refuse("a window has at least one key, the number of first keys is not negative");
   if (batch == 1 && seq == 1) ld_qkv = (heads + 2ll * kv_heads) * D, ldo = (int64_t)heads * D;   // a pitch of one row says nothing
@@ -947,23 +954,23 @@ int iris_k_attention_window_fwd(const void* qkv, int64_t ld_qkv, void* out, int6
   p.out = out;
   p.ldo = ldo;
   p.status = static_cast<iris::StatusBlock*>(status);
-  p.timeout_ns = timeout_ns ? timeout_ns : 2000000000ull;
-  p.batch = batch, p.seq = seq, p.heads = heads;
+  p.timeout_ns = timeout_ns > 0 ? (uint64_t)timeout_ns : 2000000000ull;
+  p.batch = (int)batch, p.seq = (int)seq, p.heads = (int)heads;
   p.causal = 1;
-  p.kv_heads = kv_heads, p.head_group = heads / kv_heads;
-  p.window = window < seq ? window : seq;
-  p.sinks = sinks < seq ? sinks : seq;
+  p.kv_heads = (int)kv_heads, p.head_group = (int)(heads / kv_heads);
+  p.window = (int)(window < seq ? window : seq);
+  p.sinks = (int)(sinks < seq ? sinks : seq);
   p.scale_log2 = 1.4426950408889634f / 11.313708498984761f;   // log2(e) / sqrt(128)
   int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) {
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      sms < 1) {
     (void)cudaGetLastError();
     return refuse("no device") - 2;
   }
-  const int split = split_window(batch, seq, heads, p.window, p.sinks, sms) ? 1 : 0;
+  const int split = split_window(p.batch, p.seq, p.heads, p.window, p.sinks, sms) ? 1 : 0;
   const auto kern = split ? (dtype ? attention_fwd_kernel<true, true, true> : attention_fwd_kernel<false, true, true>)
                           : (dtype ? attention_fwd_kernel<true, false, true> : attention_fwd_kernel<false, false, true>);
-  return attn_launch(p, kern, attn_attr[4 + dtype * 2 + split], split, (seq + BQ - 1) / BQ, sms, dev, stream);
+  return attn_launch(p, kern, attn_attr[4 + dtype * 2 + split], split, (p.seq + BQ - 1) / BQ, sms, dev, stream);
 }
 
 }  // extern "C"

@@ -249,15 +249,23 @@ extern "C" {
 
 const char* iris_pages_last_error() { return iris::pages::g_err; }
 
-// All arrays int32 on the current device.  table [batch, wide] with rows table_pitch apart; free [capacity], count [1].
-// slots, positions [tokens]: row_stride rows to a request, or, with row_stride 0, packed; rows of no token get -1.
-// lens_out and count_out may be lens and count.
-int iris_k_reserve_slots(const void* lens, const void* new_lens, void* table, int64_t table_pitch, int64_t wide, void* free,
-                         int64_t capacity, const void* count, int page_size, int64_t batch, void* slots, void* positions,
-                         int64_t tokens, int64_t row_stride, void* lens_out, void* count_out, void* stream) {
+// The arguments of a call, packed (see paged_attention.cu).  All arrays int32 on the current device.  table [batch, wide] with
+// rows table_pitch apart; free [capacity], count [1].  slots, positions [tokens]: row_stride rows to a request, or, with
+// row_stride 0, packed; rows of no token get -1.  lens_out and count_out may be lens and count.
+struct IrisReserveArgs {
+  const void *lens, *new_lens;
+  void *table, *free;
+  const void *count;
+  void *slots, *positions, *lens_out, *count_out, *stream;
+  int64_t table_pitch, wide, capacity, page_size, batch, tokens, row_stride;
+};
+
+int iris_k_reserve_slots(const IrisReserveArgs* args) {
   using namespace iris::pages;
   g_err[0] = 0;
-  if (page_size < 1 || (page_size & (page_size - 1))) return refuse("page size must be a power of two");
+  const auto [lens, new_lens, table, free, count, slots, positions, lens_out, count_out, stream, table_pitch, wide, capacity,
+              page_size, batch, tokens, row_stride] = *args;
+  if (page_size < 1 || (page_size & (page_size - 1)) || page_size > (1 << 30)) return refuse("page size must be a power of two");
   if (batch < 1 || batch > 0x7fffffff - kThreads || wide < 1 || wide > 0x7fffffff || capacity < 0 || capacity > 0x7fffffff || tokens < 0 || row_stride < 0)
     return refuse("sizes out of range");
   Params p;

@@ -223,21 +223,35 @@ extern "C" {
 
 const char* iris_rotary_last_error() { return iris::rotary::g_err; }
 
-// qkv [tokens, (heads + 2 kv_heads) * dim], 16-bit (dtype 0 bf16, 1 fp16); out [tokens, out_heads * dim], or qkv itself with
-// out_heads = heads + kv_heads.  table [positions_in_table, rotary] fp32, or null with rotary 0; positions, slots int32 [tokens].  Pitches in elements.
-int iris_k_qk_norm_rope(const void* qkv, int64_t ld_in, void* out, int64_t ld_out, int out_heads, const void* positions,
-                        const void* table, int64_t ld_table, int64_t positions_in_table, int rotary, int interleaved,
-                        const void* q_weight, const void* k_weight, float eps, void* k_cache, void* v_cache,
-                        int64_t page_pitch, int64_t slot_pitch, int64_t head_pitch, int64_t pages, int page_size,
-                        const void* slots, int64_t tokens, int heads, int kv_heads, int dim, int dtype, void* status,
-                        void* stream) {
+// The arguments of a call, packed (see paged_attention.cu).  qkv [tokens, (heads + 2 kv_heads) * dim], 16-bit (dtype 0 bf16,
+// 1 fp16); out [tokens, out_heads * dim], or qkv itself with out_heads = heads + kv_heads.  table [positions_in_table, rotary]
+// fp32, or null with rotary 0; positions, slots int32 [tokens].  Pitches in elements.
+struct IrisQkNormRopeArgs {
+  const void *qkv;
+  void *out;
+  const void *positions, *table, *q_weight, *k_weight;
+  void *k_cache, *v_cache;
+  const void *slots;
+  void *status, *stream;
+  int64_t ld_in, ld_out, ld_table, page_pitch, slot_pitch, head_pitch;
+  int64_t out_heads, positions_in_table, rotary, interleaved, pages, page_size, tokens, heads, kv_heads, dim, dtype;
+  double eps;
+};
+
+int iris_k_qk_norm_rope(const IrisQkNormRopeArgs* args) {
   using namespace iris::rotary;
   g_err[0] = 0;
+  const auto [qkv, out, positions, table, q_weight, k_weight, k_cache, v_cache, slots, status, stream, ld_in0, ld_out0, ld_table0,
+              page_pitch0, slot_pitch0, head_pitch0, out_heads, positions_in_table, rotary, interleaved, pages, page_size, tokens,
+              heads, kv_heads, dim, dtype, eps] = *args;
+  int64_t ld_in = ld_in0, ld_out = ld_out0, ld_table = ld_table0, page_pitch = page_pitch0, slot_pitch = slot_pitch0;
+  int64_t head_pitch = head_pitch0;
   if (tokens < 1 || tokens > 0x7fffffff || heads < 1 || kv_heads < 1 || heads > 65536 || kv_heads > 65536) return refuse("sizes out of range");
   if (dim < 16 || dim > 512 || dim % 16) return refuse("head dimension must be a multiple of 16, at most 512");
   if (rotary < 0 || rotary > dim || rotary % 16 || (rotary && !table)) return refuse("rotated part must be a multiple of 16 within the head");
   if (dtype != 0 && dtype != 1) return refuse("dtype must be 0 (bf16) or 1 (fp16)");
-  if (k_cache && (page_size < 1 || (page_size & (page_size - 1)) || pages < 1)) return refuse("page size must be a power of two");
+  if (k_cache && (page_size < 1 || (page_size & (page_size - 1)) || page_size > (1 << 30) || pages < 1 || pages > 0x7fffffff))
+    return refuse("page size must be a power of two");
   // a pitch along one element says nothing
   if (tokens == 1) ld_in = ld_out = 0;
   if (positions_in_table == 1) ld_table = 0;
@@ -265,13 +279,14 @@ int iris_k_qk_norm_rope(const void* qkv, int64_t ld_in, void* out, int64_t ld_ou
   p.page_pitch = page_pitch * 2, p.slot_pitch = slot_pitch * 2, p.head_pitch = head_pitch * 2;
   p.cache_slots = k_cache ? pages * page_size : 0;
   p.positions_in_table = !table || positions_in_table > 0x7fffffff ? 0x7fffffff : (int)positions_in_table;
-  p.heads = heads, p.kv_heads = kv_heads, p.dim = dim, p.half = rotary / 2, p.out_heads = out_heads, p.eps = eps;
+  p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.dim = (int)dim, p.half = (int)rotary / 2, p.out_heads = (int)out_heads;
+  p.eps = (float)eps;
   while (k_cache && (1 << p.page_shift) < page_size) ++p.page_shift;
-  const int pieces = dim / 16;
-  const cudaError_t e = pieces <= 4    ? launch<4>(p, tokens, dtype, interleaved, stream)
-                        : pieces <= 8  ? launch<8>(p, tokens, dtype, interleaved, stream)
-                        : pieces <= 16 ? launch<16>(p, tokens, dtype, interleaved, stream)
-                                       : launch<32>(p, tokens, dtype, interleaved, stream);
+  const int pieces = (int)dim / 16;
+  const cudaError_t e = pieces <= 4    ? launch<4>(p, tokens, (int)dtype, (int)interleaved, stream)
+                        : pieces <= 8  ? launch<8>(p, tokens, (int)dtype, (int)interleaved, stream)
+                        : pieces <= 16 ? launch<16>(p, tokens, (int)dtype, (int)interleaved, stream)
+                                       : launch<32>(p, tokens, (int)dtype, (int)interleaved, stream);
   if (e == cudaSuccess) return 0;
   (void)cudaGetLastError();   // reported here: it must not turn up at someone else's launch
   snprintf(g_err, sizeof(g_err), "launch: %s", cudaGetErrorString(e));

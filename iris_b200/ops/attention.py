@@ -8,6 +8,7 @@ No counterpart in the reference, which has no model code; the tensor-parallel de
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -47,8 +48,7 @@ def attention_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: int, he
     return out
 
 
-_WINDOW_ARGTYPES = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_int] * 7 + \
-    [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]
+_WINDOW_ARGS = struct.Struct("@14q")
 
 
 def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: int, heads: int, kv_heads: Optional[int] = None, *,
@@ -64,16 +64,18 @@ def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: 
     the rows of padding have to be finite.
     """
     kv_heads = heads if kv_heads is None else kv_heads
-    if qkv.dtype not in _DT or out.dtype != qkv.dtype:
+    dtype, shape = qkv.dtype, qkv.shape
+    if dtype not in _DT or out.dtype is not dtype:
         raise TypeError("qkv and out must both be bfloat16 or both float16")
-    if qkv.dim() != 2 or out.dim() != 2 or qkv.stride(1) != 1 or out.stride(1) != 1:
-        raise ValueError("qkv and out must be 2-D with contiguous rows")
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError("query heads must be a multiple of key heads")
-    if batch < 0 or seq < 0 or qkv.shape != (batch * seq, (heads + 2 * kv_heads) * HEAD_DIM) or \
+    if batch < 0 or seq < 0 or shape != (batch * seq, (heads + 2 * kv_heads) * HEAD_DIM) or \
             out.shape != (batch * seq, heads * HEAD_DIM):
         raise ValueError(f"expected qkv [{batch * seq}, {(heads + 2 * kv_heads) * HEAD_DIM}] and out [{batch * seq}, "
-                         f"{heads * HEAD_DIM}], got {tuple(qkv.shape)} and {tuple(out.shape)}")
+                         f"{heads * HEAD_DIM}], got {tuple(shape)} and {tuple(out.shape)}")
+    (ld_in, one), (ld_out, out_one) = qkv.stride(), out.stride()
+    if one != 1 or out_one != 1:
+        raise ValueError("rows of qkv and out must be contiguous")
     if window < 1 or sinks < 0:
         raise ValueError("a window has at least one key, the number of first keys is not negative")
     device = qkv.get_device()
@@ -85,12 +87,12 @@ def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: 
         with torch.cuda.device(device):
             return attention_window_fwd(qkv, out, batch, seq, heads, kv_heads, window=window, sinks=sinks, status=status,
                                         timeout_ms=timeout_ms, stream=stream)
-    lib = _native.kernels()
-    fn = _native.typed(lib.iris_k_attention_window_fwd, _WINDOW_ARGTYPES)
-    rc = fn(qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), batch, seq, heads, kv_heads, min(window, seq),
-            min(sinks, seq), _DT[qkv.dtype], status.data_ptr() if status is not None else 0, int(timeout_ms * 1e6),
-            _native.current_stream(device) if stream is None else stream)
+    rc = _native.entry("iris_k_attention_window_fwd")(_WINDOW_ARGS.pack(
+        qkv.data_ptr(), out.data_ptr(), 0 if status is None else status.data_ptr(),
+        torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, ld_in, ld_out, batch, seq, heads, kv_heads,
+        window, sinks, _DT[dtype], int(timeout_ms * 1e6)))
     if rc != 0:
+        lib = _native.kernels()
         lib.iris_attention_last_error.restype = ctypes.c_char_p
         raise RuntimeError(lib.iris_attention_last_error().decode() or f"attention launch failed ({rc})")
     return out

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -17,17 +18,24 @@ import torch
 from .. import _native
 
 _DT = {torch.bfloat16: 0, torch.float16: 1}
-_P, _L, _I, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
-_ATTENTION = [_P, _L, _L, _P, _P, _L, _L, _L, _L, _I, _I, _P, _L, _L, _P, _P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _I, _F, _L, _I,
-              _P, _L, _P, _I, _P]
-_RESERVE = [_P, _P, _P, _L, _L, _P, _L, _P, _I, _L, _P, _P, _L, _L, _P, _P, _P]
+_P, _L, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+_ATTENTION, _RESERVE = struct.Struct("@33qd"), struct.Struct("@17q")
 _RELEASE = [_P, _P, _P, _L, _L, _P, _L, _P, _I, _L, _P]
 
 
 def _ints(t: torch.Tensor, name: str, shape) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{name} must be int32 {list(shape)} with contiguous rows, got {t.dtype} {list(t.shape)}")
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
     return t
+
+
+def _rows(table: torch.Tensor, batch: int):
+    """Shape and strides of a block table."""
+    shape, strides = table.shape, table.stride()
+    if table.dtype is not torch.int32 or len(shape) != 2 or shape[0] != batch or (strides[1] != 1 and shape[1] > 1) or \
+            (strides[0] < shape[1] and batch > 1):
+        raise ValueError(f"block_table must be int32 [{batch}, pages of a request] with contiguous rows that do not overlap")
+    return shape, strides
 
 
 def same_strides(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -54,36 +62,44 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     given.  ``longest``: what the lengths are expected not to exceed, where that is much less than the table's width; it is
     for speed alone.
     """
-    if q.dtype not in _DT or out.dtype != q.dtype or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    dtype, shape, cache_shape = q.dtype, q.shape, k_cache.shape
+    if dtype not in _DT or out.dtype is not dtype or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise TypeError("q, out and the cache must all be bfloat16 or all float16")
-    if q.dim() != 3 or out.shape != q.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+    if len(shape) != 3 or out.shape != shape or len(cache_shape) != 4 or v_cache.shape != cache_shape:
         raise ValueError("expected q and out [batch, heads, head_dim] and a cache [pages, page_size, kv_heads, head_dim]")
-    batch, heads, dim = q.shape
-    pages, size, kv_heads, cache_dim = k_cache.shape
+    batch, heads, dim = shape
+    pages, size, kv_heads, cache_dim = cache_shape
     if cache_dim != dim or kv_heads < 1 or heads < 1 or heads % kv_heads or dim not in (64, 128, 256):
         raise ValueError(f"{heads} query heads of {dim} do not go with {kv_heads} key heads of {cache_dim} (64, 128 or 256)")
     q_batch, q_head, q_one = q.stride()
     out_batch, out_head, out_one = out.stride()
-    page, slot, head, one = k_cache.stride()
-    if one != 1 or q_one != 1 or out_one != 1 or not same_strides(k_cache, v_cache):
+    strides = page, slot, head, one = k_cache.stride()
+    if one != 1 or q_one != 1 or out_one != 1 or (v_cache.stride() != strides and not same_strides(k_cache, v_cache)):
         raise ValueError("k_cache and v_cache must have the same strides, and all heads be contiguous")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or (
-            block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise ValueError(f"block_table must be int32 [{batch}, pages of a sequence] with contiguous rows")
-    if lens.dtype != torch.int32 or lens.shape != (batch,) or (batch > 1 and lens.stride(0) != 1):
-        raise ValueError(f"lens must be contiguous int32 [{batch}]")
+    table_shape = block_table.shape
+    if block_table.dtype is not torch.int32 or len(table_shape) != 2 or table_shape[0] != batch:
+        raise ValueError(f"block_table must be int32 [{batch}, pages of a sequence]")
+    table_pitch, table_one = block_table.stride()
+    if lens.dtype is not torch.int32 or lens.shape != (batch,) or not lens.is_contiguous() or (table_one != 1 and table_shape[1] > 1):
+        raise ValueError(f"lens must be int32 [{batch}], and it and the rows of block_table contiguous")
     if (batch > 1 and out_batch < dim) or (heads > 1 and out_head < dim):
         raise ValueError("rows of out must not overlap")
     device = q.get_device()
     same = (out.get_device() == device and k_cache.get_device() == device and v_cache.get_device() == device and
             block_table.get_device() == device and lens.get_device() == device)
-    lse_ptr = lse_batch = 0
+    lse_ptr = lse_batch = status_ptr = 0
     if lse is not None:
-        if lse.dtype != torch.float32 or lse.shape != (batch, heads) or (heads > 1 and lse.stride(1) != 1):
-            raise ValueError(f"lse must be fp32 [{batch}, {heads}] with contiguous rows")
+        if lse.dtype is not torch.float32 or lse.shape != (batch, heads):
+            raise ValueError(f"lse must be fp32 [{batch}, {heads}]")
+        lse_batch, lse_one = lse.stride()
+        if (lse_one != 1 and heads > 1) or (batch > 1 and lse_batch < heads):
+            raise ValueError("rows of lse must be contiguous and not overlap")
         same = same and lse.get_device() == device
-        lse_ptr, lse_batch = lse.data_ptr(), lse.stride(0)
-    if not same or (status is not None and status.get_device() != device):
+        lse_ptr = lse.data_ptr()
+    if status is not None:
+        same = same and status.get_device() == device
+        status_ptr = status.data_ptr()
+    if not same:
         raise ValueError("all tensors must be on one device")
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
@@ -93,23 +109,25 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         with torch.cuda.device(device):
             return paged_attention(q, k_cache, v_cache, block_table, lens, out, window=window, sinks=sinks, scale=scale, lse=lse,
                                    longest=longest, status=status, stream=stream)
-    lib = _native.kernels()
-    fn = _native.typed(lib.iris_k_paged_attention, _ATTENTION)
-    raw = _native.current_stream(device) if stream is None else stream
-    work, bytes_ = None, 0
+    fn = _native.entry("iris_k_paged_attention")
+    current = torch._C._cuda_getCurrentRawStream(device)
+    work, work_ptr, work_bytes = None, 0, 0
     while True:
-        rc = fn(q.data_ptr(), q_batch, q_head, k_cache.data_ptr(), v_cache.data_ptr(), page, slot, head, pages, size, kv_heads,
-                block_table.data_ptr(), block_table.stride(0), block_table.shape[1], lens.data_ptr(), out.data_ptr(), out_batch,
-                out_head, lse_ptr, lse_batch, batch, heads, dim, _DT[q.dtype], window, sinks,
-                dim ** -0.5 if scale is None else scale, longest or 0, -1, 0 if work is None else work.data_ptr(), bytes_,
-                0 if status is None else status.data_ptr(), device, raw)
-        if rc <= 0 or bytes_:
+        rc = fn(_ATTENTION.pack(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lens.data_ptr(), out.data_ptr(), lse_ptr,
+            work_ptr, status_ptr, current if stream is None else stream, q_batch, q_head, page, slot, head, table_pitch, out_batch,
+            out_head, lse_batch, batch, heads, dim, pages, size, kv_heads, table_shape[1], _DT[dtype], window, sinks, longest or 0,
+            -1, work_bytes, device, dim ** -0.5 if scale is None else scale))
+        if rc <= 0 or work_bytes:
             break
-        work, bytes_ = torch.empty(rc, dtype=torch.uint8, device=q.device), rc   # sums of sequences that several CTAs share
+        # sums of sequences that several CTAs share, of this call alone
+        work, work_bytes = torch.empty(rc, dtype=torch.uint8, device=q.device), rc
+        work_ptr = work.data_ptr()
     if rc:
+        lib = _native.kernels()
         lib.iris_paged_attention_last_error.restype = ctypes.c_char_p
         raise RuntimeError(lib.iris_paged_attention_last_error().decode() or f"paged attention failed ({rc})")
-    if work is not None and stream is not None and stream != _native.current_stream(device):
+    if work is not None and stream is not None and stream != current:
         work.record_stream(torch.cuda.ExternalStream(stream, device=device))
     return out
 
@@ -130,42 +148,40 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     A request for which the free pages do not last (nor for any later one that lacks a page), whose tokens do not fit its row of
     the table, or have not enough rows, gets nothing: its length stays, its rows get -1.  All tensors int32.
     """
-    batch = lens.shape[0] if lens.dim() == 1 else -1
-    _ints(lens, "lens", (batch,))
-    _ints(new_lens, "new_lens", (batch,))
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or (
-            block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise ValueError(f"block_table must be int32 [{batch}, pages of a request] with contiguous rows")
-    if free_pages.dim() != 1 or slots.dim() != 1:
-        raise ValueError("free_pages and slots must be 1-D")
-    _ints(free_pages, "free_pages", free_pages.shape)
-    _ints(free_count, "free_count", (1,))
-    _ints(slots, "slots", slots.shape)
-    _ints(positions, "positions", slots.shape)
+    i32, shape, rows = torch.int32, lens.shape, slots.shape
+    lens_out = lens if lens_out is None else lens_out
+    free_count_out = free_count if free_count_out is None else free_count_out
+    for t in (lens, new_lens, free_pages, free_count, slots, positions, lens_out, free_count_out):
+        if t.dtype is not i32 or not t.is_contiguous():
+            raise ValueError("all tensors must be int32 and contiguous (block_table: its rows)")
+    if len(shape) != 1 or new_lens.shape != shape or lens_out.shape != shape:
+        raise ValueError(f"lens, new_lens and lens_out must be 1-D and of one length, got {list(shape)}, {list(new_lens.shape)} and "
+                         f"{list(lens_out.shape)}")
+    if len(rows) != 1 or positions.shape != rows or free_pages.dim() != 1 or free_count.shape != (1,) or free_count_out.shape != (1,):
+        raise ValueError("slots, positions and free_pages must be 1-D, the first two of one length, and the counts of one element")
+    batch, tokens = shape[0], rows[0]
+    table_shape, (pitch, one) = _rows(block_table, batch)
     if page_size < 1 or page_size & (page_size - 1):
         raise ValueError("page_size must be a power of two")
-    if row_stride < 0 or slots.shape[0] < batch * row_stride:
-        raise ValueError(f"{slots.shape[0]} rows do not hold {batch} requests of {row_stride}")
-    lens_out = lens if lens_out is None else _ints(lens_out, "lens_out", (batch,))
-    free_count_out = free_count if free_count_out is None else _ints(free_count_out, "free_count_out", (1,))
+    if row_stride < 0 or tokens < batch * row_stride:
+        raise ValueError(f"{tokens} rows do not hold {batch} requests of {row_stride}")
     device = lens.get_device()
     for t in (new_lens, block_table, free_pages, free_count, slots, positions, lens_out, free_count_out):
         if t.get_device() != device:
             raise ValueError("all tensors must be on one device")
-    if batch == 0 or block_table.shape[1] == 0:
+    if batch == 0 or table_shape[1] == 0:
         raise ValueError("no requests, or no room in the block table")
     if device != _native.current_device(device):
         with torch.cuda.device(device):
             return reserve_slots(lens, new_lens, block_table, free_pages, free_count, page_size, slots, positions,
                                  row_stride=row_stride, lens_out=lens_out, free_count_out=free_count_out, stream=stream)
-    lib = _native.kernels()
-    rc = _native.typed(lib.iris_k_reserve_slots, _RESERVE)(
-        lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, batch, slots.data_ptr(),
-        positions.data_ptr(), slots.shape[0], row_stride, lens_out.data_ptr(), free_count_out.data_ptr(),
-        _native.current_stream(device) if stream is None else stream)
+    rc = _native.entry("iris_k_reserve_slots")(_RESERVE.pack(
+        lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+        slots.data_ptr(), positions.data_ptr(), lens_out.data_ptr(), free_count_out.data_ptr(),
+        torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, pitch, table_shape[1], free_pages.shape[0],
+        page_size, batch, tokens, row_stride))
     if rc:
-        _raise(lib, "reserve_slots", rc)
+        _raise("reserve_slots", rc)
 
 
 def release_slots(lens: torch.Tensor, which: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -176,9 +192,7 @@ def release_slots(lens: torch.Tensor, which: torch.Tensor, block_table: torch.Te
     batch = lens.shape[0] if lens.dim() == 1 else -1
     _ints(lens, "lens", (batch,))
     _ints(which, "which", (batch,))
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or (
-            block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise ValueError(f"block_table must be int32 [{batch}, pages of a request] with contiguous rows")
+    table_shape, (pitch, one) = _rows(block_table, batch)
     if free_pages.dim() != 1:
         raise ValueError("free_pages must be 1-D")
     _ints(free_pages, "free_pages", free_pages.shape)
@@ -189,21 +203,22 @@ def release_slots(lens: torch.Tensor, which: torch.Tensor, block_table: torch.Te
     for t in (which, block_table, free_pages, free_count):
         if t.get_device() != device:
             raise ValueError("all tensors must be on one device")
-    if batch == 0 or block_table.shape[1] == 0:
+    if batch == 0 or table_shape[1] == 0:
         raise ValueError("no requests, or no room in the block table")
     if device != _native.current_device(device):
         with torch.cuda.device(device):
             return release_slots(lens, which, block_table, free_pages, free_count, page_size, stream=stream)
     lib = _native.kernels()
     rc = _native.typed(lib.iris_k_release_slots, _RELEASE)(
-        lens.data_ptr(), which.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        lens.data_ptr(), which.data_ptr(), block_table.data_ptr(), pitch, table_shape[1],
         free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, batch,
         _native.current_stream(device) if stream is None else stream)
     if rc:
-        _raise(lib, "release_slots", rc)
+        _raise("release_slots", rc)
 
 
-def _raise(lib, what: str, rc: int):
+def _raise(what: str, rc: int):
+    lib = _native.kernels()
     lib.iris_pages_last_error.restype = ctypes.c_char_p
     raise RuntimeError(f"{what}: " + (lib.iris_pages_last_error().decode() or f"launch failed ({rc})"))
 

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -13,8 +14,7 @@ from .. import _native
 from .paged import same_strides
 
 _DT = {torch.bfloat16: 0, torch.float16: 1}
-_P, _L, _I, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
-_ARGTYPES = [_P, _L, _P, _L, _I, _P, _P, _L, _L, _I, _I, _P, _P, _F, _P, _P, _L, _L, _L, _L, _I, _P, _L, _I, _I, _I, _I, _P, _P]
+_ARGS = struct.Struct("@28qd")
 
 
 def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0, *, scaling: Optional[str] = None,
@@ -52,16 +52,20 @@ def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0, *, sca
     return torch.cat([angle.cos(), angle.sin()], 1).to(torch.float32)
 
 
-def _may_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two matrices of 16-bit elements share memory; column blocks of one matrix, with its pitch, do not."""
-    rows, pitch, size = a.shape[0], a.stride(0), 2
-    a0, b0 = a.data_ptr(), b.data_ptr()
-    a1, b1 = a0 + ((rows - 1) * pitch + a.shape[1]) * size, b0 + ((rows - 1) * b.stride(0) + b.shape[1]) * size
-    if a1 <= b0 or b1 <= a0:
+def _weight(w: torch.Tensor, head_dim: int, dtype: torch.dtype) -> int:
+    if w.dtype is not dtype or w.shape != (head_dim,) or not w.is_contiguous():
+        raise ValueError(f"norm weights must be contiguous [{head_dim}] of the type of qkv")
+    return w.data_ptr()
+
+
+def _may_overlap(rows: int, a: int, a_pitch: int, a_width: int, b: int, b_pitch: int, b_width: int) -> bool:
+    """Whether two matrices of 16-bit elements (address, pitch and width in elements) share memory; column blocks of one matrix,
+    with its pitch, do not."""
+    if a + ((rows - 1) * a_pitch + a_width) * 2 <= b or b + ((rows - 1) * b_pitch + b_width) * 2 <= a:
         return False
-    if pitch == b.stride(0) and rows > 1:
-        off = (b0 - a0) % (pitch * size)
-        return off < a.shape[1] * size or off + b.shape[1] * size > pitch * size
+    if a_pitch == b_pitch and rows > 1:
+        off = (b - a) % (a_pitch * 2) if a_pitch else 0
+        return off < a_width * 2 or off + b_width * 2 > a_pitch * 2
     return True
 
 
@@ -83,75 +87,83 @@ def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, 
     are left as they were, in ``out`` and in the cache.  A position behind the table or a slot behind the cache is skipped and
     recorded in ``status`` (an ``Iris`` context's status block) if that is given.
     """
-    if qkv.dtype not in _DT or out.dtype != qkv.dtype:
+    dtype, shape, out_shape = qkv.dtype, qkv.shape, out.shape
+    if dtype not in _DT or out.dtype is not dtype:
         raise TypeError("qkv and out must both be bfloat16 or both float16")
-    if qkv.dim() != 2 or out.dim() != 2 or qkv.stride(1) != 1 or out.stride(1) != 1:
-        raise ValueError("qkv and out must be 2-D with contiguous rows")
-    tokens, width = qkv.shape
+    if len(shape) != 2 or len(out_shape) != 2:
+        raise ValueError("qkv and out must be 2-D")
+    (tokens, width), (ld_in, one), (ld_out, out_one) = shape, qkv.stride(), out.stride()
     if heads < 1 or kv_heads < 1 or head_dim < 16 or head_dim % 16 or head_dim > 512:
         raise ValueError("need heads, and a head dimension that is a multiple of 16, at most 512")
-    if width != (heads + 2 * kv_heads) * head_dim or out.shape[0] != tokens or out.shape[1] not in (width, heads * head_dim):
+    out_width = out_shape[1]
+    if width != (heads + 2 * kv_heads) * head_dim or out_shape[0] != tokens or (out_width != width and out_width != heads * head_dim):
         raise ValueError(f"expected qkv [tokens, {(heads + 2 * kv_heads) * head_dim}] and out like it or [tokens, "
-                         f"{heads * head_dim}], got {tuple(qkv.shape)} and {tuple(out.shape)}")
+                         f"{heads * head_dim}], got {tuple(shape)} and {tuple(out_shape)}")
+    if positions.dtype is not torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous() or one != 1 or out_one != 1:
+        raise ValueError(f"positions must be int32 [{tokens}], and they and the rows of qkv and out contiguous")
     device = qkv.get_device()
-    if positions.dtype != torch.int32 or positions.shape != (tokens,) or (tokens > 1 and positions.stride(0) != 1):
-        raise ValueError(f"positions must be contiguous int32 [{tokens}]")
     same = out.get_device() == device and positions.get_device() == device
     turns = table_ptr = table_pitch = rotary = 0
     if table is not None:
-        if table.dtype != torch.float32 or table.dim() != 2 or table.stride(1) != 1 or table.shape[1] > head_dim or table.shape[1] % 16:
-            raise ValueError("table must be fp32 [positions, rotary dimension], at most as wide as a head, a multiple of 16")
+        if table.dtype is not torch.float32 or table.dim() != 2:
+            raise ValueError("table must be fp32 [positions, rotary dimension]")
+        (turns, rotary), (table_pitch, one) = table.shape, table.stride()
+        if one != 1 or rotary > head_dim or rotary % 16:
+            raise ValueError("the rotary dimension must be a multiple of 16 within the head, the table's rows contiguous")
         same = same and table.get_device() == device
-        (turns, rotary), table_ptr, table_pitch = table.shape, table.data_ptr(), table.stride(0)
-    for w in (q_weight, k_weight):
-        if w is not None:
-            if w.dtype != qkv.dtype or w.shape != (head_dim,) or w.stride(0) != 1:
-                raise ValueError(f"norm weights must be [{head_dim}] of the type of qkv")
-            same = same and w.get_device() == device
-    in_place = False
-    if tokens:
-        in_place = out.data_ptr() == qkv.data_ptr() and out.stride(0) == qkv.stride(0)
-        if tokens > 1 and out.stride(0) < out.shape[1]:
-            raise ValueError("rows of out must not overlap")
-        if not in_place and _may_overlap(qkv, out):
-            raise ValueError("out must be qkv itself, or share no memory with it")
-    k_ptr = v_ptr = slots_ptr = 0
-    page = slot = head = pages = size = 0
+        table_ptr = table.data_ptr()
+    q_ptr = k_ptr = 0
+    if q_weight is not None:
+        same = same and q_weight.get_device() == device
+        q_ptr = _weight(q_weight, head_dim, dtype)
+    if k_weight is not None:
+        same = same and k_weight.get_device() == device
+        k_ptr = _weight(k_weight, head_dim, dtype)
+    k_cache_ptr = v_cache_ptr = slots_ptr = page = slot = head = pages = size = 0
     if k_cache is not None or v_cache is not None or slots is not None:
         if k_cache is None or v_cache is None or slots is None:
             raise ValueError("k_cache, v_cache and slots belong together")
-        if k_cache.dtype != qkv.dtype or v_cache.dtype != qkv.dtype:
+        if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
             raise TypeError("the cache must have the type of qkv")
-        if k_cache.dim() != 4 or k_cache.shape[2:] != (kv_heads, head_dim) or v_cache.shape != k_cache.shape:
+        cache_shape = k_cache.shape
+        if len(cache_shape) != 4 or cache_shape[2] != kv_heads or cache_shape[3] != head_dim or v_cache.shape != cache_shape:
             raise ValueError(f"the cache must be [pages, page_size, {kv_heads}, {head_dim}]")
-        page, slot, head, one = k_cache.stride()
-        if one != 1 or not same_strides(k_cache, v_cache):
+        strides = page, slot, head, one = k_cache.stride()
+        if one != 1 or (v_cache.stride() != strides and not same_strides(k_cache, v_cache)):
             raise ValueError("k_cache and v_cache must have the same strides, with contiguous heads")
-        if slots.dtype != torch.int32 or slots.shape != (tokens,) or (tokens > 1 and slots.stride(0) != 1):
+        if slots.dtype is not torch.int32 or slots.shape != (tokens,) or not slots.is_contiguous():
             raise ValueError(f"slots must be contiguous int32 [{tokens}]")
         same = same and k_cache.get_device() == device and v_cache.get_device() == device and slots.get_device() == device
-        pages, size = k_cache.shape[0], k_cache.shape[1]
-        k_ptr, v_ptr, slots_ptr = k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr()
-    elif out.shape[1] != width:
+        pages, size = cache_shape[0], cache_shape[1]
+        k_cache_ptr, v_cache_ptr, slots_ptr = k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr()
+    elif out_width != width:
         raise ValueError("an output of queries alone needs a cache for the keys and values")
-    if not same or (status is not None and status.get_device() != device):
+    status_ptr = 0
+    if status is not None:
+        same = same and status.get_device() == device
+        status_ptr = status.data_ptr()
+    if not same:
         raise ValueError("all tensors must be on one device")
     if tokens == 0:
         return out
+    qkv_ptr, out_ptr = qkv.data_ptr(), out.data_ptr()
+    in_place = out_ptr == qkv_ptr and ld_out == ld_in
+    if tokens > 1 and ld_out < out_width:
+        raise ValueError("rows of out must not overlap")
+    if not in_place and _may_overlap(tokens, qkv_ptr, ld_in, width, out_ptr, ld_out, out_width):
+        raise ValueError("out must be qkv itself, or share no memory with it")
     if device != _native.current_device(device):
         with torch.cuda.device(device):
             return qk_norm_rope(qkv, out, positions, table, heads, kv_heads, head_dim, q_weight=q_weight, k_weight=k_weight,
                                 eps=eps, interleaved=interleaved, k_cache=k_cache, v_cache=v_cache, slots=slots, status=status,
                                 stream=stream)
-    out_heads = heads + kv_heads if in_place and out.shape[1] == width else out.shape[1] // head_dim
-    lib = _native.kernels()
-    fn = _native.typed(lib.iris_k_qk_norm_rope, _ARGTYPES)
-    rc = fn(qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), out_heads, positions.data_ptr(), table_ptr,
-            table_pitch, turns, rotary, 1 if interleaved else 0,
-            0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), eps, k_ptr, v_ptr,
-            page, slot, head, pages, size, slots_ptr, tokens, heads, kv_heads, head_dim, _DT[qkv.dtype],
-            0 if status is None else status.data_ptr(), _native.current_stream(device) if stream is None else stream)
+    rc = _native.entry("iris_k_qk_norm_rope")(_ARGS.pack(
+        qkv_ptr, out_ptr, positions.data_ptr(), table_ptr, q_ptr, k_ptr, k_cache_ptr, v_cache_ptr, slots_ptr, status_ptr,
+        torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, ld_in, ld_out, table_pitch, page, slot, head,
+        heads + kv_heads if in_place and out_width == width else out_width // head_dim, turns, rotary, 1 if interleaved else 0,
+        pages, size, tokens, heads, kv_heads, head_dim, _DT[dtype], eps))
     if rc:
+        lib = _native.kernels()
         lib.iris_rotary_last_error.restype = ctypes.c_char_p
         raise RuntimeError("qk_norm_rope: " + (lib.iris_rotary_last_error().decode() or f"launch failed ({rc})"))
     return out
