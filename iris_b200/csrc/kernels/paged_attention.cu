@@ -7,14 +7,17 @@
 // h / (heads / kv_heads).  16-bit elements, fp32 sums, head dimension 64, 128 or 256.  No counterpart in the reference.
 //
 // Every key and value is read once and used for 2 * group products: HBM bounds it, and the work goes into an even share of
-// the bytes for every SM and enough of them in flight.
-//   * The keys that are seen are counted through (sinks first, then the window), so a mask costs nothing: a position in that
-//     count gives the key, the key its page.
-//   * A warp is a worker of its own: it takes 16 of the 64 keys of a tile, copies their rows into a ring of its own with
-//     cp.async (16 bytes a lane, rows found through the block table one step ahead), and keeps its own running maximum, sum
-//     and output in registers (one pass).  No barrier inside a sequence; the four warps meet when a sequence's tiles end.
-//   * Products go through mma.sync m16n8k16: up to 16 query heads that share a key head are the 16 rows.  (The rate that a
-//     group of 16 asks of them is 2 % of what the tensor cores do; a tcgen05 tile is 128 rows.)
+// the bytes for every SM, enough of them in flight, and few instructions per byte.
+//   * The keys that are seen are counted through in blocks of 16 (first keys, then the window), so a mask costs nothing but at
+//     the blocks' edges: a position in that count gives the key, the key its page.
+//   * A warp is a worker of its own: it takes its blocks of a tile, copies their rows into a ring of its own with cp.async (16
+//     bytes a lane, rows found through the block table one step ahead; a block lies in one page unless pages are smaller), and
+//     keeps its own running maximum, sum and output in registers (one pass).  No barrier inside a sequence; the warps meet when
+//     a sequence's tiles end.
+//   * Products go through mma.sync m16n8k16 with the keys (for the scores) and the components (for the output) as the 16 rows
+//     and the query heads that share a key head as the 8 columns: half as many instructions as with the heads as rows, for up
+//     to 8 heads.  (A tcgen05 tile is 128 rows; the rate asked for here is 1 % of what those do.)
+//   * A step that raises no running maximum, which a vote finds out, needs no reduction over lanes.
 //   * The weights enter the second product as two 16-bit numbers, the rounded value and what it lost, so that the output has
 //     one rounding to 16 bits, its own.
 // Two ways to share out the keys:
@@ -41,28 +44,30 @@ namespace paged {
 
 using namespace iris::ptx;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kWarpKeys = 16;                    // keys of a warp in a tile
-constexpr int kTile = kWarps * kWarpKeys;        // keys of a tile
-constexpr int kRows = 16;                        // query heads of a tile
-constexpr int kJoinThreads = 256;
+constexpr int kRows = 16;                        // query heads of a segment, at most
+constexpr int kBlock = 16;                       // keys of a product
+constexpr int kJoinThreads = 512;
 constexpr uint32_t kSitePage = 95;
 
-template <int D>
+template <int D, int COLS = 8>
 struct Shape {
-  static constexpr int kStages = D == 64 ? 6 : 3;              // ring of a warp
-  static constexpr int kQBufs = D == 64 ? 8 : 4;               // queries of the sequences that the ring reaches: stages + 1, a power of two
+  static constexpr int kWarps = D == 256 ? 2 : 4;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kBlocks = D == 64 ? 2 : 1;              // blocks of a warp's step
+  static constexpr int kWarpKeys = kBlocks * kBlock;
+  static constexpr int kTile = kWarps * kWarpKeys;             // keys of a tile
+  static constexpr int kStages = D == 256 && COLS == 16 ? 2 : 3;   // ring of a warp
+  static constexpr int kQBufs = 4;                             // queries of the segments that the ring reaches: stages + 1
   static constexpr int kHalf = kWarpKeys * D * 2;              // keys (or values) of a stage
-  static constexpr int kStageBytes = 2 * kHalf;                // = the fp32 output of a warp, which takes its place at the end
+  static constexpr int kStageBytes = 2 * kHalf;                // holds the fp32 output of a warp, which takes its place at the end
   static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kQBytes = COLS * D * 2;
   static constexpr int kStats = 2 * kWarps * kRows * 4;        // maxima and sums of the warps
-  static constexpr int kMasks = kWarps * 8 * 4;                // which keys of a stage count
-  static constexpr int kSmem = kRing + kQBufs * kQBytes + kStats + kMasks + 64;
-  static constexpr int kPerSm = D == 256 ? 1 : 2;
-  static_assert(kStages <= 8 && kStages < kQBufs, "ring");
-  static_assert(kPerSm * (kSmem + 1024) <= 228 * 1024 && kSmem <= 227 * 1024, "shared-memory budget");
+  static constexpr int kMasks = kWarps * 4 * 4;                // which keys of a stage count
+  static constexpr int kSmem = kRing + kQBufs * kQBytes + kStats + kMasks + 16;
+  static constexpr int kPerSm = 2;
+  static_assert(kStages < kQBufs && kStageBytes >= COLS * D * 4, "ring");
+  static_assert(kPerSm * (kSmem + 1024) <= 228 * 1024, "shared-memory budget");
 };
 
 struct Params {
@@ -114,6 +119,12 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The 8 x 8 matrix of 16-bit elements whose row g lane 4 g + t holds columns 2 t and 2 t + 1 of, transposed.
+__device__ __forceinline__ uint32_t transpose(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 template <bool F16>
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   if (F16) {
@@ -128,21 +139,34 @@ __device__ __forceinline__ float2 unpack(uint32_t v) {
   return F16 ? __half22float2(*reinterpret_cast<__half2*>(&v)) : __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
 }
 
-// The keys that a sequence's newest token sees, counted through: position v is key v below `sinks`, key v + skip above.
+// The keys that a sequence's newest token sees, counted through in whole blocks: positions 0 .. head - 1 are the keys of that
+// number, of which those below `sinks` count, the others key position + skip, of which those from `start` to `len` do.
 struct Seen {
-  int n, sinks, skip;
+  int n, head, sinks, skip, start, len;
 };
 __device__ __forceinline__ Seen seen_of(const Params& p, int len) {
   const int64_t cap = (int64_t)p.wide << p.page_shift;
   len = len < 0 ? 0 : (int64_t)len > cap ? (int)cap : len;
-  const int start = p.window > 0 && len > p.window ? len - p.window : 0;
   Seen s;
-  s.sinks = p.sinks < start ? p.sinks : start;
-  s.skip = start - s.sinks;
+  s.len = len;
+  s.start = p.window > 0 && len > p.window ? len - p.window : 0;
+  s.sinks = min(p.sinks, s.start);
+  s.head = (s.sinks + kBlock - 1) & ~(kBlock - 1);
+  s.skip = (s.start & ~(kBlock - 1)) - s.head;
   s.n = len - s.skip;
   return s;
 }
+// The block's keys that count, a bit each, and the first of them all.
+__device__ __forceinline__ uint32_t block_mask(const Seen& s, int at, int& key) {
+  const bool first = at < s.head;
+  key = first ? at : at + s.skip;
+  const int from = first ? 0 : s.start - key, to = (first ? s.sinks : s.len) - key;
+  if (to <= 0) return 0;
+  return (to >= kBlock ? 0xffffu : (1u << to) - 1) & (from > 0 ? 0xffffu << from : 0xffffu);
+}
+template <int D>
 __device__ __forceinline__ int tiles_of(const Seen& s) {   // a sequence without keys has one tile too: its output is zeros
+  constexpr int kTile = Shape<D>::kTile;
   const int t = s.n / kTile + (s.n % kTile != 0);
   return t ? t : 1;
 }
@@ -152,18 +176,20 @@ struct Cursor {
   Seen s;
   int b, seg, tile, tiles, next_len;
 };
+template <int D>
 __device__ __forceinline__ void enter(const Params& p, Cursor& c, int len) {
   c.s = seen_of(p, len);
-  c.tiles = tiles_of(c.s);
+  c.tiles = tiles_of<D>(c.s);
   c.next_len = c.b + 1 < p.batch ? p.lens[c.b + 1] : 0;
 }
 // Whether a new segment begins.
+template <int D>
 __device__ __forceinline__ bool advance(const Params& p, Cursor& c) {
   if (++c.tile < c.tiles) return false;
   c.tile = 0;
   if (++c.seg == p.segments_per_seq) {
     c.seg = 0;
-    if (++c.b < p.batch) enter(p, c, c.next_len);
+    if (++c.b < p.batch) enter<D>(p, c, c.next_len);
   }
   return true;
 }
@@ -188,18 +214,22 @@ __device__ __forceinline__ void store4(uint8_t* dst, float4 a, float f) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack<F16>(a.x * f, a.y * f), pack<F16>(a.z * f, a.w * f));
 }
 
-template <int D, bool F16, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_kernel(const __grid_constant__ Params p) {
-  using S = Shape<D>;
+// COLS: columns of heads, 8 or 16.
+template <int D, bool F16, bool CLUSTER, int COLS>
+__global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPerSm)
+    paged_attention_kernel(const __grid_constant__ Params p) {
+  using S = Shape<D, COLS>;
+  constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kB = S::kBlocks, kTile = S::kTile;
+  constexpr int kN = COLS / 8;
   constexpr int kChunks = D / 8;             // 16-byte pieces of a row
   constexpr int kRowsPer = 32 / kChunks;     // rows that a warp copies at a time
   extern __shared__ __align__(128) uint8_t smem[];
   float* stat_m = reinterpret_cast<float*>(smem + S::kRing + S::kQBufs * S::kQBytes);
   float* stat_l = stat_m + kWarps * kRows;
   volatile uint32_t* masks = reinterpret_cast<uint32_t*>(stat_l + kWarps * kRows);
-  volatile int* words = reinterpret_cast<int*>(const_cast<uint32_t*>(masks) + kWarps * 8);
+  volatile int* words = reinterpret_cast<int*>(const_cast<uint32_t*>(masks) + kWarps * 4);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;     // an accumulator's row (and row + 8), and column pair
+  const int g = lane >> 2, t = lane & 3;     // scores: keys g and g + 8 of a block, heads 2 t and 2 t + 1
   const uint32_t q_s = smem_u32(smem) + S::kRing;
   const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStageBytes;
   const float* ring_f = reinterpret_cast<const float*>(smem);
@@ -214,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
   if (CLUSTER) {
     c.b = blockIdx.z;
     c.seg = blockIdx.y;
-    enter(p, c, p.lens[c.b]);
+    enter<D>(p, c, p.lens[c.b]);
     const int parts = gridDim.x, r = blockIdx.x;
     c.tile = (int)((int64_t)c.tiles * r / parts);
     count = (int)((int64_t)c.tiles * (r + 1) / parts) - c.tile;
@@ -223,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
     const int per = (p.batch + kThreads - 1) / kThreads;
     const int b0 = min(p.batch, (int)threadIdx.x * per), b1 = min(p.batch, b0 + per);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(seen_of(p, p.lens[b]));
+    for (int b = b0; b < b1; ++b) mine += tiles_of<D>(seen_of(p, p.lens[b]));
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -250,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
       int64_t left = first - before;
       int b = b0, n;
       for (;; ++b) {
-        n = tiles_of(seen_of(p, p.lens[b]));
+        n = tiles_of<D>(seen_of(p, p.lens[b]));
         if (left < (int64_t)n * p.segments_per_seq) break;
         left -= (int64_t)n * p.segments_per_seq;
       }
@@ -261,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
     __syncthreads();
     c.b = words[0];
     c.seg = words[1];
-    enter(p, c, p.lens[c.b]);
+    enter<D>(p, c, p.lens[c.b]);
     c.tile = words[2];
   }
 
@@ -269,63 +299,101 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
   Cursor l = c;
   int l_left = count, l_stage = 0, l_seg = 0;
   bool l_new = true;                          // the next step is its segment's first here
-  int l_page = 0;                             // page of this lane's row of the next step
-  auto find_page = [&]() {
-    const int at = l.tile * kTile + warp * kWarpKeys + (lane & 15);
-    const int key = at < l.s.sinks ? at : at + l.s.skip;
-    l_page = l_left > 0 && at < l.s.n ? p.table[l.b * p.table_pitch + (key >> p.page_shift)] : 0;
+  int l_page[kB];                             // pages of the next step's blocks (pages of fewer than 16: of this lane's rows)
+  auto find_pages = [&]() {
+#pragma unroll
+    for (int i = 0; i < kB; ++i) {
+      int key;
+      const uint32_t mask = l_left > 0 ? block_mask(l.s, l.tile * kTile + warp * S::kWarpKeys + i * kBlock, key) : 0;
+      if (p.page_shift < 4) key += lane & 15;
+      l_page[i] = 0;
+      if (p.page_shift < 4 ? mask >> (lane & 15) & 1 : mask != 0) l_page[i] = p.table[l.b * p.table_pitch + (key >> p.page_shift)];
+    }
   };
   auto issue = [&]() {
     if (l_left > 0) {
       const int kv = p.row_tiles == 1 ? l.seg : l.seg / p.row_tiles;
-      if (l_new) {                            // the queries: four rows a warp
+      if (l_new) {                            // the queries, shared out over the warps; zeros where there is no head
         const int r0 = (l.seg - kv * p.row_tiles) * kRows;
         const uint8_t* src = p.q + l.b * p.q_batch + (int64_t)(kv * p.group + r0) * p.q_head;
         const uint32_t dst = q_s + (l_seg & (S::kQBufs - 1)) * S::kQBytes;
 #pragma unroll
-        for (int i = 0; i < 4 / kRowsPer; ++i) {
-          const int row = warp * 4 + i * kRowsPer + lane / kChunks, ch = lane % kChunks;
-          if (r0 + row < p.group) cp_async16(dst + row * D * 2 + ((ch ^ (row & 7)) << 4), src + row * p.q_head + ch * 16, true);
+        for (int i = 0; i < (COLS / kWarps + kRowsPer - 1) / kRowsPer; ++i) {
+          const int row = warp * (COLS / kWarps) + i * kRowsPer + lane / kChunks, ch = lane % kChunks;
+          if (i * kRowsPer + lane / kChunks < COLS / kWarps) {
+            const bool take = r0 + row < p.group;
+            cp_async16(dst + row * D * 2 + ((ch ^ (row & 7)) << 4), take ? src + row * p.q_head + ch * 16 : p.q, take);
+          }
         }
       }
-      const int at = l.tile * kTile + warp * kWarpKeys + (lane & 15);
-      const int key = at < l.s.sinks ? at : at + l.s.skip;
-      const bool inside = at < l.s.n;
-      const bool ok = inside && (uint32_t)l_page < (uint32_t)p.pages;
-      if (inside && !ok) record_status(p.status, kBadPointer, kSitePage, l.b, key, (uint64_t)(int64_t)l_page);
-      const int64_t off =
-          ok ? l_page * p.page_pitch + (key & ((1 << p.page_shift) - 1)) * p.slot_pitch + kv * p.head_pitch : 0;
-      const uint32_t mask = __ballot_sync(0xffffffffu, ok);
-      if (lane == 0) masks[warp * 8 + l_stage] = mask;
-      const uint32_t dst = ring + l_stage * S::kStageBytes;
+      uint32_t word = 0;
 #pragma unroll
-      for (int i = 0; i < kWarpKeys / kRowsPer; ++i) {
-        const int row = i * kRowsPer + lane / kChunks, ch = lane % kChunks;
-        const int64_t o = __shfl_sync(0xffffffffu, off, row) + ch * 16;
-        const bool take = mask >> row & 1;
-        const uint32_t d = dst + row * D * 2 + ((ch ^ (row & 7)) << 4);
-        cp_async16(d, p.k + o, take);
-        cp_async16(d + S::kHalf, p.v + o, take);
+      for (int i = 0; i < kB; ++i) {
+        int key;
+        uint32_t mask = block_mask(l.s, l.tile * kTile + warp * S::kWarpKeys + i * kBlock, key);
+        const int row0 = lane / kChunks, ch = lane % kChunks;
+        const uint32_t dst = ring + l_stage * S::kStageBytes + i * kBlock * D * 2 + row0 * D * 2;
+        const int64_t head = kv * p.head_pitch + ch * 16;
+        if (p.page_shift >= 4) {
+          if (mask && (uint32_t)l_page[i] >= (uint32_t)p.pages) {
+            if (lane == 0) record_status(p.status, kBadPointer, kSitePage, l.b, key, (uint64_t)(int64_t)l_page[i]);
+            mask = 0;
+          }
+          if (mask) {
+            const int64_t off = l_page[i] * p.page_pitch + ((key & ((1 << p.page_shift) - 1)) + row0) * p.slot_pitch + head;
+            const uint8_t *k = p.k + off, *v = p.v + off;
+#pragma unroll
+            for (int j = 0; j < kBlock / kRowsPer; ++j) {
+              const bool take = mask >> (j * kRowsPer + row0) & 1;
+              const uint32_t d = dst + j * kRowsPer * D * 2 + ((ch ^ ((j * kRowsPer + row0) & 7)) << 4);
+              cp_async16(d, k, take);
+              cp_async16(d + S::kHalf, v, take);
+              k += kRowsPer * p.slot_pitch;
+              v += kRowsPer * p.slot_pitch;
+            }
+          }
+        } else {
+          const int r = key + (lane & 15);
+          const bool in = mask >> (lane & 15) & 1, ok = in && (uint32_t)l_page[i] < (uint32_t)p.pages;
+          if (in && !ok) record_status(p.status, kBadPointer, kSitePage, l.b, r, (uint64_t)(int64_t)l_page[i]);
+          const int64_t off = ok ? l_page[i] * p.page_pitch + (r & ((1 << p.page_shift) - 1)) * p.slot_pitch : 0;
+          mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+#pragma unroll
+          for (int j = 0; j < kBlock / kRowsPer; ++j) {
+            const int row = j * kRowsPer + row0;
+            const int64_t o = __shfl_sync(0xffffffffu, off, row) + head;
+            const bool take = mask >> row & 1;
+            const uint32_t d = dst + j * kRowsPer * D * 2 + ((ch ^ (row & 7)) << 4);
+            cp_async16(d, p.k + o, take);
+            cp_async16(d + S::kHalf, p.v + o, take);
+          }
+        }
+        word |= mask << 16 * i;
       }
+      if (lane == 0) masks[warp * 4 + l_stage] = word;
       l_stage = l_stage + 1 == S::kStages ? 0 : l_stage + 1;
       --l_left;
-      l_new = advance(p, l);
+      l_new = advance<D>(p, l);
       if (l_new) ++l_seg;
-      find_page();
+      find_pages();
     }
     cp_commit();
   };
-  find_page();
+  find_pages();
 #pragma unroll 1
   for (int i = 0; i < S::kStages; ++i) issue();
 
   // ---- products ----
-  float o[D / 8][4], m[2], sum[2];
+  float o[D / 16][kN][4], m[kN][2], sum[kN][2];   // output: components g and g + 8 of 16, heads 2 t and 2 t + 1
+  uint32_t q[D / 16][kN][2];
   auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    m[0] = m[1] = -INFINITY;
-    sum[0] = sum[1] = 0.f;
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      sum[n][0] = sum[n][1] = 0.f;
+    }
   };
   clear();
   const int mat = lane >> 3, mrow = lane & 7;   // ldmatrix: which of the four 8 x 8 pieces this lane addresses, and its row
@@ -333,11 +401,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
   bool fresh = true, whole = c.tile == 0;       // whole: the segment began in this CTA
   int64_t seg_first = first - c.tile;           // stream: its first tile among all
 
-  // The four warps' results of a segment (whose last stage here is `stage`): sum over them of this thread's four columns
-  // of a row.
+  // The warps' results of a segment (whose last stage here is `stage`): sum over them of this thread's four columns of a row.
   auto merged = [&](int item, float& mx, float& l) {
     const int row = item / (D / 4), col = item % (D / 4);
-    mx = fmaxf(fmaxf(stat_m[row], stat_m[kRows + row]), fmaxf(stat_m[2 * kRows + row], stat_m[3 * kRows + row]));
+    mx = stat_m[row];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, stat_m[w * kRows + row]);
     l = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -345,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
       const float mw = stat_m[w * kRows + row], lw = stat_l[w * kRows + row];
       const float f = mw == mx ? 1.f : exp2_fast(mw - mx);
       const float4 x = *reinterpret_cast<const float4*>(ring_f + (w * S::kStages + stage) * (S::kStageBytes / 4) + row * D +
-                                                        ((((col >> 1) ^ (row & 7)) << 3) | ((col & 1) << 2)));
+                                                        ((((col >> 1) ^ (row >> 1 & 3)) << 3) | ((col & 1) << 2)));
       if (lw != 0.f) {    // (a warp without keys, or with keys of minus infinity only, adds nothing; one with a NaN adds that)
         l += lw * f;
         a.x += x.x * f, a.y += x.y * f, a.z += x.z * f, a.w += x.w * f;
@@ -358,24 +427,28 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
     store4<F16>(p.out + b * p.out_batch + head * p.out_head + col * 8, a, l == 0.f ? 0.f : 1.f / l);
     if (p.lse && col == 0) p.lse[b * p.lse_batch + head] = log_sum(mx, l);
   };
-  // this warp's results into the ring stage it has just used up
+  // this warp's results into the ring stage it has just used up; rows of 8-column groups in an order that keeps the banks apart
   auto deposit = [&]() {
     float* dst = reinterpret_cast<float*>(smem) + (warp * S::kStages + stage) * (S::kStageBytes / 4);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float x = sum[h];
-      x += __shfl_xor_sync(0xffffffffu, x, 1);
-      x += __shfl_xor_sync(0xffffffffu, x, 2);
-      if (t == 0) {
-        stat_m[warp * kRows + g + 8 * h] = m[h];
-        stat_l[warp * kRows + g + 8 * h] = x;
-      }
-      if (h == 0 || p.group > 8) {
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          *reinterpret_cast<float2*>(dst + (g + 8 * h) * D + ((i ^ g) << 3) + 2 * t) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+      for (int e = 0; e < 2; ++e) {
+        float x = sum[n][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int row = 8 * n + 2 * t + e;
+        if (g == 0) {
+          stat_m[warp * kRows + row] = m[n][e];
+          stat_l[warp * kRows + row] = x;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          dst[row * D + (((2 * i) ^ (row >> 1 & 3)) << 3) + g] = o[i][n][e];
+          dst[row * D + (((2 * i + 1) ^ (row >> 1 & 3)) << 3) + g] = o[i][n][2 + e];
+        }
       }
-    }
   };
 
 #pragma unroll 1
@@ -383,73 +456,110 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
     cp_wait<S::kStages - 1>();
     __syncwarp();
     if (fresh) {
-      __syncthreads();   // all four warps' rows of the queries are there
+      __syncthreads();   // all warps' rows of the queries are there
       fresh = false;
+      const uint32_t qs = q_s + (c_seg & (S::kQBufs - 1)) * S::kQBytes;
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk += 2) {
+          uint32_t r[4];
+          ldsm4(r, qs + (8 * n + mrow) * D * 2 + (((kk * 2 + mat) ^ mrow) << 4));
+          q[kk][n][0] = r[0], q[kk][n][1] = r[1], q[kk + 1][n][0] = r[2], q[kk + 1][n][1] = r[3];
+        }
     }
     const uint32_t ks = ring + stage * S::kStageBytes, vs = ks + S::kHalf;
-    const uint32_t qs = q_s + (c_seg & (S::kQBufs - 1)) * S::kQBytes;
-    const uint32_t mask = masks[warp * 8 + stage] & 0xffffu;
-    if (mask) {
-      float sc[2][2][4];                        // two chains each: even and odd steps of the dimension
+    const uint32_t word = masks[warp * 4 + stage];
+    if (word) {
+      constexpr int kChains = kB * kN == 1 ? 2 : 1;   // of additions to a score, so that products overlap
+      float s[kB][kN][4];
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int j = 0; j < kB; ++j) {
+        float sc[kChains][kN][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) sc[x][n][0] = sc[x][n][1] = sc[x][n][2] = sc[x][n][3] = 0.f;
+        for (int x = 0; x < kChains; ++x)
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t a[4], b[4];
-        const int ra = (mat & 1) * 8 + mrow, rb = (mat >> 1) * 8 + mrow;
-        ldsm4(a, qs + ra * D * 2 + (((kk * 2 + (mat >> 1)) ^ mrow) << 4));
-        ldsm4(b, ks + rb * D * 2 + (((kk * 2 + (mat & 1)) ^ mrow) << 4));
-        mma<F16>(sc[kk & 1][0], a, b[0], b[1]);
-        mma<F16>(sc[kk & 1][1], a, b[2], b[3]);
-      }
-      float s[2][4];                            // [row half][key 2t, 2t + 1, 2t + 8, 2t + 9]
+          for (int n = 0; n < kN; ++n) sc[x][n][0] = sc[x][n][1] = sc[x][n][2] = sc[x][n][3] = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t a[4];
+          ldsm4(a, ks + (j * kBlock + (mat & 1) * 8 + mrow) * D * 2 + (((kk * 2 + (mat >> 1)) ^ mrow) << 4));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = e >> 1, r = 2 * h + (e & 1);
-          const bool ok = mask >> (8 * n + 2 * t + (e & 1)) & 1;
-          s[h][e] = ok ? sc[0][n][r] + sc[1][n][r] : -INFINITY;
+          for (int n = 0; n < kN; ++n) mma<F16>(sc[kk % kChains][n], a, q[kk][n][0], q[kk][n][1]);
         }
-      const int halves = p.group > 8 ? 2 : 1;
-      uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+        const uint32_t mask = word >> 16 * j & 0xffffu;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h < halves) {
-          float mx = fmaxf(fmaxf(s[h][0], s[h][1]), fmaxf(s[h][2], s[h][3]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * p.scale_log2;
-          if (__any_sync(0xffffffffu, mx > m[h])) {
-            const float m_new = fmaxf(m[h], mx);
-            const float f = m_new == m[h] ? 1.f : exp2_fast(m[h] - m_new);
-            m[h] = m_new;
-            sum[h] *= f;
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-            for (int d = 0; d < D / 8; ++d) o[d][2 * h] *= f, o[d][2 * h + 1] *= f;
-          }
-          const float shift = m[h] == -INFINITY ? 0.f : -m[h];
-          float w[4];
+          for (int e = 0; e < 4; ++e) s[j][n][e] = sc[0][n][e] + (kChains == 2 ? sc[kChains - 1][n][e] : 0.f);
+        if (mask != 0xffffu) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = exp2_fast(fmaf(s[h][e], p.scale_log2, shift));
-          sum[h] += (w[0] + w[1]) + (w[2] + w[3]);
+          for (int e = 0; e < 4; ++e)
+            if (!(mask >> (g + 8 * (e >> 1)) & 1))
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            hi[h + 2 * n] = pack<F16>(w[2 * n], w[2 * n + 1]);
-            const float2 r = unpack<F16>(hi[h + 2 * n]);
-            lo[h + 2 * n] = pack<F16>(w[2 * n] - r.x, w[2 * n + 1] - r.y);
-          }
+              for (int n = 0; n < kN; ++n) s[j][n][e] = -INFINITY;
         }
       }
+      float mx[kN][2];
+      bool grows = false;
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        uint32_t b[4];
-        ldsm4_t(b, vs + ((mat & 1) * 8 + mrow) * D * 2 + (((d * 2 + (mat >> 1)) ^ mrow) << 4));
-        mma<F16>(o[2 * d], hi, b[0], b[1]);
-        mma<F16>(o[2 * d + 1], hi, b[2], b[3]);
-        mma<F16>(o[2 * d], lo, b[0], b[1]);
-        mma<F16>(o[2 * d + 1], lo, b[2], b[3]);
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(s[0][n][e], s[0][n][2 + e]);
+#pragma unroll
+          for (int j = 1; j < kB; ++j) x = fmaxf(x, fmaxf(s[j][n][e], s[j][n][2 + e]));
+          mx[n][e] = x * p.scale_log2;
+          grows |= mx[n][e] > m[n][e];
+        }
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = mx[n][e];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float m_new = fmaxf(m[n][e], x);
+            const float f = m_new == m[n][e] ? 1.f : exp2_fast(m[n][e] - m_new);
+            m[n][e] = m_new;
+            sum[n][e] *= f;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) o[d][n][e] *= f, o[d][n][2 + e] *= f;
+          }
+      }
+      uint32_t hi[kB][kN][2], lo[kB][kN][2];
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        const float s0 = m[n][0] == -INFINITY ? 0.f : -m[n][0], s1 = m[n][1] == -INFINITY ? 0.f : -m[n][1];
+#pragma unroll
+        for (int j = 0; j < kB; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {     // keys g, g + 8
+            const float w0 = exp2_fast(fmaf(s[j][n][2 * h], p.scale_log2, s0));
+            const float w1 = exp2_fast(fmaf(s[j][n][2 * h + 1], p.scale_log2, s1));
+            sum[n][0] += w0;
+            sum[n][1] += w1;
+            const uint32_t r = pack<F16>(w0, w1);
+            const float2 back = unpack<F16>(r);
+            hi[j][n][h] = transpose(r);
+            lo[j][n][h] = transpose(pack<F16>(w0 - back.x, w1 - back.y));
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < kB; ++j) {
+        if (kB > 1 && !(word >> 16 * j & 0xffffu)) continue;   // (nothing was copied there)
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          uint32_t a[4];
+          ldsm4_t(a, vs + (j * kBlock + (mat >> 1) * 8 + mrow) * D * 2 + (((d * 2 + (mat & 1)) ^ mrow) << 4));
+#pragma unroll
+          for (int n = 0; n < kN; ++n) {
+            mma<F16>(o[d][n], a, hi[j][n][0], hi[j][n][1]);
+            mma<F16>(o[d][n], a, lo[j][n][0], lo[j][n][1]);
+          }
+        }
       }
     }
     __syncwarp();        // every lane has read the stage
@@ -492,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
       seg_first += c.tiles;
       ++c_seg;
     }
-    if (!CLUSTER || i + 1 < count) advance(p, c);
+    if (!CLUSTER || i + 1 < count) advance<D>(p, c);
     issue();
     if (CLUSTER && i + 1 == count) break;
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
@@ -500,7 +610,6 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
 
   if (CLUSTER) {
     cp_wait<0>();
-    if (count == 0) __syncthreads();   // (the queries' barrier)
     deposit();
     __syncthreads();
     const int kv = p.row_tiles == 1 ? (int)blockIdx.y : (int)blockIdx.y / p.row_tiles, r0 = ((int)blockIdx.y - kv * p.row_tiles) * kRows;
@@ -516,8 +625,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) paged_attention_ke
     }
     // where the queries were: this CTA's part, for the others to read
     float* part = reinterpret_cast<float*>(smem + S::kRing);
-    float2* ml = reinterpret_cast<float2*>(part + kRows * D);
-    static_assert(kRows * D * 4 + kRows * 8 <= S::kQBufs * S::kQBytes, "the part fits");
+    float2* ml = reinterpret_cast<float2*>(part + COLS * D);
+    static_assert(COLS * D * 4 + COLS * 8 <= S::kQBufs * S::kQBytes, "the part fits");
     for (int item = threadIdx.x; item < rows * (D / 4); item += kThreads) {
       float mx, l;
       const float4 a = merged(item, mx, l);
@@ -572,7 +681,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   for (int v = 0; v < kV; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   const int n = job.y - job.x + 1;
   if (live) {
-    constexpr int U = 4;
+    constexpr int U = 8;
 #pragma unroll 1
     for (int i0 = w; i0 < n; i0 += share * U) {
       float2 s[U];
@@ -664,9 +773,12 @@ cudaError_t allow_smem(K kernel, int bytes, int device, std::atomic<uint64_t>& d
 
 template <int D, bool F16>
 int launch_paged(Params& p, int cluster, int device, cudaStream_t stream) {
-  static std::atomic<uint64_t> done[2];
-  const auto kern = cluster ? paged_attention_kernel<D, F16, true> : paged_attention_kernel<D, F16, false>;
-  cudaError_t e = allow_smem(kern, Shape<D>::kSmem, device, done[cluster ? 1 : 0]);
+  static std::atomic<uint64_t> done[4];
+  const int wide = p.group > 8;
+  const auto kern = cluster ? wide ? paged_attention_kernel<D, F16, true, 16> : paged_attention_kernel<D, F16, true, 8>
+                            : wide ? paged_attention_kernel<D, F16, false, 16> : paged_attention_kernel<D, F16, false, 8>;
+  const int smem = wide ? Shape<D, 16>::kSmem : Shape<D, 8>::kSmem;
+  cudaError_t e = allow_smem(kern, smem, device, done[wide * 2 + (cluster ? 1 : 0)]);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -675,8 +787,8 @@ int launch_paged(Params& p, int cluster, int device, cudaStream_t stream) {
   attr[1].val.clusterDim.x = cluster ? cluster : 1;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.gridDim = cluster ? dim3(cluster, p.segments_per_seq, p.batch) : dim3(p.ctas);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Shape<D>::kSmem;
+  cfg.blockDim = dim3(Shape<D>::kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
@@ -685,7 +797,7 @@ int launch_paged(Params& p, int cluster, int device, cudaStream_t stream) {
     // jobs times rows: a block for every row while there are few, else several rows a block
     const int64_t segments = (int64_t)p.batch * p.segments_per_seq;
     const int jobs = (int)(segments < p.ctas ? segments : p.ctas);
-    int per = 8;
+    int per = kJoinThreads / 32;
     while (per > 1 && jobs * ((p.rows + per - 1) / per) < 296) per /= 2;
     cfg.gridDim = dim3(jobs, (p.rows + per - 1) / per);
     cfg.blockDim = dim3(kJoinThreads);
@@ -772,14 +884,14 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
   p.sinks = sinks < 0x7fffffff ? (int)sinks : 0x7fffffff;
   p.scale_log2 = scale_log2;
   p.rows = p.group < kRows ? p.group : kRows;
-  const int per_sm = dim == 256 ? 1 : 2;
-  p.ctas = sms * per_sm;
+  p.ctas = sms * 2;
   const int64_t segments = batch * p.segments_per_seq;
   if (cluster < 0) {
     int64_t most = wide * (int64_t)page_size;
     if (longest > 0 && longest < most) most = longest;
     if (window > 0 && window < most && window + sinks < most) most = window + sinks;
-    const int64_t tiles = (most + kTile - 1) / kTile;
+    const int64_t tile = dim == 64 ? Shape<64>::kTile : dim == 128 ? Shape<128>::kTile : Shape<256>::kTile;
+    const int64_t tiles = (most + tile - 1) / tile;
     cluster = 0;
     if (tiles <= 32) {
       cluster = 1;
