@@ -10,10 +10,11 @@
 // the bytes for every SM, enough of them in flight, and few instructions per byte.
 //   * The keys that are seen are counted through in blocks of 16 (first keys, then the window), so a mask costs nothing but at
 //     the blocks' edges: a position in that count gives the key, the key its page.
-//   * A warp is a worker of its own: it takes its blocks of a tile, copies their rows into a ring of its own with cp.async (16
-//     bytes a lane, rows found through the block table one step ahead; a block lies in one page unless pages are smaller), and
-//     keeps its own running maximum, sum and output in registers (one pass).  No barrier inside a sequence; the warps meet when
-//     a sequence's tiles end.
+//   * One warp loads: it looks the pages of 32 blocks up at a time, a batch ahead, and has the TMA unit copy the blocks (a 4-D
+//     tensor map over component, head, slot and page, so any order of them in memory) into a ring of tiles.  (With the copies
+//     in the warps that compute, cp.async a lane, a step was 460 instructions and 1300 cycles.)
+//   * The other warps are workers of their own: each takes its blocks of every tile and keeps its own running maximum, sum and
+//     output in registers (one pass).  They meet when a sequence's tiles end.
 //   * Products go through mma.sync m16n8k16 with the keys (for the scores) and the components (for the output) as the 16 rows
 //     and the query heads that share a key head as the 8 columns: half as many instructions as with the heads as rows, for up
 //     to 8 heads.  (A tcgen05 tile is 128 rows; the rate asked for here is 1 % of what those do.)
@@ -26,6 +27,10 @@
 //   stream   every CTA takes an equal part of all tiles of all sequences in a row, wherever that part begins and ends; parts
 //            of a sequence that spans CTAs go to a workspace and a second kernel, started early, adds them up in their order.
 // Both give the same bits in every run: no atomics, and parts are added in a fixed order.
+//
+// Every wait on an mbarrier is bounded by timeout_ns: on expiry the CTA records a status, the loads stop, and the other warps run
+// their loops to the end without computing, so that they meet at all their barriers.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -35,6 +40,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "iris/iris.cuh"
 #include "iris/ptx_sm100.cuh"
@@ -47,33 +53,36 @@ using namespace iris::ptx;
 constexpr int kRows = 16;                        // query heads of a segment, at most
 constexpr int kBlock = 16;                       // keys of a product
 constexpr int kJoinThreads = 512;
-constexpr uint32_t kSitePage = 95;
+constexpr uint32_t kSitePage = 95, kSiteLoad = 98, kSiteTile = 99;
 
 template <int D, int COLS = 8>
 struct Shape {
-  static constexpr int kWarps = D == 256 ? 2 : 4;
-  static constexpr int kThreads = kWarps * 32;
-  static constexpr int kBlocks = D == 64 ? 2 : 1;              // blocks of a warp's step
-  static constexpr int kWarpKeys = kBlocks * kBlock;
-  static constexpr int kTile = kWarps * kWarpKeys;             // keys of a tile
-  static constexpr int kStages = D == 256 && COLS == 16 ? 2 : 3;   // ring of a warp
-  static constexpr int kQBufs = 4;                             // queries of the segments that the ring reaches: stages + 1
-  static constexpr int kHalf = kWarpKeys * D * 2;              // keys (or values) of a stage
-  static constexpr int kStageBytes = 2 * kHalf;                // holds the fp32 output of a warp, which takes its place at the end
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kQBytes = COLS * D * 2;
+  static constexpr int kWarps = D == 256 ? 2 : 4;              // that compute; one more loads
+  static constexpr int kThreads = (kWarps + 1) * 32;
+  static constexpr int kBlocks = D == 64 ? 2 : 1;              // blocks of a warp in a tile
+  static constexpr int kTileBlocks = kWarps * kBlocks;
+  static constexpr int kTile = kTileBlocks * kBlock;           // keys of a tile
+  static constexpr int kStages = D == 256 ? 2 : 3;             // ring of tiles
+  static constexpr int kQBufs = kStages;                       // queries of the segments that the ring reaches
+  static constexpr int kPanels = D / 64;                       // a tile's keys (or values) lie in panels of 64 components,
+  static constexpr int kPanel = kTile * 128;                   // rows of 128 bytes
+  static constexpr int kStageBytes = 2 * kPanels * kPanel;     // keys, then values: 32 KB
+  static constexpr int kBlockBytes = kBlock * 128;             // a block of a panel
+  static constexpr int kQPitch = D * 2 + 16;                   // (rows 16 bytes apart in the banks)
+  static constexpr int kQBytes = COLS * kQPitch;
   static constexpr int kStats = 2 * kWarps * kRows * 4;        // maxima and sums of the warps
-  static constexpr int kMasks = kWarps * 4 * 4;                // which keys of a stage count
-  static constexpr int kSmem = kRing + kQBufs * kQBytes + kStats + kMasks + 16;
+  static constexpr int kBars = 2 * kStages * 8;
+  static constexpr int kWords = (kStages * kTileBlocks + 8) * 4;   // which keys of a block count, and a few others
+  static constexpr int kUsed = kStages * kStageBytes + kQBufs * kQBytes + kStats + kBars + kWords;
+  static constexpr int kSmem = kUsed + 1024;                   // (the ring begins on 1024 bytes)
   static constexpr int kPerSm = 2;
-  static_assert(kStages < kQBufs && kStageBytes >= COLS * D * 4, "ring");
+  static_assert(kStageBytes >= kWarps * COLS * D * 4, "ring");
   static_assert(kPerSm * (kSmem + 1024) <= 228 * 1024, "shared-memory budget");
 };
 
 struct Params {
+  CUtensorMap k, v;          // [pages, slots, key heads, components], box: 64 components of one head, a block or a page of rows
   const uint8_t* q;          // strides in bytes
-  const uint8_t* k;
-  const uint8_t* v;
   const int* table;
   const int* lens;
   uint8_t* out;
@@ -81,7 +90,8 @@ struct Params {
   StatusBlock* status;       // may be null
   float* parts;              // stream: [ctas][2][rows][D], then maxima and sums [ctas][2][rows][2]
   int4* jobs;                // stream: what the second kernel adds up
-  int64_t q_batch, q_head, page_pitch, slot_pitch, head_pitch, table_pitch, out_batch, out_head, lse_batch;
+  uint64_t timeout_ns;
+  int64_t q_batch, q_head, table_pitch, out_batch, out_head, lse_batch;
   int batch, group, row_tiles, segments_per_seq, pages, page_shift, wide, window, sinks;
   int ctas, rows;            // stream: CTAs of the first kernel; rows of a part
   float scale_log2;
@@ -91,14 +101,6 @@ __device__ __forceinline__ float exp2_fast(float x) {   // ex2.approx: 2 ulp, 2^
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {   // zeros where not taken
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -219,21 +221,38 @@ template <int D, bool F16, bool CLUSTER, int COLS>
 __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPerSm)
     paged_attention_kernel(const __grid_constant__ Params p) {
   using S = Shape<D, COLS>;
-  constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kB = S::kBlocks, kTile = S::kTile;
+  constexpr int kWarps = S::kWarps, kB = S::kBlocks, kTile = S::kTile, kTB = S::kTileBlocks;
   constexpr int kN = COLS / 8;
-  constexpr int kChunks = D / 8;             // 16-byte pieces of a row
-  constexpr int kRowsPer = 32 / kChunks;     // rows that a warp copies at a time
-  extern __shared__ __align__(128) uint8_t smem[];
-  float* stat_m = reinterpret_cast<float*>(smem + S::kRing + S::kQBufs * S::kQBytes);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_mem = smem + S::kStages * S::kStageBytes;
+  float* stat_m = reinterpret_cast<float*>(q_mem + S::kQBufs * S::kQBytes);
   float* stat_l = stat_m + kWarps * kRows;
-  volatile uint32_t* masks = reinterpret_cast<uint32_t*>(stat_l + kWarps * kRows);
-  volatile int* words = reinterpret_cast<int*>(const_cast<uint32_t*>(masks) + kWarps * 4);
+  const uint32_t bars = smem_u32(stat_l + kWarps * kRows);
+  volatile uint32_t* masks = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(stat_l + kWarps * kRows) + S::kBars);
+  volatile int* words = reinterpret_cast<int*>(const_cast<uint32_t*>(masks) + S::kStages * kTB);
+  volatile uint32_t* abort_flag = const_cast<volatile uint32_t*>(masks) + S::kStages * kTB + 4;
+  volatile uint32_t* never = abort_flag + 1;
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (S::kStages + s); };
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;     // scores: keys g and g + 8 of a block, heads 2 t and 2 t + 1
-  const uint32_t q_s = smem_u32(smem) + S::kRing;
-  const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStageBytes;
-  const float* ring_f = reinterpret_cast<const float*>(smem);
+  const uint32_t ring = smem_u32(smem), q_s = smem_u32(q_mem);
 
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&p.k);
+    prefetch_tensormap(&p.v);
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), kWarps);
+    }
+    *abort_flag = *never = 0;
+    mbar_fence_init();
+  }
+  // columns of no head are zeros
+  for (int i = threadIdx.x; i < S::kQBufs * S::kQBytes / 16; i += S::kThreads) reinterpret_cast<uint4*>(q_mem)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncthreads();
   grid_dependency_wait();
   grid_dependency_launch();
 
@@ -250,7 +269,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
     count = (int)((int64_t)c.tiles * (r + 1) / parts) - c.tile;
   } else {
     // tiles of the sequences before each thread's share of them
-    const int per = (p.batch + kThreads - 1) / kThreads;
+    const int per = (p.batch + S::kThreads - 1) / S::kThreads;
     const int b0 = min(p.batch, (int)threadIdx.x * per), b1 = min(p.batch, b0 + per);
     int64_t mine = 0;
     for (int b = b0; b < b1; ++b) mine += tiles_of<D>(seen_of(p, p.lens[b]));
@@ -265,7 +284,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
     __syncthreads();
     int64_t before = upto - mine;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w <= kWarps; ++w) {
       if (w < warp) before += sums[w];
       total += sums[w];
     }
@@ -295,93 +314,141 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
     c.tile = words[2];
   }
 
-  // ---- copies: the cursor of the loads runs a ring ahead of that of the products ----
-  Cursor l = c;
-  int l_left = count, l_stage = 0, l_seg = 0;
-  bool l_new = true;                          // the next step is its segment's first here
-  int l_page[kB];                             // pages of the next step's blocks (pages of fewer than 16: of this lane's rows)
-  auto find_pages = [&]() {
+  if (warp == kWarps) {
+    // ---- loads ----
+    // A batch: 32 blocks of one segment, a lane each: which of its keys count, its page and its first slot there.
+    constexpr int kBatch = 32 / kTB;          // tiles
+    struct Batch {
+      uint32_t mask;
+      int page, slot, key;
+    };
+    const bool whole_blocks = p.page_shift >= 4;
+    auto look_up = [&](const Cursor& at, int left) {
+      Batch b;
+      b.key = 0;
+      b.mask = left > 0 ? block_mask(at.s, at.tile * kTile + lane * kBlock, b.key) : 0;
+      b.page = 0;
+      b.slot = b.key & ((1 << p.page_shift) - 1);
+      if (whole_blocks && b.mask) b.page = p.table[at.b * p.table_pitch + (b.key >> p.page_shift)];
+      return b;
+    };
+    // the cursor of the batch behind the one at c, of `left` tiles yet to come: what the latter leaves of them
+    auto next_batch = [&](Cursor& at, int& left) {
+      const int n = min(kBatch, at.tiles - at.tile);
+      left -= n;
+      if (left <= 0) return;
+      at.tile += n - 1;
+      advance<D>(p, at);
+    };
+    Cursor l = c, ahead = c;
+    int ahead_left = count, in_batch = 0, stage = 0, q_buf = 0;
+    bool fresh = true, ok = true;             // fresh: the next tile is its segment's first here
+    Batch now = look_up(l, count);
+    next_batch(ahead, ahead_left);
+    Batch next = look_up(ahead, ahead_left);
+    int issued = 0;
+    for (; issued < count; ++issued) {
+      const int use = issued / S::kStages;
+      if (use > 0 && !mbar_wait(empty(stage), (use - 1) & 1, p.timeout_ns, abort_flag)) {
+        if (lane == 0) record_status(p.status, kTimeout, kSiteLoad, blockIdx.x, issued, 0);
+        *abort_flag = 1;
+        ok = false;
+        break;
+      }
+      const int first_lane = in_batch * kTB;
+      const bool mine = lane >= first_lane && lane < first_lane + kTB;
+      uint32_t mask = now.mask;
+      if (whole_blocks && mask && (uint32_t)now.page >= (uint32_t)p.pages) {
+        if (mine) record_status(p.status, kBadPointer, kSitePage, l.b, now.key, (uint64_t)(int64_t)now.page);
+        mask = 0;
+      }
+      const int kv = p.row_tiles == 1 ? l.seg : l.seg / p.row_tiles, r0 = (l.seg - kv * p.row_tiles) * kRows;
+      const int rows = fresh ? min(COLS, p.group - r0) : 0;
+      const uint32_t tile = ring + stage * S::kStageBytes;
+      if (whole_blocks) {
+        const uint32_t blocks = __ballot_sync(0xffffffffu, mine && mask) >> first_lane;
+        if (mine) masks[stage * kTB + lane - first_lane] = mask;
+        __syncwarp();
+        const bool one = elect_one();
+        if (one) mbar_expect_tx(full(stage), __popc(blocks) * (2 * S::kPanels * S::kBlockBytes) + rows * D * 2);
 #pragma unroll
-    for (int i = 0; i < kB; ++i) {
-      int key;
-      const uint32_t mask = l_left > 0 ? block_mask(l.s, l.tile * kTile + warp * S::kWarpKeys + i * kBlock, key) : 0;
-      if (p.page_shift < 4) key += lane & 15;
-      l_page[i] = 0;
-      if (p.page_shift < 4 ? mask >> (lane & 15) & 1 : mask != 0) l_page[i] = p.table[l.b * p.table_pitch + (key >> p.page_shift)];
-    }
-  };
-  auto issue = [&]() {
-    if (l_left > 0) {
-      const int kv = p.row_tiles == 1 ? l.seg : l.seg / p.row_tiles;
-      if (l_new) {                            // the queries, shared out over the warps; zeros where there is no head
-        const int r0 = (l.seg - kv * p.row_tiles) * kRows;
-        const uint8_t* src = p.q + l.b * p.q_batch + (int64_t)(kv * p.group + r0) * p.q_head;
-        const uint32_t dst = q_s + (l_seg & (S::kQBufs - 1)) * S::kQBytes;
+        for (int b = 0; b < kTB; ++b) {
+          const int page = __shfl_sync(0xffffffffu, now.page, first_lane + b), slot = __shfl_sync(0xffffffffu, now.slot, first_lane + b);
+          if (one && (blocks >> b & 1)) {
 #pragma unroll
-        for (int i = 0; i < (COLS / kWarps + kRowsPer - 1) / kRowsPer; ++i) {
-          const int row = warp * (COLS / kWarps) + i * kRowsPer + lane / kChunks, ch = lane % kChunks;
-          if (i * kRowsPer + lane / kChunks < COLS / kWarps) {
-            const bool take = r0 + row < p.group;
-            cp_async16(dst + row * D * 2 + ((ch ^ (row & 7)) << 4), take ? src + row * p.q_head + ch * 16 : p.q, take);
+            for (int h = 0; h < S::kPanels; ++h)
+              tma_load_4d(tile + h * S::kPanel + b * S::kBlockBytes, &p.k, h * 64, kv, slot, page, full(stage));
+#pragma unroll
+            for (int h = 0; h < S::kPanels; ++h)
+              tma_load_4d(tile + (S::kPanels + h) * S::kPanel + b * S::kBlockBytes, &p.v, h * 64, kv, slot, page, full(stage));
           }
         }
-      }
-      uint32_t word = 0;
-#pragma unroll
-      for (int i = 0; i < kB; ++i) {
-        int key;
-        uint32_t mask = block_mask(l.s, l.tile * kTile + warp * S::kWarpKeys + i * kBlock, key);
-        const int row0 = lane / kChunks, ch = lane % kChunks;
-        const uint32_t dst = ring + l_stage * S::kStageBytes + i * kBlock * D * 2 + row0 * D * 2;
-        const int64_t head = kv * p.head_pitch + ch * 16;
-        if (p.page_shift >= 4) {
-          if (mask && (uint32_t)l_page[i] >= (uint32_t)p.pages) {
-            if (lane == 0) record_status(p.status, kBadPointer, kSitePage, l.b, key, (uint64_t)(int64_t)l_page[i]);
-            mask = 0;
-          }
-          if (mask) {
-            const int64_t off = l_page[i] * p.page_pitch + ((key & ((1 << p.page_shift) - 1)) + row0) * p.slot_pitch + head;
-            const uint8_t *k = p.k + off, *v = p.v + off;
-#pragma unroll
-            for (int j = 0; j < kBlock / kRowsPer; ++j) {
-              const bool take = mask >> (j * kRowsPer + row0) & 1;
-              const uint32_t d = dst + j * kRowsPer * D * 2 + ((ch ^ ((j * kRowsPer + row0) & 7)) << 4);
-              cp_async16(d, k, take);
-              cp_async16(d + S::kHalf, v, take);
-              k += kRowsPer * p.slot_pitch;
-              v += kRowsPer * p.slot_pitch;
+        if (one && rows > 0) {
+          const uint8_t* src = p.q + l.b * p.q_batch + (int64_t)(kv * p.group + r0) * p.q_head;
+          const uint32_t dst = q_s + q_buf * S::kQBytes;
+          for (int r = 0; r < rows; ++r) bulk_load(dst + r * S::kQPitch, src + r * p.q_head, D * 2, full(stage));
+        }
+      } else {
+        // pages of fewer than 16 keys: looked up a key a lane, copied a page at a time
+        const int size = 1 << p.page_shift;
+        uint32_t bytes = 0;
+        for (int pass = 0; pass < 2; ++pass) {   // count, then copy
+          for (int b = 0; b < kTB; ++b) {
+            const uint32_t m = __shfl_sync(0xffffffffu, now.mask, first_lane + b);
+            const int key = __shfl_sync(0xffffffffu, now.key, first_lane + b) + (lane & 15);
+            const bool in = m >> (lane & 15) & 1;
+            const int page = in ? p.table[l.b * p.table_pitch + (key >> p.page_shift)] : -1;
+            const bool good = in && (uint32_t)page < (uint32_t)p.pages;
+            if (pass == 0 && in && !good) record_status(p.status, kBadPointer, kSitePage, l.b, key, (uint64_t)(int64_t)page);
+            const uint32_t got = __ballot_sync(0xffffffffu, good) & 0xffffu;
+            if (pass == 0 && lane == 0) masks[stage * kTB + b] = got;
+            for (int j = 0; j < kBlock; j += size) {
+              const uint32_t part = got >> j & ((1u << size) - 1);
+              const int from = __shfl_sync(0xffffffffu, page, part ? j + __ffs(part) - 1 : 0);
+              if (!part) continue;
+              if (pass == 0) {
+                bytes += size * 128 * 2 * S::kPanels;
+              } else if (lane == 0) {
+                const uint32_t at = tile + b * S::kBlockBytes + j * 128;
+                for (int h = 0; h < S::kPanels; ++h) {
+                  tma_load_4d(at + h * S::kPanel, &p.k, h * 64, kv, 0, from, full(stage));
+                  tma_load_4d(at + (S::kPanels + h) * S::kPanel, &p.v, h * 64, kv, 0, from, full(stage));
+                }
+              }
             }
           }
-        } else {
-          const int r = key + (lane & 15);
-          const bool in = mask >> (lane & 15) & 1, ok = in && (uint32_t)l_page[i] < (uint32_t)p.pages;
-          if (in && !ok) record_status(p.status, kBadPointer, kSitePage, l.b, r, (uint64_t)(int64_t)l_page[i]);
-          const int64_t off = ok ? l_page[i] * p.page_pitch + (r & ((1 << p.page_shift) - 1)) * p.slot_pitch : 0;
-          mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-#pragma unroll
-          for (int j = 0; j < kBlock / kRowsPer; ++j) {
-            const int row = j * kRowsPer + row0;
-            const int64_t o = __shfl_sync(0xffffffffu, off, row) + head;
-            const bool take = mask >> row & 1;
-            const uint32_t d = dst + j * kRowsPer * D * 2 + ((ch ^ (row & 7)) << 4);
-            cp_async16(d, p.k + o, take);
-            cp_async16(d + S::kHalf, p.v + o, take);
-          }
+          __syncwarp();
+          if (pass == 0 && lane == 0) mbar_expect_tx(full(stage), bytes + rows * D * 2);
         }
-        word |= mask << 16 * i;
+        if (lane == 0) {
+          const uint8_t* src = p.q + l.b * p.q_batch + (int64_t)(kv * p.group + r0) * p.q_head;
+          const uint32_t dst = q_s + q_buf * S::kQBytes;
+          for (int r = 0; r < rows; ++r) bulk_load(dst + r * S::kQPitch, src + r * p.q_head, D * 2, full(stage));
+        }
       }
-      if (lane == 0) masks[warp * 4 + l_stage] = word;
-      l_stage = l_stage + 1 == S::kStages ? 0 : l_stage + 1;
-      --l_left;
-      l_new = advance<D>(p, l);
-      if (l_new) ++l_seg;
-      find_pages();
+      __syncwarp();
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
+      fresh = advance<D>(p, l);
+      if (fresh) q_buf = q_buf + 1 == S::kQBufs ? 0 : q_buf + 1;
+      if (++in_batch == kBatch || fresh) {
+        in_batch = 0;
+        now = next;
+        next_batch(ahead, ahead_left);
+        next = look_up(ahead, ahead_left);
+      }
     }
-    cp_commit();
-  };
-  find_pages();
-#pragma unroll 1
-  for (int i = 0; i < S::kStages; ++i) issue();
+    if (!ok) {   // loads in flight still write into shared memory: wait for each, bounded
+      for (int s = 0; s < S::kStages; ++s) {
+        const int n = (issued + S::kStages - 1 - s) / S::kStages;
+        if (n > 0) mbar_wait(full(s), (n - 1) & 1, 200000, never);
+      }
+    }
+    if (CLUSTER && gridDim.x > 1) {
+      cluster_sync_all();
+      cluster_sync_all();
+    }
+    return;
+  }
 
   // ---- products ----
   float o[D / 16][kN][4], m[kN][2], sum[kN][2];   // output: components g and g + 8 of 16, heads 2 t and 2 t + 1
@@ -397,9 +464,17 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
   };
   clear();
   const int mat = lane >> 3, mrow = lane & 7;   // ldmatrix: which of the four 8 x 8 pieces this lane addresses, and its row
-  int stage = 0, c_seg = 0;
-  bool fresh = true, whole = c.tile == 0;       // whole: the segment began in this CTA
+  int stage = 0, q_buf = 0;
+  uint32_t parity = 0;
+  bool fresh = true, whole = c.tile == 0, ok = true;   // whole: the segment began in this CTA
   int64_t seg_first = first - c.tile;           // stream: its first tile among all
+  // where a warp leaves its results: its own rows of the tile it has just used up, 512 floats in each block of a panel
+  auto result_of = [&](int w, int row, int col) {
+    constexpr int kPer = 512 / D;               // rows of a block
+    const int piece = row / kPer, block = w * kB + piece % kB, panel = piece / kB;
+    return reinterpret_cast<float*>(smem + stage * S::kStageBytes + panel * S::kPanel + block * S::kBlockBytes) + (row % kPer) * D + col;
+  };
+  auto meet = [&]() { named_barrier_sync(1, kWarps * 32); };
 
   // The warps' results of a segment (whose last stage here is `stage`): sum over them of this thread's four columns of a row.
   auto merged = [&](int item, float& mx, float& l) {
@@ -413,8 +488,8 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
     for (int w = 0; w < kWarps; ++w) {
       const float mw = stat_m[w * kRows + row], lw = stat_l[w * kRows + row];
       const float f = mw == mx ? 1.f : exp2_fast(mw - mx);
-      const float4 x = *reinterpret_cast<const float4*>(ring_f + (w * S::kStages + stage) * (S::kStageBytes / 4) + row * D +
-                                                        ((((col >> 1) ^ (row >> 1 & 3)) << 3) | ((col & 1) << 2)));
+      const float4 x =
+          *reinterpret_cast<const float4*>(result_of(w, row, (((col >> 1) ^ (row >> 1 & 3)) << 3) | ((col & 1) << 2)));
       if (lw != 0.f) {    // (a warp without keys, or with keys of minus infinity only, adds nothing; one with a NaN adds that)
         l += lw * f;
         a.x += x.x * f, a.y += x.y * f, a.z += x.z * f, a.w += x.w * f;
@@ -427,9 +502,8 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
     store4<F16>(p.out + b * p.out_batch + head * p.out_head + col * 8, a, l == 0.f ? 0.f : 1.f / l);
     if (p.lse && col == 0) p.lse[b * p.lse_batch + head] = log_sum(mx, l);
   };
-  // this warp's results into the ring stage it has just used up; rows of 8-column groups in an order that keeps the banks apart
+  // this warp's results; groups of 8 columns in an order that keeps the banks apart
   auto deposit = [&]() {
-    float* dst = reinterpret_cast<float*>(smem) + (warp * S::kStages + stage) * (S::kStageBytes / 4);
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -445,32 +519,51 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-          dst[row * D + (((2 * i) ^ (row >> 1 & 3)) << 3) + g] = o[i][n][e];
-          dst[row * D + (((2 * i + 1) ^ (row >> 1 & 3)) << 3) + g] = o[i][n][2 + e];
+          *result_of(warp, row, (((2 * i) ^ (row >> 1 & 3)) << 3) + g) = o[i][n][e];
+          *result_of(warp, row, (((2 * i + 1) ^ (row >> 1 & 3)) << 3) + g) = o[i][n][2 + e];
         }
       }
   };
 
 #pragma unroll 1
   for (int i = 0; i < count; ++i) {
-    cp_wait<S::kStages - 1>();
-    __syncwarp();
-    if (fresh) {
-      __syncthreads();   // all warps' rows of the queries are there
-      fresh = false;
-      const uint32_t qs = q_s + (c_seg & (S::kQBufs - 1)) * S::kQBytes;
+    if (ok && !mbar_wait(full(stage), parity, p.timeout_ns, abort_flag)) {
+      if (lane == 0) record_status(p.status, kTimeout, kSiteTile, blockIdx.x, i, 0);
+      *abort_flag = 1;
+      ok = false;
+    }
+    if (fresh && ok) {
+      const uint32_t qs = q_s + q_buf * S::kQBytes;
 #pragma unroll
       for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int kk = 0; kk < D / 16; kk += 2) {
           uint32_t r[4];
-          ldsm4(r, qs + (8 * n + mrow) * D * 2 + (((kk * 2 + mat) ^ mrow) << 4));
+          ldsm4(r, qs + (8 * n + mrow) * S::kQPitch + ((kk * 2 + mat) << 4));
           q[kk][n][0] = r[0], q[kk][n][1] = r[1], q[kk + 1][n][0] = r[2], q[kk + 1][n][1] = r[3];
         }
     }
-    const uint32_t ks = ring + stage * S::kStageBytes, vs = ks + S::kHalf;
-    const uint32_t word = masks[warp * 4 + stage];
+    fresh = false;
+    const uint32_t ks = ring + stage * S::kStageBytes + warp * kB * S::kBlockBytes, vs = ks + S::kPanels * S::kPanel;
+    uint32_t word = 0;
+    if (ok) {
+#pragma unroll
+      for (int j = 0; j < kB; ++j) word |= masks[stage * kTB + warp * kB + j] << 16 * j;
+    }
+    bool cleared = false;
     if (word) {
+#pragma unroll
+      for (int j = 0; j < kB; ++j) {
+        const uint32_t mask = word >> 16 * j & 0xffffu;
+        if (mask && mask != 0xffffu) {   // values of keys that do not count: zeros, since zero times them has to be zero
+          for (int x = lane; x < S::kPanels * kBlock * 8; x += 32)
+            if (!(mask >> (x / 8 % kBlock) & 1))
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + (x / (8 * kBlock)) * S::kPanel + j * S::kBlockBytes +
+                                                                           x % (8 * kBlock) * 16), "r"(0) : "memory");
+          cleared = true;
+        }
+      }
+      if (cleared) __syncwarp();
       constexpr int kChains = kB * kN == 1 ? 2 : 1;   // of additions to a score, so that products overlap
       float s[kB][kN][4];
 #pragma unroll
@@ -483,7 +576,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           uint32_t a[4];
-          ldsm4(a, ks + (j * kBlock + (mat & 1) * 8 + mrow) * D * 2 + (((kk * 2 + (mat >> 1)) ^ mrow) << 4));
+          ldsm4(a, ks + (kk >> 2) * S::kPanel + (j * kBlock + (mat & 1) * 8 + mrow) * 128 + ((((kk & 3) * 2 + (mat >> 1)) ^ mrow) << 4));
 #pragma unroll
           for (int n = 0; n < kN; ++n) mma<F16>(sc[kk % kChains][n], a, q[kk][n][0], q[kk][n][1]);
         }
@@ -549,11 +642,11 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
       }
 #pragma unroll
       for (int j = 0; j < kB; ++j) {
-        if (kB > 1 && !(word >> 16 * j & 0xffffu)) continue;   // (nothing was copied there)
+        if (kB > 1 && !(word >> 16 * j & 0xffffu)) continue;   // (nothing was loaded there)
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
           uint32_t a[4];
-          ldsm4_t(a, vs + (j * kBlock + (mat >> 1) * 8 + mrow) * D * 2 + (((d * 2 + (mat & 1)) ^ mrow) << 4));
+          ldsm4_t(a, vs + (d >> 2) * S::kPanel + (j * kBlock + (mat >> 1) * 8 + mrow) * 128 + ((((d & 3) * 2 + (mat & 1)) ^ mrow) << 4));
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
             mma<F16>(o[d][n], a, hi[j][n][0], hi[j][n][1]);
@@ -562,19 +655,20 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
         }
       }
     }
-    __syncwarp();        // every lane has read the stage
+    __syncwarp();        // every lane has read the tile
 
-    const bool ends = c.tile + 1 == c.tiles;
-    if (!CLUSTER && (ends || i + 1 == count)) {
+    const bool ends = c.tile + 1 == c.tiles, last_one = i + 1 == count;
+    if (CLUSTER && last_one) break;
+    if (!CLUSTER && (ends || last_one)) {
       deposit();
-      __syncthreads();
+      meet();
       const int kv = p.row_tiles == 1 ? c.seg : c.seg / p.row_tiles, r0 = (c.seg - kv * p.row_tiles) * kRows;
       const int rows = min(kRows, p.group - r0);
       const bool direct = whole && ends;
       float* part = p.parts + ((int64_t)blockIdx.x * 2 + (whole ? 1 : 0)) * p.rows * D;
       float* ml = p.parts + (int64_t)p.ctas * 2 * p.rows * D + ((int64_t)blockIdx.x * 2 + (whole ? 1 : 0)) * p.rows * 2;
 #pragma unroll 1
-      for (int item = threadIdx.x; item < rows * (D / 4); item += kThreads) {
+      for (int item = threadIdx.x; item < rows * (D / 4); item += kWarps * 32) {
         float mx, l;
         const float4 a = merged(item, mx, l);
         const int row = item / (D / 4), col = item % (D / 4);
@@ -592,31 +686,37 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
         const int last = ends ? (int)blockIdx.x : (int)(((seg_first + c.tiles) * ctas - 1) / total);
         const int4 job = make_int4(blockIdx.x, last, ends ? -1 : c.b, c.seg);
         if (segments <= p.ctas) p.jobs[id] = job;
-        else if (!ends || i + 1 == count) p.jobs[blockIdx.x] = job;
+        else if (!ends || last_one) p.jobs[blockIdx.x] = job;
       }
-      if (threadIdx.x == 0 && !whole && i + 1 == count && p.batch * (int64_t)p.segments_per_seq > p.ctas)
+      if (threadIdx.x == 0 && !whole && last_one && p.batch * (int64_t)p.segments_per_seq > p.ctas)
         p.jobs[blockIdx.x] = make_int4(0, 0, -1, 0);
-      __syncthreads();   // the stage and the statistics are free again
+      meet();            // the tile and the statistics are free again
+      cleared = true;
       clear();
       fresh = whole = true;
       seg_first += c.tiles;
-      ++c_seg;
+      q_buf = q_buf + 1 == S::kQBufs ? 0 : q_buf + 1;
     }
-    if (!CLUSTER || i + 1 < count) advance<D>(p, c);
-    issue();
-    if (CLUSTER && i + 1 == count) break;
-    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    if (cleared) {       // (written to like ordinary memory, before the next copy into it)
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
+    if (lane == 0) mbar_arrive(empty(stage));
+    advance<D>(p, c);
+    if (++stage == S::kStages) {
+      stage = 0;
+      parity ^= 1;
+    }
   }
 
   if (CLUSTER) {
-    cp_wait<0>();
     deposit();
-    __syncthreads();
+    meet();
     const int kv = p.row_tiles == 1 ? (int)blockIdx.y : (int)blockIdx.y / p.row_tiles, r0 = ((int)blockIdx.y - kv * p.row_tiles) * kRows;
     const int rows = min(kRows, p.group - r0);
     const int parts = gridDim.x;
     if (parts == 1) {
-      for (int item = threadIdx.x; item < rows * (D / 4); item += kThreads) {
+      for (int item = threadIdx.x; item < rows * (D / 4); item += kWarps * 32) {
         float mx, l;
         const float4 a = merged(item, mx, l);
         finish(blockIdx.z, kv * p.group + r0 + item / (D / 4), item % (D / 4), a, mx, l);
@@ -624,10 +724,10 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
       return;
     }
     // where the queries were: this CTA's part, for the others to read
-    float* part = reinterpret_cast<float*>(smem + S::kRing);
+    float* part = reinterpret_cast<float*>(q_mem);
     float2* ml = reinterpret_cast<float2*>(part + COLS * D);
     static_assert(COLS * D * 4 + COLS * 8 <= S::kQBufs * S::kQBytes, "the part fits");
-    for (int item = threadIdx.x; item < rows * (D / 4); item += kThreads) {
+    for (int item = threadIdx.x; item < rows * (D / 4); item += kWarps * 32) {
       float mx, l;
       const float4 a = merged(item, mx, l);
       *reinterpret_cast<float4*>(part + item * 4) = a;
@@ -635,7 +735,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
     }
     cluster_sync_all();
     const uint32_t part_s = smem_u32(part), ml_s = smem_u32(ml);
-    for (int item = blockIdx.x * kThreads + threadIdx.x; item < rows * (D / 4); item += parts * kThreads) {
+    for (int item = blockIdx.x * kWarps * 32 + threadIdx.x; item < rows * (D / 4); item += parts * kWarps * 32) {
       const int row = item / (D / 4);
       float mx = -INFINITY, l = 0.f;
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -771,6 +871,24 @@ cudaError_t allow_smem(K kernel, int bytes, int device, std::atomic<uint64_t>& d
   return e;
 }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, []() {
+    void* q = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) == cudaSuccess &&
+        r == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(q);
+    else
+      (void)cudaGetLastError();
+  });
+  return fn;
+}
+
 template <int D, bool F16>
 int launch_paged(Params& p, int cluster, int device, cudaStream_t stream) {
   static std::atomic<uint64_t> done[4];
@@ -827,7 +945,7 @@ struct IrisPagedAttentionArgs {
   const void *q, *k, *v, *table, *lens;
   void *out, *lse, *work, *status, *stream;
   int64_t q_batch, q_head, page_pitch, slot_pitch, head_pitch, table_pitch, out_batch, out_head, lse_batch;
-  int64_t batch, heads, dim, pages, page_size, kv_heads, wide, dtype, window, sinks, longest, cluster, work_bytes, device;
+  int64_t batch, heads, dim, pages, page_size, kv_heads, wide, dtype, window, sinks, longest, cluster, work_bytes, device, timeout_ns;
   double scale;
 };
 
@@ -837,7 +955,7 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
   g_paged_err[0] = 0;
   const auto [q, k, v, table, lens, out, lse, work, status, stream, q_batch0, q_head0, page_pitch0, slot_pitch0, head_pitch0,
               table_pitch0, out_batch0, out_head0, lse_batch0, batch, heads, dim, pages, page_size, kv_heads, wide, dtype, window,
-              sinks, longest, cluster0, work_bytes, device, scale] = *args;
+              sinks, longest, cluster0, work_bytes, device, timeout_ns, scale] = *args;
   int64_t q_batch = q_batch0, q_head = q_head0, page_pitch = page_pitch0, slot_pitch = slot_pitch0, head_pitch = head_pitch0;
   int64_t table_pitch = table_pitch0, out_batch = out_batch0, out_head = out_head0, lse_batch = lse_batch0, cluster = cluster0;
   if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > (1 << 20)) return refuse("query heads must be a multiple of key heads");
@@ -856,20 +974,40 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
        reinterpret_cast<uintptr_t>(out)) % 16 || (q_batch | q_head | page_pitch | slot_pitch | head_pitch | out_batch | out_head) % 8)
     return refuse("rows of q, k, v and out must start on 16 bytes");
+  if ((pages > 1 && page_pitch < dim) || (page_size > 1 && slot_pitch < dim) || (kv_heads > 1 && head_pitch < dim))
+    return refuse("rows of the cache must not overlap");
   const int sms = sms_of((int)device);
   if (sms < 1) return refuse("no device");
   Params p;
   memset(&p, 0, sizeof(p));
   p.q = static_cast<const uint8_t*>(q);
-  p.k = static_cast<const uint8_t*>(k);
-  p.v = static_cast<const uint8_t*>(v);
   p.table = static_cast<const int*>(table);
   p.lens = static_cast<const int*>(lens);
   p.out = static_cast<uint8_t*>(out);
   p.lse = static_cast<float*>(lse);
   p.status = static_cast<iris::StatusBlock*>(status);
   p.q_batch = q_batch * 2, p.q_head = q_head * 2;
-  p.page_pitch = page_pitch * 2, p.slot_pitch = slot_pitch * 2, p.head_pitch = head_pitch * 2;
+  const EncodeTiledFn encode = encode_fn();
+  if (!encode) return refuse("cuTensorMapEncodeTiled is not available");
+  {
+    // (a pitch along one element has to be a legal one all the same)
+    const auto pitch = [row = dim * 2](int64_t x) { return (cuuint64_t)(x ? x * 2 : row); };
+    const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)kv_heads, (cuuint64_t)page_size, (cuuint64_t)pages};
+    const cuuint64_t strides[3] = {pitch(head_pitch), pitch(slot_pitch), pitch(page_pitch)};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)(page_size < kBlock ? page_size : kBlock), 1}, ones[4] = {1, 1, 1, 1};
+    const auto type = dtype ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int i = 0; i < 2; ++i) {
+      const CUresult r = encode(i ? &p.v : &p.k, type, 4, const_cast<void*>(i ? v : k), dims, strides, box, ones,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                dim == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      if (r != CUDA_SUCCESS) {
+        snprintf(g_paged_err, sizeof(g_paged_err), "paged attention: cuTensorMapEncodeTiled failed with %d", (int)r);
+        return -2;
+      }
+    }
+  }
+  p.timeout_ns = timeout_ns > 0 ? (uint64_t)timeout_ns : 2000000000ull;
   p.table_pitch = table_pitch;
   p.out_batch = out_batch * 2, p.out_head = out_head * 2;
   p.lse_batch = lse_batch;

@@ -19,7 +19,7 @@ from .. import _native
 
 _DT = {torch.bfloat16: 0, torch.float16: 1}
 _P, _L, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
-_ATTENTION, _RESERVE = struct.Struct("@33qd"), struct.Struct("@17q")
+_ATTENTION, _RESERVE = struct.Struct("@34qd"), struct.Struct("@17q")
 _RELEASE = [_P, _P, _P, _L, _L, _P, _L, _P, _I, _L, _P]
 
 
@@ -46,7 +46,7 @@ def same_strides(a: torch.Tensor, b: torch.Tensor) -> bool:
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                     lens: torch.Tensor, out: torch.Tensor, *, window: int = 0, sinks: int = 0, scale: Optional[float] = None,
                     lse: Optional[torch.Tensor] = None, longest: Optional[int] = None, status: Optional[torch.Tensor] = None,
-                    stream=None) -> torch.Tensor:
+                    timeout_ms: float = 2000.0, stream=None) -> torch.Tensor:
     """Attention of every sequence's newest token over its cached keys and values.
 
     ``q`` and ``out`` are ``[batch, heads, head_dim]`` (any strides with contiguous heads, e.g. the query columns of a
@@ -59,7 +59,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     A sequence of no keys gets zeros (and minus infinity in ``lse``).  Memory behind a sequence's last key is not looked at.  A
     key whose table entry is no page is left out and recorded in ``status`` (an ``Iris`` context's status block) if that is
-    given.  ``longest``: what the lengths are expected not to exceed, where that is much less than the table's width; it is
+    given, as is a bounded wait of the kernel that ran out.  ``longest``: what the lengths are expected not to exceed, where that is much less than the table's width; it is
     for speed alone.
     """
     dtype, shape, cache_shape = q.dtype, q.shape, k_cache.shape
@@ -108,7 +108,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if device != _native.current_device(device):
         with torch.cuda.device(device):
             return paged_attention(q, k_cache, v_cache, block_table, lens, out, window=window, sinks=sinks, scale=scale, lse=lse,
-                                   longest=longest, status=status, stream=stream)
+                                   longest=longest, status=status, timeout_ms=timeout_ms, stream=stream)
     fn = _native.entry("iris_k_paged_attention")
     current = torch._C._cuda_getCurrentRawStream(device)
     work, work_ptr, work_bytes = None, 0, 0
@@ -117,7 +117,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lens.data_ptr(), out.data_ptr(), lse_ptr,
             work_ptr, status_ptr, current if stream is None else stream, q_batch, q_head, page, slot, head, table_pitch, out_batch,
             out_head, lse_batch, batch, heads, dim, pages, size, kv_heads, table_shape[1], _DT[dtype], window, sinks, longest or 0,
-            -1, work_bytes, device, dim ** -0.5 if scale is None else scale))
+            -1, work_bytes, device, int(timeout_ms * 1e6), dim ** -0.5 if scale is None else scale))
         if rc <= 0 or work_bytes:
             break
         # sums of sequences that several CTAs share, of this call alone
