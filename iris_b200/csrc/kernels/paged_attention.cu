@@ -26,6 +26,9 @@
 //            memory: one launch, no workspace.  For sequences of few tiles.
 //   stream   every CTA takes an equal part of all tiles of all sequences in a row, wherever that part begins and ends; parts
 //            of a sequence that spans CTAs go to a workspace and a second kernel, started early, adds them up in their order.
+//            Neighbouring heads, whose rows are neighbours in memory where the slot comes before the head, belong to CTAs that
+//            run side by side through the same keys (`lanes`), which DRAM rewards: 256 sequences of up to 2000 keys, 32 heads of
+//            64, 437 us with the heads one behind the other.
 // Both give the same bits in every run: no atomics, and parts are added in a fixed order.
 //
 // Every wait on an mbarrier is bounded by timeout_ns: on expiry the CTA records a status, the loads stop, and the other warps run
@@ -93,7 +96,8 @@ struct Params {
   uint64_t timeout_ns;
   int64_t q_batch, q_head, table_pitch, out_batch, out_head, lse_batch;
   int batch, group, row_tiles, segments_per_seq, pages, page_shift, wide, window, sinks;
-  int ctas, rows;            // stream: CTAs of the first kernel; rows of a part
+  int lanes, turns;          // segments of a sequence (key head and row tile) = turns * lanes: number turn * lanes + lane
+  int groups, rows;          // stream: CTA g * lanes + lane of the first kernel takes the g-th part of the lane's tiles; rows of a part
   float scale_log2;
 };
 
@@ -173,7 +177,7 @@ __device__ __forceinline__ int tiles_of(const Seen& s) {   // a sequence without
   return t ? t : 1;
 }
 
-// Where a worker is: tile `tile` of `tiles` of segment `seg` (key head and row tile) of sequence b.
+// Where a worker is: tile `tile` of `tiles` of the segment that is its lane's in turn `seg` of sequence b.
 struct Cursor {
   Seen s;
   int b, seg, tile, tiles, next_len;
@@ -189,7 +193,7 @@ template <int D>
 __device__ __forceinline__ bool advance(const Params& p, Cursor& c) {
   if (++c.tile < c.tiles) return false;
   c.tile = 0;
-  if (++c.seg == p.segments_per_seq) {
+  if (++c.seg == p.turns) {
     c.seg = 0;
     if (++c.b < p.batch) enter<D>(p, c, c.next_len);
   }
@@ -259,10 +263,12 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
   // ---- this CTA's tiles: from cursor c on, `count` of them ----
   Cursor c;
   int64_t first = 0, total = 0;              // stream: its first tile among all
-  int count, ctas = 1;
+  int count, groups = 1;
+  const int lane_of = CLUSTER ? blockIdx.y : blockIdx.x % p.lanes, my_group = CLUSTER ? 0 : blockIdx.x / p.lanes;
+  auto segment_of = [&](const Cursor& at) { return at.seg * p.lanes + lane_of; };
   if (CLUSTER) {
     c.b = blockIdx.z;
-    c.seg = blockIdx.y;
+    c.seg = 0;
     enter<D>(p, c, p.lens[c.b]);
     const int parts = gridDim.x, r = blockIdx.x;
     c.tile = (int)((int64_t)c.tiles * r / parts);
@@ -288,29 +294,32 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
       if (w < warp) before += sums[w];
       total += sums[w];
     }
-    total *= p.segments_per_seq;
-    before *= p.segments_per_seq;
-    mine *= p.segments_per_seq;
-    ctas = (int)min((int64_t)p.ctas, total);   // with a tile each at least: a part from every CTA that a segment spans
-    if ((int)blockIdx.x >= ctas) return;       // (then the jobs are listed by segment)
-    first = total * blockIdx.x / ctas;
-    count = (int)(total * (blockIdx.x + 1) / ctas - first);
+    total *= p.turns;
+    before *= p.turns;
+    mine *= p.turns;
+    groups = (int)min((int64_t)p.groups, total);   // with a tile each at least: a part from every CTA that a segment spans
+    if (my_group >= groups) return;                // (then the jobs are listed by segment)
+    first = total * my_group / groups;
+    count = (int)(total * (my_group + 1) / groups - first);
     if (mine > 0 && before <= first && first < before + mine) {
       int64_t left = first - before;
-      int b = b0, n;
+      int b = b0, n, len;
       for (;; ++b) {
-        n = tiles_of<D>(seen_of(p, p.lens[b]));
-        if (left < (int64_t)n * p.segments_per_seq) break;
-        left -= (int64_t)n * p.segments_per_seq;
+        len = p.lens[b];
+        n = tiles_of<D>(seen_of(p, len));
+        if (left < (int64_t)n * p.turns) break;
+        left -= (int64_t)n * p.turns;
       }
+      const int turn = p.turns == 1 ? 0 : (int)(left / n);
       words[0] = b;
-      words[1] = (int)(left / n);
-      words[2] = (int)(left % n);
+      words[1] = turn;
+      words[2] = (int)(left - (int64_t)turn * n);
+      words[3] = len;
     }
     __syncthreads();
     c.b = words[0];
     c.seg = words[1];
-    enter<D>(p, c, p.lens[c.b]);
+    enter<D>(p, c, words[3]);
     c.tile = words[2];
   }
 
@@ -362,7 +371,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
         if (mine) record_status(p.status, kBadPointer, kSitePage, l.b, now.key, (uint64_t)(int64_t)now.page);
         mask = 0;
       }
-      const int kv = p.row_tiles == 1 ? l.seg : l.seg / p.row_tiles, r0 = (l.seg - kv * p.row_tiles) * kRows;
+      const int seg = segment_of(l), kv = p.row_tiles == 1 ? seg : seg / p.row_tiles, r0 = (seg - kv * p.row_tiles) * kRows;
       const int rows = fresh ? min(COLS, p.group - r0) : 0;
       const uint32_t tile = ring + stage * S::kStageBytes;
       if (whole_blocks) {
@@ -662,11 +671,11 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
     if (!CLUSTER && (ends || last_one)) {
       deposit();
       meet();
-      const int kv = p.row_tiles == 1 ? c.seg : c.seg / p.row_tiles, r0 = (c.seg - kv * p.row_tiles) * kRows;
+      const int seg = segment_of(c), kv = p.row_tiles == 1 ? seg : seg / p.row_tiles, r0 = (seg - kv * p.row_tiles) * kRows;
       const int rows = min(kRows, p.group - r0);
       const bool direct = whole && ends;
       float* part = p.parts + ((int64_t)blockIdx.x * 2 + (whole ? 1 : 0)) * p.rows * D;
-      float* ml = p.parts + (int64_t)p.ctas * 2 * p.rows * D + ((int64_t)blockIdx.x * 2 + (whole ? 1 : 0)) * p.rows * 2;
+      float* ml = p.parts + (int64_t)gridDim.x * 2 * p.rows * D + ((int64_t)blockIdx.x * 2 + (whole ? 1 : 0)) * p.rows * 2;
 #pragma unroll 1
       for (int item = threadIdx.x; item < rows * (D / 4); item += kWarps * 32) {
         float mx, l;
@@ -682,13 +691,13 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
       if (threadIdx.x == 0 && whole) {
         // what the second kernel adds up: a segment's parts from this CTA to that of its last tile; listed by segment
         // where there are fewer of them than CTAs, else by the CTA in which it begins
-        const int64_t segments = (int64_t)p.batch * p.segments_per_seq, id = (int64_t)c.b * p.segments_per_seq + c.seg;
-        const int last = ends ? (int)blockIdx.x : (int)(((seg_first + c.tiles) * ctas - 1) / total);
-        const int4 job = make_int4(blockIdx.x, last, ends ? -1 : c.b, c.seg);
-        if (segments <= p.ctas) p.jobs[id] = job;
+        const int64_t segments = (int64_t)p.batch * p.segments_per_seq, id = (int64_t)c.b * p.segments_per_seq + seg;
+        const int last = ends ? my_group : (int)(((seg_first + c.tiles) * groups - 1) / total);
+        const int4 job = make_int4(my_group, last, ends ? -1 : c.b, seg);
+        if (segments <= gridDim.x) p.jobs[id] = job;
         else if (!ends || last_one) p.jobs[blockIdx.x] = job;
       }
-      if (threadIdx.x == 0 && !whole && last_one && p.batch * (int64_t)p.segments_per_seq > p.ctas)
+      if (threadIdx.x == 0 && !whole && last_one && p.batch * (int64_t)p.segments_per_seq > gridDim.x)
         p.jobs[blockIdx.x] = make_int4(0, 0, -1, 0);
       meet();            // the tile and the statistics are free again
       cleared = true;
@@ -757,7 +766,84 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
   }
 }
 
-// Second kernel of the stream form: the parts of a segment that spans CTAs, in their order.  A warp takes 128 columns of a
+// Second kernel of the stream form where few segments span many CTAs each: a block adds up 32 columns of a row, 8 lanes to a
+// part, so that all parts of the row are on their way at once.  (2 x 8 rows of 148 parts, a block of 16 warps to a row and a warp
+// to every 16th part: 28.7 us for the whole call instead of 26.7.)
+template <int D, bool F16>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_long_kernel(const __grid_constant__ Params p) {
+  constexpr int kTeams = kJoinThreads / 8, U = 4;
+  __shared__ float4 acc[kJoinThreads / 32][8];
+  __shared__ float2 stats[kJoinThreads / 32];
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int4 job = p.jobs[blockIdx.x];
+  if (job.z < 0) return;
+  const int kv = job.w / p.row_tiles, r0 = (job.w - kv * p.row_tiles) * kRows, row = blockIdx.y;
+  if (row >= min(kRows, p.group - r0)) return;
+  const int team = threadIdx.x / 8, c = threadIdx.x % 8, col = blockIdx.z * 32 + c * 4, lane_of = job.w % p.lanes;
+  const float* ml = p.parts + (int64_t)p.groups * p.lanes * 2 * p.rows * D;
+  const int n = job.y - job.x + 1;
+  float mx = -INFINITY, l = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i0 = team; i0 < n; i0 += kTeams * U) {
+    float2 s[U];
+    float4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kTeams;
+      s[u] = make_float2(-INFINITY, 0.f);
+      if (i < n) {
+        const int64_t slot = ((int64_t)((job.x + i) * p.lanes + lane_of) * 2 + (i == 0 ? 1 : 0)) * p.rows + row;
+        s[u] = *reinterpret_cast<const float2*>(ml + slot * 2);
+        x[u] = *reinterpret_cast<const float4*>(p.parts + slot * D + col);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s[u].y == 0.f) continue;
+      float fo, fr;
+      join(mx, l, s[u].x, s[u].y, fo, fr);
+      add(a, fo, x[u], fr);
+    }
+  }
+  // the four teams of a warp, then the warps, four at a time
+  auto over_teams = [&]() {
+#pragma unroll
+    for (int o = 8; o < 32; o *= 2) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, mx, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+      const float4 x = make_float4(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o),
+                                   __shfl_xor_sync(0xffffffffu, a.z, o), __shfl_xor_sync(0xffffffffu, a.w, o));
+      if (l2 != 0.f) {
+        float fo, fr;
+        join(mx, l, m2, l2, fo, fr);
+        add(a, fo, x, fr);
+      }
+    }
+  };
+  over_teams();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane < 8) acc[warp][lane] = a;
+  if (lane == 0) stats[warp] = make_float2(mx, l);
+  __syncthreads();
+  if (warp != 0) return;
+  mx = -INFINITY, l = 0.f;
+  a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int w = lane / 8; w < kJoinThreads / 32; w += 4) {
+    const float2 s = stats[w];
+    if (s.y == 0.f) continue;
+    float fo, fr;
+    join(mx, l, s.x, s.y, fo, fr);
+    add(a, fo, acc[w][c], fr);
+  }
+  over_teams();
+  if (lane >= 8) return;
+  const int head = kv * p.group + r0 + row;
+  store4<F16>(p.out + job.z * p.out_batch + head * p.out_head + col * 2, a, l == 0.f ? 0.f : 1.f / l);
+  if (p.lse && col == 0) p.lse[job.z * p.lse_batch + head] = log_sum(mx, l);
+}
+
+// The same for more segments, of fewer parts each: the parts of a segment that spans CTAs, in their order.  A warp takes 128 columns of a
 // row (`rows_per` rows a block); the block's warps share out the parts of a row where there are fewer rows than warps.
 template <int D, bool F16>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ Params p, int rows_per) {
@@ -774,7 +860,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   const int row = blockIdx.y * rows_per + warp / share, w = warp % share;
   const int kv = job.w / p.row_tiles, r0 = (job.w - kv * p.row_tiles) * kRows;
   const bool live = row < min(kRows, p.group - r0);
-  const float* ml = p.parts + (int64_t)p.ctas * 2 * p.rows * D;
+  const int lane_of = job.w % p.lanes;
+  const float* ml = p.parts + (int64_t)p.groups * p.lanes * 2 * p.rows * D;
   float mx = -INFINITY, l = 0.f;
   float4 a[kV];
 #pragma unroll
@@ -791,7 +878,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         const int i = i0 + u * share;
         s[u] = make_float2(-INFINITY, 0.f);
         if (i < n) {
-          const int64_t slot = ((int64_t)(job.x + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + row;
+          const int64_t slot = ((int64_t)((job.x + i) * p.lanes + lane_of) * 2 + (i == 0 ? 1 : 0)) * p.rows + row;
           s[u] = *reinterpret_cast<const float2*>(ml + slot * 2);
 #pragma unroll
           for (int v = 0; v < kV; ++v)
@@ -889,6 +976,23 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// CTAs of a cluster, or 0 for the stream form, for so many segments of at most so many tiles on a GPU that holds `resident` CTAs.
+// A tile takes a CTA alone 0.67 us.  The stream form shares any lengths out evenly, but begins with sums over all lengths and
+// ends with a second kernel.  us, 4 query heads of 128 to a key head, pages of 16 (cluster of 1 / 2 / 4 / 8, stream):
+//      8 segments   64 keys 3.5 / 4.5 / 4.9 / 5.5, 5.9    1024 keys 13.7 / 9.2 / 7.2 / 7.1, 8.5    4096 keys 47 / 26 / 15 / 11, 9.8
+//    128 segments   256 keys 5.7 / 6.1 / 10.9 / 23, 14    1024 keys 14.7 / 11.1 / 15.7 / 30, 19    4096 keys 49 / 31 / 32 / 43, 33
+//    512 segments   256 keys 14 / 24 / 45 / 100, 18       1024 keys 32 / 39 / 60 / 118, 34         4096 keys 108 / 97 / 109 / 169, 94
+//   2048 segments   64 keys 30 / 73 / 153 / 359, 20       512 keys 58.5 / 99 / 188 / 418, 58       1024 keys 99.6 / 133 / ..., 102
+int choose_cluster(int64_t segments, int64_t tiles, int resident) {
+  if (segments > 4 * resident) return 0;                       // many short ones: a CTA for each costs more than it works
+  if (segments > resident) return tiles <= 20 ? 1 : 0;         // more than one round of CTAs, the last of them not full
+  int cluster = 1;
+  while (cluster < 8 && cluster < tiles && segments * cluster * 2 <= resident) cluster *= 2;
+  // the chain of a CTA's tiles against the stream form's, which is longer by 4.8 tiles' time for its beginning and end; uneven
+  // lengths speak for the latter, the more the longer they are
+  return tiles <= 128 && (double)tiles / cluster <= 4.8 + 1.1 * segments * tiles / resident ? cluster : 0;
+}
+
 template <int D, bool F16>
 int launch_paged(Params& p, int cluster, int device, cudaStream_t stream) {
   static std::atomic<uint64_t> done[4];
@@ -904,7 +1008,8 @@ int launch_paged(Params& p, int cluster, int device, cudaStream_t stream) {
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = cluster ? cluster : 1;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = cluster ? dim3(cluster, p.segments_per_seq, p.batch) : dim3(p.ctas);
+  const int ctas = p.groups * p.lanes;
+  cfg.gridDim = cluster ? dim3(cluster, p.segments_per_seq, p.batch) : dim3(ctas);
   cfg.blockDim = dim3(Shape<D>::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -912,16 +1017,21 @@ int launch_paged(Params& p, int cluster, int device, cudaStream_t stream) {
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kern, (const Params)p);
   if (e == cudaSuccess && !cluster) {
-    // jobs times rows: a block for every row while there are few, else several rows a block
     const int64_t segments = (int64_t)p.batch * p.segments_per_seq;
-    const int jobs = (int)(segments < p.ctas ? segments : p.ctas);
-    int per = kJoinThreads / 32;
-    while (per > 1 && jobs * ((p.rows + per - 1) / per) < 296) per /= 2;
-    cfg.gridDim = dim3(jobs, (p.rows + per - 1) / per);
+    const int jobs = (int)(segments < ctas ? segments : ctas);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<D, F16>, (const Params)p, per);
+    if (jobs * 16 <= ctas) {
+      cfg.gridDim = dim3(jobs, p.rows, D / 32);
+      e = cudaLaunchKernelEx(&cfg, paged_join_long_kernel<D, F16>, (const Params)p);
+    } else {
+      // a block for every row while there are few, else several rows a block
+      int per = kJoinThreads / 32;
+      while (per > 1 && jobs * ((p.rows + per - 1) / per) < ctas) per /= 2;
+      cfg.gridDim = dim3(jobs, (p.rows + per - 1) / per);
+      e = cudaLaunchKernelEx(&cfg, paged_join_kernel<D, F16>, (const Params)p, per);
+    }
   }
   if (e != cudaSuccess) {
     (void)cudaGetLastError();   // reported here: it must not turn up at someone else's launch
@@ -1022,7 +1132,13 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
   p.sinks = sinks < 0x7fffffff ? (int)sinks : 0x7fffffff;
   p.scale_log2 = scale_log2;
   p.rows = p.group < kRows ? p.group : kRows;
-  p.ctas = sms * 2;
+  // lanes: as many of a sequence's segments side by side as leave no more than one CTA in 32 without work
+  const int resident = sms * 2;
+  p.lanes = 1;
+  for (int n = 2; n <= p.segments_per_seq && n <= resident; ++n)
+    if (p.segments_per_seq % n == 0 && resident / n * n * 32 >= resident * 31) p.lanes = n;
+  p.turns = p.segments_per_seq / p.lanes;
+  p.groups = resident / p.lanes;
   const int64_t segments = batch * p.segments_per_seq;
   if (cluster < 0) {
     int64_t most = wide * (int64_t)page_size;
@@ -1030,19 +1146,18 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
     if (window > 0 && window < most && window + sinks < most) most = window + sinks;
     const int64_t tile = dim == 64 ? Shape<64>::kTile : dim == 128 ? Shape<128>::kTile : Shape<256>::kTile;
     const int64_t tiles = (most + tile - 1) / tile;
-    cluster = 0;
-    if (tiles <= 32) {
-      cluster = 1;
-      while (cluster < 8 && cluster < tiles && segments * cluster < p.ctas) cluster *= 2;
-    }
+    cluster = choose_cluster(segments, tiles, resident);
   }
   if (batch > 65535 || p.segments_per_seq > 65535) cluster = 0;
   if (cluster == 0) {
-    const int64_t need = (int64_t)p.ctas * (16 + 2 * p.rows * (dim + 2) * 4);
+    const int64_t ctas = (int64_t)p.groups * p.lanes, need = ctas * (16 + 2 * p.rows * (dim + 2) * 4);
     if (!work || work_bytes < need) return (int)need;
     p.jobs = static_cast<int4*>(work);
-    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + (int64_t)p.ctas * 16);
-  } else if (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) {
+    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ctas * 16);
+  } else {
+    p.lanes = p.turns = 1;   // (a CTA's lane is its block's y)
+  }
+  if (cluster != 0 && cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) {
     return refuse("a cluster has 1, 2, 4 or 8 CTAs");
   }
   const auto st = static_cast<cudaStream_t>(stream);
