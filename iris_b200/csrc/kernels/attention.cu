@@ -78,6 +78,10 @@ static_assert(kSmemBytes <= 227 * 1024, "shared-memory budget");
 // nothing from it.
 constexpr int kPolyEvery = 4;
 
+// Up to so many first keys make a tile of their own width instead of a whole one (2 x 8192 tokens, 32 heads, window 1024, 4 first
+// keys: with whole tiles, and with side B going through the tile that it sees nothing of, 400 us).
+constexpr int kNarrow = 32;
+
 enum Site : uint32_t { kSiteLoad = 90, kSiteMma = 91, kSiteSoftmax = 92 };
 
 // 2^x on the special-function unit (ex2.approx: 2 ulp, 2^-inf = 0), which is what bounds the softmax warps.
@@ -182,7 +186,14 @@ struct Params {
 struct Item {
   int bh, qa, n, na, nb;
   int ns, w0;            // windows: the first ns tiles of the list are key tiles 0 .. ns - 1, then w0, w0 + 1, ...
+  int skip;              // 1: side B (of a pair) sees no key of tile w0
+  bool narrow;           // the list's first tile counts with its first kNarrow keys only
 };
+// Which tile of the list side x uses in its step j.
+template <bool SPLIT, bool WIN>
+__device__ __forceinline__ int list_index(const Item& it, int x, int j) {
+  return SPLIT ? 2 * j + x : WIN && x == 1 && j >= it.ns ? j + it.skip : j;
+}
 // Key tile i of the list.
 template <bool WIN>
 __device__ __forceinline__ int listed_tile(const Item& it, int i) { return WIN && i >= it.ns ? i - it.ns + it.w0 : i; }
@@ -212,10 +223,13 @@ __device__ __forceinline__ bool item_of(const Params& p, int r, Item& it) {
       it.na = (n + 1) / 2;
       it.nb = n / 2;
     } else {
+      const int sink_tiles = (p.sinks + BKV - 1) / BKV;
+      it.skip = it.ns == sink_tiles && it.w0 * BKV + BKV <= oldest + BQ ? 1 : 0;
       it.na = n;
-      it.nb = it.qa + 1 < nq ? n + 1 : 0;
+      it.nb = it.qa + 1 < nq ? n + 1 - it.skip : 0;
       it.n = it.nb ? n + 1 : n;
     }
+    it.narrow = it.ns == 1 && p.sinks <= kNarrow;
   } else if (SPLIT) {
     it.qa = q;
     it.n = p.causal ? q + 1 : nq;
@@ -362,6 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
   } else if (warp == 9) {
     if (elect_one()) {   // elect.sync, not a lane number: see the same place in gemm_local.cu
       constexpr uint32_t idesc_qk = umma_idesc_f16_major(BQ, BKV, !F16, false, false);
+      constexpr uint32_t idesc_narrow = umma_idesc_f16_major(BQ, kNarrow, !F16, false, false);
       constexpr uint32_t idesc_pv = umma_idesc_f16_major(BQ, D, !F16, false, true);   // V is MN-major
       bool ok = true;
       uint32_t base = 0;                      // ring position of the current item's first tile
@@ -376,12 +391,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
       };
       auto pos_k = [&](int i) { return (uint32_t)(i + (i >= lead ? i - lead + 1 : 0)); };
       auto pos_v = [&](const Item& it, int i) { return (uint32_t)(i + (i + lead < it.n ? i + lead : it.n)); };
-      auto key_tile = [&](int x, int j) { return SPLIT ? 2 * j + x : j; };
-      // a tile's slot is free after its last use: side B's where both sides use it
-      auto last_use = [&](const Item& it, int x, int j) { return SPLIT || x == 1 || j >= it.nb; };
+      auto key_tile = [&](const Item& it, int x, int j) { return list_index<SPLIT, WIN>(it, x, j); };
+      // a tile's slot is free after its last use: side B's where both sides use it in one step; where side B skips a tile it is
+      // a step ahead from there on, and side A is the last to use what it uses
+      auto last_use = [&](const Item& it, int x, int j) {
+        if (SPLIT) return true;
+        if (WIN && it.nb > 0 && it.skip && j >= it.ns) return x == 0 || j + 1 >= it.na;
+        return x == 1 || j >= it.nb;
+      };
       // S = Q K_j^T of side x; `first` = ring position of the item's first tile
       auto scores = [&](const Item& it, uint32_t first, int x, int j) {
-        const int kt = key_tile(x, j);
+        const int kt = key_tile(it, x, j);
         const uint32_t pos = first + pos_k(kt);
         const int s = pos % kSlots;
         if (!mbar_wait(kv_full(s), (pos / kSlots) & 1, p.timeout_ns, abort_flag)) return stop(1);
@@ -391,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
-          umma_f16_ss(tmem + x * 128, qd + off, kd + off, idesc_qk, kk ? 1u : 0u);
+          umma_f16_ss(tmem + x * 128, qd + off, kd + off, WIN && it.narrow && kt == 0 ? idesc_narrow : idesc_qk, kk ? 1u : 0u);
         }
         umma_commit(s_full(x));
         if (last_use(it, x, j)) umma_commit(kv_empty(s));
@@ -436,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
               }
               ++on[x];
             }
-            const uint32_t pos = base + pos_v(it, key_tile(x, j));
+            const uint32_t pos = base + pos_v(it, key_tile(it, x, j));
             const int s = pos % kSlots;
             if (!mbar_wait(kv_full(s), (pos / kSlots) & 1, p.timeout_ns, abort_flag) ||
                 !mbar_wait(p_half(x), sn[x] & 1, p.timeout_ns, abort_flag)) {
@@ -446,10 +466,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
             tc_fence_after();
             // 16 keys = two groups of 8 rows (1024 bytes apart); the second 64 columns of d are one half tile further on
             const uint64_t vd = umma_desc_mn_sw128(ring + s * kTileBytes, kHalfBytes, 1024);
+            const bool narrow = WIN && it.narrow && key_tile(it, x, j) == 0;
             auto product = [&](int k0) {   // 64 keys
 #pragma unroll
               for (int kk = k0; kk < k0 + BKV / 32; ++kk)
-                umma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, vd + kk * (16 * 128 >> 4), idesc_pv,
+                if (!narrow || kk < kNarrow / 16) umma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, vd + kk * (16 * 128 >> 4), idesc_pv,
                             (j > 0 || kk > 0) ? 1u : 0u);
             };
             product(0);   // runs while the other half's exponentials are made
@@ -467,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
               umma_commit(o_full(x));
               // go on with the next item on this side if its operands are there already
               if (more && (x == 0 || (nx.nb > 0 && ahead[0]))) {   // (B never before A: see last_use)
-                const uint32_t np = next + pos_k(key_tile(x, 0));
+                const uint32_t np = next + pos_k(key_tile(nx, x, 0));
                 const bool q_here = (x == 1 && SPLIT) || mbar_test(q_full(x), qn[x] & 1);
                 if (q_here && mbar_test(kv_full(np % kSlots), (np / kSlots) & 1)) {
                   begin(nx, next, x);
@@ -516,11 +537,42 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
         }
         ++sn;
         tc_fence_after();
+        if (WIN && it.narrow && j == 0 && (!SPLIT || x == 0)) {   // the first keys alone, all of them behind the window
+          uint32_t v[kNarrow];
+          tmem_ld_32x32b_x32(s_t, v);
+          tmem_wait_ld();
+          mask_after<kNarrow>(v, p.sinks - 1);
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kNarrow; i += 2) mx = max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          m_run = mx * p.scale_log2;
+          const float shift = m_run == -INFINITY ? 0.f : -m_run;
+          const float2 neg = make_float2(shift, shift);
+          float2 sum = make_float2(0.f, 0.f);
+          uint32_t pk[kNarrow / 2];
+#pragma unroll
+          for (int i = 0; i < kNarrow / 2; ++i) {
+            const float2 t = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, neg);
+            const float2 q = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+            sum = add2(sum, q);
+            pk[i] = pack2<F16>(q.x, q.y);
+          }
+          tmem_st_32x32b_x16(s_t, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(p_half(x));
+            mbar_arrive(p_ready(x));
+          }
+          l_run = sum.x + sum.y;
+          continue;
+        }
         // 168 registers do not hold the row and everything else: its last part is read for the maximum and again when
         // its turn comes (P overwrites only the first half of the scores)
         constexpr int kKept = SPLIT ? 64 : 96;
         uint32_t v[kKept];
-        const int kt = listed_tile<WIN>(it, SPLIT ? 2 * j + x : j);
+        const int index = list_index<SPLIT, WIN>(it, x, j), kt = listed_tile<WIN>(it, index);
         const bool diag = p.causal && kt == qt;                        // keys after the query: 0 after the exponential
         // windows: a tile with the diagonal, behind it, or with the far border of some row's window; borders from its key 0
         const int first = WIN ? (qt - kt) * BQ + row - p.window : 0, sinks = WIN ? p.sinks - kt * BKV : 0;
@@ -783,7 +835,7 @@ bool split_window(int batch, int seq, int heads, int window, int sinks, int sms)
     for (long long b = 0; b < blocks; ++b) {
       const long long qa = split ? b : 2 * b, oldest = qa * BQ - window + 1, w0 = oldest > 0 ? oldest / BKV : 0;
       const long long ns = (sinks + BKV - 1) / BKV < w0 ? (sinks + BKV - 1) / BKV : w0;
-      const long long keys = ns + qa - w0 + (split || qa + 1 == nq ? 1 : 2);
+      const long long keys = ns - (ns == 1 && sinks <= kNarrow && !split ? 1 : 0) + qa - w0 + 1;   // (a narrow tile is hardly a step)
       const long long steps = (split ? (keys + 1) / 2 : keys) + 1;
       const long long same = w0 > (sinks + BKV - 1) / BKV && qa + 2 < nq ? (split ? nq - 1 : (nq - 1) / 2) - b : 1;   // equal blocks from here on
       const long long n = same > 1 ? same : 1;
