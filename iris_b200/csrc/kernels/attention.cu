@@ -78,6 +78,12 @@ static_assert(kSmemBytes <= 227 * 1024, "shared-memory budget");
 // nothing from it.
 constexpr int kPolyEvery = 4;
 
+// With windows a row's maximum is renewed only when it has grown by 2^kGrowth (weights of up to 256 are as exact in 16 bits as
+// those of up to 1, and the sums are in fp32): 394 -> 340 us for 2 x 8192 tokens, 32 heads, window 1024 (with masks by
+// border, the masks a third of that).  It costs that the largest weight
+// of a row is rounded like the others instead of being 1.
+constexpr float kGrowth = 8.f;
+
 // Up to so many first keys make a tile of their own width instead of a whole one (2 x 8192 tokens, 32 heads, window 1024, 4 first
 // keys: with whole tiles, and with side B going through the tile that it sees nothing of, 400 us).
 constexpr int kNarrow = 32;
@@ -157,6 +163,12 @@ __device__ __forceinline__ void mask_window(uint32_t* v, int last, int before, i
 #pragma unroll
   for (int i = 0; i < N; ++i)
     if (i > last || (i <= before && i >= sinks)) v[i] = 0xff800000u;
+}
+template <int N>
+__device__ __forceinline__ void mask_before(uint32_t* v, int before) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i <= before) v[i] = 0xff800000u;
 }
 // Scores of the keys after `row` become minus infinity.
 template <int N>
@@ -576,7 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
         const bool diag = p.causal && kt == qt;                        // keys after the query: 0 after the exponential
         // windows: a tile with the diagonal, behind it, or with the far border of some row's window; borders from its key 0
         const int first = WIN ? (qt - kt) * BQ + row - p.window : 0, sinks = WIN ? p.sinks - kt * BKV : 0;
-        const bool border = WIN && (kt >= qt || (qt - kt + 1) * BQ - 1 >= p.window);
+        const bool late = kt >= qt, early = (qt - kt + 1) * BQ - 1 >= p.window;
+        const int border = !WIN || !(late || early) ? 0 : !late && sinks <= 0 ? 1 : kt == qt && !early ? 2 : 3;
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};    // four chains instead of one long one
         {
           uint32_t t[128 - kKept];
@@ -586,7 +599,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
           for (int c = 0; c < kKept; c += 32) tmem_ld_32x32b_x32(s_t + c, v + c);
           tmem_wait_ld();
           if (WIN) {
-            if (border) {
+            if (border == 1) {
+              mask_before<128 - kKept>(t, first - kKept), mask_before<kKept>(v, first);
+            } else if (border == 2) {
+              mask_after<128 - kKept>(t, row - kKept), mask_after<kKept>(v, row);
+            } else if (border == 3) {
               mask_window<128 - kKept>(t, (qt - kt) * BQ + row - kKept, first - kKept, sinks - kKept);
               mask_window<kKept>(v, (qt - kt) * BQ + row, first, sinks);
             }
@@ -607,12 +624,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
         if (j == 0) {
           m_run = mx;
-        } else if (__any_sync(0xffffffffu, mx > m_run)) {
+        } else if (__any_sync(0xffffffffu, mx > m_run + (WIN ? kGrowth : 0.f))) {
           // Each row takes its new maximum at once, so that its largest weight is exactly 1 in the 16 bits of P, and what has
           // been summed is rescaled.  These scores are complete, so the products issued before them are too, and the next
           // one waits for P.  (32 columns at a time and two to an instruction: 317 us for 8 x 2048 x 32 causal from a rest;
           // 16 at a time 328, one to an instruction 322, between the exponentials 336, two loads in flight 328.)
-          const float m_new = fmaxf(m_run, mx);
+          // (each row by itself, so that none depends on what its neighbours in the warp see)
+          const float m_new = WIN && !(mx > m_run + kGrowth) ? m_run : fmaxf(m_run, mx);
           const float alpha = m_new == m_run ? 1.f : fast_exp2(m_run - m_new);
           const float2 alpha2 = make_float2(alpha, alpha);
           l_run *= alpha;
@@ -642,7 +660,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
             tmem_ld_32x32b_x32(s_t + c * 32, v + c * 32 % kKept);
             tmem_wait_ld();
             if (WIN) {
-              if (border) mask_window<32>(v + c * 32 % kKept, (qt - kt) * BQ + row - c * 32, first - c * 32, sinks - c * 32);
+              if (border == 1) mask_before<32>(v + c * 32 % kKept, first - c * 32);
+              else if (border == 2) mask_after<32>(v + c * 32 % kKept, row - c * 32);
+              else if (border == 3)
+                mask_window<32>(v + c * 32 % kKept, (qt - kt) * BQ + row - c * 32, first - c * 32, sinks - c * 32);
             } else if (diag) {
               mask_after<32>(v + c * 32 % kKept, row - c * 32);
             }

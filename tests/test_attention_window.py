@@ -35,7 +35,7 @@ def _check(qkv, out, batch, seq, heads, kv, window, sinks):
             ref = torch.softmax(s, 1) @ v
             v_max = torch.stack([v[seen[i]].abs().max() for i in range(seq)]) if seq <= 200 else v.abs().max().expand(seq)
             tol = half * ref.abs() + ((1.05 * half + 2.0 ** -13) * v_max)[:, None]
-            err = (out.view(batch, seq, heads, 128)[b, :, h].double() - ref).abs()
+            err = (out.unflatten(0, (batch, seq)).unflatten(2, (heads, 128))[b, :, h].double() - ref).abs()
             assert bool((err <= tol).all()), f"batch {b} head {h}: {(err / tol).max().item()} of the tolerance"
 
 
@@ -78,11 +78,19 @@ def test_many_heads(batch, seq, heads, kv, window, sinks, dtype):
 @gpu
 @pytest.mark.parametrize("batch,seq,heads", [(1, 512, 2), (2, 1024, 40)])
 def test_a_window_of_all_keys_is_causal_attention(batch, seq, heads):
+    """Both are within the bounds of the same formula.  (Not bit by bit: the weights of the two are scaled by different powers of
+    e before they are rounded, as far apart as 2^8, since the windowed form renews a row's maximum less often.)"""
     qkv, _, out = _inputs(batch, seq, heads, heads, torch.bfloat16)
     want = torch.empty_like(out)
     A.attention_fwd(qkv, want, batch, seq, heads)
     A.attention_window_fwd(qkv, out, batch, seq, heads, window=seq)
-    assert torch.equal(out, want)
+    w = heads * 128
+    for b in range(batch):
+        for h in {0, heads - 1}:
+            x = qkv[b * seq:(b + 1) * seq]
+            part = torch.cat([x[:, n * w + h * 128:n * w + (h + 1) * 128] for n in range(3)], 1)
+            for o in (out, want):
+                _check(part, o[b * seq:(b + 1) * seq, h * 128:(h + 1) * 128], 1, seq, 1, 1, seq, 0)
 
 
 @gpu
