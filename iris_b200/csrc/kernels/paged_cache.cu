@@ -159,29 +159,53 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__
       const int n = min(kThreads, p.batch - base);
       const int64_t row0 = p.row_stride ? base * p.row_stride : tokens;
       const int64_t row1 = min(p.tokens, p.row_stride ? (base + n) * p.row_stride : tokens + all_tokens);
-      for (int64_t row = row0 + at0; row < row1; row += step) {
+      // Many rows: four in a row to a thread, one search, and a page looked up once for the rows that lie in it (32 prompts,
+      // 65536 rows: 9.3 -> 7.8 us).  Few: one to a thread (512 requests of one token: 4.1 us, 5.5 with four).
+      const int width = row1 - row0 > 2 * step ? 4 : 1;
+      for (int64_t at = row0 + width * at0; at < row1; at += width * step) {
         int r;
         int64_t j;
-        bool valid = true;
         if (p.row_stride) {
-          r = (int)((row - row0) / p.row_stride);
-          j = row - row0 - r * p.row_stride;
-          valid = j < c.tokens_upto[r] - (r ? c.tokens_upto[r - 1] : 0);
+          r = (int)((at - row0) / p.row_stride);
+          j = at - row0 - r * p.row_stride;
         } else {
-          r = search(c.tokens_upto, row - row0);
-          j = row - row0 - (r ? c.tokens_upto[r - 1] : 0);
+          r = search(c.tokens_upto, at - row0);
+          j = at - row0 - (r ? c.tokens_upto[r - 1] : 0);
         }
-        int pos = -1, slot = -1;
-        if (valid && c.granted[r]) {
-          pos = (int)(c.len[r] + j);
-          const int i = pos >> p.page_shift, fresh = i - c.held[r];
-          const int page = fresh < 0 ? p.table[(base + r) * p.table_pitch + i]
-                                     : p.free[count - 1 - (pages + (r ? c.pages_upto[r - 1] : 0) + fresh)];
-          const int64_t s = ((int64_t)page << p.page_shift) + (pos & mask);
-          slot = page < 0 || s > 0x7fffffff ? -1 : (int)s;   // an entry that is no page: as a token that is not kept
+        int slot[4], position[4], known = -1, page = -1;
+        int64_t more_here = c.tokens_upto[r] - (r ? c.tokens_upto[r - 1] : 0);
+        const int n4 = (int)min((int64_t)width, row1 - at);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          slot[u] = position[u] = -1;
+          if (u >= n4) break;
+          while (p.row_stride ? j >= p.row_stride : j >= more_here) {   // on to the next request (that has a token)
+            ++r;
+            j = 0;
+            known = -1;
+            more_here = c.tokens_upto[r] - c.tokens_upto[r - 1];
+          }
+          if (c.granted[r] && j < more_here) {
+            const int pos = (int)(c.len[r] + j), i = pos >> p.page_shift, fresh = i - c.held[r];
+            if (i != known) {
+              known = i;
+              page = fresh < 0 ? p.table[(base + r) * p.table_pitch + i]
+                               : p.free[count - 1 - (pages + (r ? c.pages_upto[r - 1] : 0) + fresh)];
+            }
+            const int64_t s = ((int64_t)page << p.page_shift) + (pos & mask);
+            position[u] = pos;
+            slot[u] = page < 0 || s > 0x7fffffff ? -1 : (int)s;   // an entry that is no page: as a token that is not kept
+          }
+          ++j;
         }
-        p.slots[row] = slot;
-        p.positions[row] = pos;
+        if (n4 == 4 && !((reinterpret_cast<uintptr_t>(p.slots + at) | reinterpret_cast<uintptr_t>(p.positions + at)) & 15)) {
+          *reinterpret_cast<int4*>(p.slots + at) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+          *reinterpret_cast<int4*>(p.positions + at) = make_int4(position[0], position[1], position[2], position[3]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (u < n4) p.slots[at + u] = slot[u], p.positions[at + u] = position[u];
+        }
       }
     }
     pages += all_pages;

@@ -30,7 +30,6 @@ namespace rotary {
 using namespace iris::ptx;
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;                // heads of a lane
 constexpr uint32_t kSitePosition = 96, kSiteSlot = 97;
 
 struct Params {
@@ -44,8 +43,9 @@ struct Params {
   uint8_t* v_cache;
   const int* slots;
   StatusBlock* status;
-  int64_t ld_in, ld_out, ld_table, page_pitch, slot_pitch, head_pitch, cache_slots;
+  int64_t tokens, ld_in, ld_out, ld_table, page_pitch, slot_pitch, head_pitch, cache_slots;
   int positions_in_table, heads, kv_heads, dim, half, page_shift;
+  int token_shift;           // log2 of the tokens of a block
   int out_heads;             // heads written to out: all, those of q and k (in place), or those of q
   float eps;
 };
@@ -78,15 +78,19 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
   return o;
 }
 
-// LANES: lanes of a head, the power of two from dim / 16 on.  Block (x, y): token x, heads y * kThreads / LANES * kHeads on.
-template <int LANES, bool F16, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ Params p) {
-  constexpr int kGroups = kThreads / LANES;
+// LANES: lanes of a head, the power of two from dim / 16 on.  HEADS: heads of a lane.  A block has `spread` groups of lanes to a
+// token; block (x, y): tokens x * (groups / spread) on, heads y * spread * HEADS on.  (64 registers, four blocks to an SM, although
+// that spills a little: 16384 tokens of 96 heads of 128, 181 us with 78 registers, 173 with 64; two heads to a lane 195.)
+template <int LANES, bool F16, bool INTERLEAVED, int HEADS>
+__global__ void __launch_bounds__(kThreads, HEADS == 1 ? 6 : 4) qk_norm_rope_kernel(const __grid_constant__ Params p) {
+  constexpr int kGroups = kThreads / LANES, kHeads = HEADS;
   grid_dependency_wait();
   grid_dependency_launch();
-  const int64_t token = blockIdx.x;
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const int head0 = blockIdx.y * kGroups * kHeads + group;
+  const int spread = kGroups >> p.token_shift;
+  const int64_t token = ((int64_t)blockIdx.x << p.token_shift) + group / spread;
+  if (token >= p.tokens) return;
+  const int head0 = blockIdx.y * spread * kHeads + group % spread;
   const int all = p.heads + 2 * p.kv_heads;
   const bool live = lane * 16 < p.dim;                   // (a dimension that is no power of two)
   const bool turns = lane * 8 < p.half;
@@ -98,7 +102,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
   const uint8_t* src = p.qkv + token * p.ld_in;
 #pragma unroll
   for (int u = 0; u < kHeads; ++u) {
-    const int h = head0 + u * kGroups;
+    const int h = head0 + u * spread;
     if (live && h < all) {
       x[u][0] = *reinterpret_cast<const uint4*>(src + (h * p.dim + c0) * 2);
       x[u][1] = *reinterpret_cast<const uint4*>(src + (h * p.dim + c1) * 2);
@@ -108,10 +112,10 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
   const int slot = p.k_cache ? p.slots[token] : -1;
   if (pos < 0) return;                                    // a row of no token
   if (pos >= p.positions_in_table) {
-    if (threadIdx.x == 0) record_status(p.status, kBadPointer, kSitePosition, 0, (uint32_t)token, (uint64_t)pos);
+    if (head0 == 0 && lane == 0) record_status(p.status, kBadPointer, kSitePosition, 0, (uint32_t)token, (uint64_t)pos);
     return;
   }
-  if (slot >= p.cache_slots && threadIdx.x == 0) record_status(p.status, kBadPointer, kSiteSlot, 0, (uint32_t)token, (uint64_t)slot);
+  if (slot >= p.cache_slots && head0 == 0 && lane == 0) record_status(p.status, kBadPointer, kSiteSlot, 0, (uint32_t)token, (uint64_t)slot);
   const bool keep = slot >= 0 && slot < p.cache_slots;
   const int64_t cached = keep ? (slot >> p.page_shift) * p.page_pitch + (slot & ((1 << p.page_shift) - 1)) * p.slot_pitch : 0;
 
@@ -127,7 +131,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_con
   uint8_t* dst = p.out + token * p.ld_out;
 #pragma unroll
   for (int u = 0; u < kHeads; ++u) {
-    const int h = head0 + u * kGroups;
+    const int h = head0 + u * spread;
     if (h >= all) break;                                  // (the same for all lanes of a head)
     if (h < p.heads + p.kv_heads) {
       float a[8], b[8];
@@ -198,11 +202,25 @@ int refuse(const char* what) {
   return -1;
 }
 
+template <int LANES, int HEADS>
+cudaError_t launch_as(const cudaLaunchConfig_t& cfg, const Params& p, int f16, int interleaved) {
+  return f16 ? interleaved ? cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, true, true, HEADS>, p)
+                           : cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, true, false, HEADS>, p)
+             : interleaved ? cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, false, true, HEADS>, p)
+                           : cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, false, false, HEADS>, p);
+}
+
 template <int LANES>
-cudaError_t launch(const Params& p, int64_t tokens, int f16, int interleaved, void* stream) {
-  constexpr int kBlockHeads = kThreads / LANES * kHeads;
+cudaError_t launch(Params& p, int64_t tokens, int f16, int interleaved, void* stream) {
+  constexpr int kGroups = kThreads / LANES;
+  const int all = p.heads + 2 * p.kv_heads;
+  // few heads: several tokens to a block; many: up to three heads to a lane, in as few blocks a token as that takes
+  p.token_shift = 0;
+  while ((kGroups >> (p.token_shift + 1)) >= all) ++p.token_shift;
+  const int passes = (all + kGroups - 1) / kGroups, blocks = (passes + 2) / 3, heads = (passes + blocks - 1) / blocks;
+  p.tokens = tokens;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)tokens, (p.heads + 2 * p.kv_heads + kBlockHeads - 1) / kBlockHeads);
+  cfg.gridDim = dim3((unsigned)((tokens + (1 << p.token_shift) - 1) >> p.token_shift), (all + kGroups * heads - 1) / (kGroups * heads));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
@@ -210,10 +228,9 @@ cudaError_t launch(const Params& p, int64_t tokens, int f16, int interleaved, vo
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return f16 ? interleaved ? cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, true, true>, p)
-                           : cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, true, false>, p)
-             : interleaved ? cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, false, true>, p)
-                           : cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, false, false>, p);
+  return heads == 1   ? launch_as<LANES, 1>(cfg, p, f16, interleaved)
+         : heads == 2 ? launch_as<LANES, 2>(cfg, p, f16, interleaved)
+                      : launch_as<LANES, 3>(cfg, p, f16, interleaved);
 }
 
 }  // namespace rotary
