@@ -12,7 +12,8 @@
 //     the blocks' edges: a position in that count gives the key, the key its page.
 //   * One warp loads: it looks the pages of 32 blocks up at a time, a batch ahead, and has the TMA unit copy the blocks (a 4-D
 //     tensor map over component, head, slot and page, so any order of them in memory) into a ring of tiles.  (With the copies
-//     in the warps that compute, cp.async a lane, a step was 460 instructions and 1300 cycles.)
+//     in the warps that compute, cp.async a lane, a step was 460 instructions and 1300 cycles.  Keys and values copied as one,
+//     through a fifth dimension: no gain, 173.8 us for 174.0 with heads of 64, 95.1 for 94.5 with heads of 128.)
 //   * The other warps are workers of their own: each takes its blocks of every tile and keeps its own running maximum, sum and
 //     output in registers (one pass).  They meet when a sequence's tiles end.
 //   * Products go through mma.sync m16n8k16 with the keys (for the scores) and the components (for the output) as the 16 rows
@@ -55,6 +56,7 @@ using namespace iris::ptx;
 
 constexpr int kRows = 16;                        // query heads of a segment, at most
 constexpr int kBlock = 16;                       // keys of a product
+constexpr int kHalfBlock = kBlock * 128;         // bytes of a block's keys (or values) in a panel
 constexpr int kJoinThreads = 512;
 constexpr uint32_t kSitePage = 95, kSiteLoad = 98, kSiteTile = 99;
 
@@ -67,10 +69,10 @@ struct Shape {
   static constexpr int kTile = kTileBlocks * kBlock;           // keys of a tile
   static constexpr int kStages = D == 256 ? 2 : 3;             // ring of tiles
   static constexpr int kQBufs = kStages;                       // queries of the segments that the ring reaches
-  static constexpr int kPanels = D / 64;                       // a tile's keys (or values) lie in panels of 64 components,
-  static constexpr int kPanel = kTile * 128;                   // rows of 128 bytes
-  static constexpr int kStageBytes = 2 * kPanels * kPanel;     // keys, then values: 32 KB
-  static constexpr int kBlockBytes = kBlock * 128;             // a block of a panel
+  static constexpr int kPanels = D / 64;                       // a tile lies in panels of 64 components,
+  static constexpr int kBlockBytes = 2 * kHalfBlock;           // a block of a panel: rows of 128 bytes, keys and values
+  static constexpr int kPanel = kTileBlocks * kBlockBytes;
+  static constexpr int kStageBytes = kPanels * kPanel;         // 32 KB
   static constexpr int kQPitch = D * 2 + 16;                   // (rows 16 bytes apart in the banks)
   static constexpr int kQBytes = COLS * kQPitch;
   static constexpr int kStats = 2 * kWarps * kRows * 4;        // maxima and sums of the warps
@@ -84,7 +86,7 @@ struct Shape {
 };
 
 struct Params {
-  CUtensorMap k, v;          // [pages, slots, key heads, components], box: 64 components of one head, a block or a page of rows
+  CUtensorMap k, v;          // [pages, slots, key heads, components], box: 64 components of one head, a block or a page of fewer rows
   const uint8_t* q;          // strides in bytes
   const int* table;
   const int* lens;
@@ -325,20 +327,22 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
 
   if (warp == kWarps) {
     // ---- loads ----
-    // A batch: 32 blocks of one segment, a lane each: which of its keys count, its page and its first slot there.
+    // A batch: 32 blocks of one segment, a lane each: which of its keys count, its page (pages of 8: its two) and its first slot.
     constexpr int kBatch = 32 / kTB;          // tiles
     struct Batch {
       uint32_t mask;
-      int page, slot, key;
+      int page, page2, slot, key;
     };
-    const bool whole_blocks = p.page_shift >= 4;
+    const bool whole_blocks = p.page_shift >= 4, two_pages = p.page_shift == 3;
     auto look_up = [&](const Cursor& at, int left) {
       Batch b;
       b.key = 0;
       b.mask = left > 0 ? block_mask(at.s, at.tile * kTile + lane * kBlock, b.key) : 0;
-      b.page = 0;
+      b.page = b.page2 = 0;
       b.slot = b.key & ((1 << p.page_shift) - 1);
-      if (whole_blocks && b.mask) b.page = p.table[at.b * p.table_pitch + (b.key >> p.page_shift)];
+      const int* row = p.table + at.b * p.table_pitch + (b.key >> p.page_shift);
+      if (whole_blocks ? b.mask : two_pages ? b.mask & 0xff : 0) b.page = row[0];
+      if (two_pages && b.mask >> 8) b.page2 = row[1];
       return b;
     };
     // the cursor of the batch behind the one at c, of `left` tiles yet to come: what the latter leaves of them
@@ -371,25 +375,48 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
         if (mine) record_status(p.status, kBadPointer, kSitePage, l.b, now.key, (uint64_t)(int64_t)now.page);
         mask = 0;
       }
+      if (two_pages) {
+        uint32_t bad = (uint32_t)now.page >= (uint32_t)p.pages ? 0xffu : 0;
+        if ((uint32_t)now.page2 >= (uint32_t)p.pages) bad |= 0xff00u;
+        if (mine && bad & mask)
+          record_status(p.status, kBadPointer, kSitePage, l.b, now.key, (uint64_t)(int64_t)(bad & mask & 0xff ? now.page : now.page2));
+        mask &= ~bad;
+      }
       const int seg = segment_of(l), kv = p.row_tiles == 1 ? seg : seg / p.row_tiles, r0 = (seg - kv * p.row_tiles) * kRows;
       const int rows = fresh ? min(COLS, p.group - r0) : 0;
       const uint32_t tile = ring + stage * S::kStageBytes;
-      if (whole_blocks) {
+      if (whole_blocks || two_pages) {
         const uint32_t blocks = __ballot_sync(0xffffffffu, mine && mask) >> first_lane;
         if (mine) masks[stage * kTB + lane - first_lane] = mask;
         __syncwarp();
         const bool one = elect_one();
-        if (one) mbar_expect_tx(full(stage), __popc(blocks) * (2 * S::kPanels * S::kBlockBytes) + rows * D * 2);
+        if (one) mbar_expect_tx(full(stage), __popc(blocks) * (S::kPanels * S::kBlockBytes) + rows * D * 2);
+        if (whole_blocks) {
 #pragma unroll
-        for (int b = 0; b < kTB; ++b) {
-          const int page = __shfl_sync(0xffffffffu, now.page, first_lane + b), slot = __shfl_sync(0xffffffffu, now.slot, first_lane + b);
-          if (one && (blocks >> b & 1)) {
+          for (int b = 0; b < kTB; ++b) {
+            const int page = __shfl_sync(0xffffffffu, now.page, first_lane + b), slot = __shfl_sync(0xffffffffu, now.slot, first_lane + b);
+            if (one && (blocks >> b & 1)) {
+              const uint32_t at = tile + b * S::kBlockBytes;
 #pragma unroll
-            for (int h = 0; h < S::kPanels; ++h)
-              tma_load_4d(tile + h * S::kPanel + b * S::kBlockBytes, &p.k, h * 64, kv, slot, page, full(stage));
+              for (int h = 0; h < S::kPanels; ++h) tma_load_4d(at + h * S::kPanel, &p.k, h * 64, kv, slot, page, full(stage));
 #pragma unroll
-            for (int h = 0; h < S::kPanels; ++h)
-              tma_load_4d(tile + (S::kPanels + h) * S::kPanel + b * S::kBlockBytes, &p.v, h * 64, kv, slot, page, full(stage));
+              for (int h = 0; h < S::kPanels; ++h)
+                tma_load_4d(at + h * S::kPanel + kHalfBlock, &p.v, h * 64, kv, slot, page, full(stage));
+            }
+          }
+        } else {
+          // pages of 8 (half of a block of which no key is seen is copied all the same, from page 0)
+#pragma unroll 1
+          for (int i = 0; i < 2 * kTB; ++i) {
+            const int page = __shfl_sync(0xffffffffu, i & 1 ? now.page2 : now.page, first_lane + i / 2);
+            if (one && (blocks >> i / 2 & 1)) {
+              const uint32_t at = tile + i / 2 * S::kBlockBytes + (i & 1) * 1024;
+#pragma unroll
+              for (int h = 0; h < S::kPanels; ++h) {
+                tma_load_4d(at + h * S::kPanel, &p.k, h * 64, kv, 0, page, full(stage));
+                tma_load_4d(at + h * S::kPanel + kHalfBlock, &p.v, h * 64, kv, 0, page, full(stage));
+              }
+            }
           }
         }
         if (one && rows > 0) {
@@ -398,7 +425,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
           for (int r = 0; r < rows; ++r) bulk_load(dst + r * S::kQPitch, src + r * p.q_head, D * 2, full(stage));
         }
       } else {
-        // pages of fewer than 16 keys: looked up a key a lane, copied a page at a time
+        // pages of fewer than 8 keys: looked up a key a lane, copied a page at a time
         const int size = 1 << p.page_shift;
         uint32_t bytes = 0;
         for (int pass = 0; pass < 2; ++pass) {   // count, then copy
@@ -421,7 +448,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
                 const uint32_t at = tile + b * S::kBlockBytes + j * 128;
                 for (int h = 0; h < S::kPanels; ++h) {
                   tma_load_4d(at + h * S::kPanel, &p.k, h * 64, kv, 0, from, full(stage));
-                  tma_load_4d(at + (S::kPanels + h) * S::kPanel, &p.v, h * 64, kv, 0, from, full(stage));
+                  tma_load_4d(at + h * S::kPanel + kHalfBlock, &p.v, h * 64, kv, 0, from, full(stage));
                 }
               }
             }
@@ -477,9 +504,9 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
   uint32_t parity = 0;
   bool fresh = true, whole = c.tile == 0, ok = true;   // whole: the segment began in this CTA
   int64_t seg_first = first - c.tile;           // stream: its first tile among all
-  // where a warp leaves its results: its own rows of the tile it has just used up, 512 floats in each block of a panel
+  // where a warp leaves its results: its own rows of the tile it has just used up, 1024 floats in each block of a panel
   auto result_of = [&](int w, int row, int col) {
-    constexpr int kPer = 512 / D;               // rows of a block
+    constexpr int kPer = 1024 / D;              // rows of a block
     const int piece = row / kPer, block = w * kB + piece % kB, panel = piece / kB;
     return reinterpret_cast<float*>(smem + stage * S::kStageBytes + panel * S::kPanel + block * S::kBlockBytes) + (row % kPer) * D + col;
   };
@@ -553,7 +580,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
         }
     }
     fresh = false;
-    const uint32_t ks = ring + stage * S::kStageBytes + warp * kB * S::kBlockBytes, vs = ks + S::kPanels * S::kPanel;
+    const uint32_t ks = ring + stage * S::kStageBytes + warp * kB * S::kBlockBytes, vs = ks + kHalfBlock;
     uint32_t word = 0;
     if (ok) {
 #pragma unroll
@@ -585,7 +612,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           uint32_t a[4];
-          ldsm4(a, ks + (kk >> 2) * S::kPanel + (j * kBlock + (mat & 1) * 8 + mrow) * 128 + ((((kk & 3) * 2 + (mat >> 1)) ^ mrow) << 4));
+          ldsm4(a, ks + (kk >> 2) * S::kPanel + j * S::kBlockBytes + ((mat & 1) * 8 + mrow) * 128 + ((((kk & 3) * 2 + (mat >> 1)) ^ mrow) << 4));
 #pragma unroll
           for (int n = 0; n < kN; ++n) mma<F16>(sc[kk % kChains][n], a, q[kk][n][0], q[kk][n][1]);
         }
@@ -655,7 +682,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
           uint32_t a[4];
-          ldsm4_t(a, vs + (d >> 2) * S::kPanel + (j * kBlock + (mat >> 1) * 8 + mrow) * 128 + ((((d & 3) * 2 + (mat & 1)) ^ mrow) << 4));
+          ldsm4_t(a, vs + (d >> 2) * S::kPanel + j * S::kBlockBytes + ((mat >> 1) * 8 + mrow) * 128 + ((((d & 3) * 2 + (mat & 1)) ^ mrow) << 4));
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
             mma<F16>(o[d][n], a, hi[j][n][0], hi[j][n][1]);
@@ -1090,6 +1117,39 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
   if (sms < 1) return refuse("no device");
   Params p;
   memset(&p, 0, sizeof(p));
+  p.batch = (int)batch;
+  p.group = (int)(heads / kv_heads);
+  p.row_tiles = (p.group + kRows - 1) / kRows;
+  p.segments_per_seq = (int)kv_heads * p.row_tiles;
+  p.rows = p.group < kRows ? p.group : kRows;
+  // lanes: as many of a sequence's segments side by side as leave no more than one CTA in 32 without work
+  const int resident = sms * 2;
+  p.lanes = 1;
+  for (int n = 2; n <= p.segments_per_seq && n <= resident; ++n)
+    if (p.segments_per_seq % n == 0 && resident / n * n * 32 >= resident * 31) p.lanes = n;
+  p.turns = p.segments_per_seq / p.lanes;
+  p.groups = resident / p.lanes;
+  const int64_t segments = batch * p.segments_per_seq;
+  if (cluster < 0) {
+    int64_t most = wide * (int64_t)page_size;
+    if (longest > 0 && longest < most) most = longest;
+    if (window > 0 && window < most && window + sinks < most) most = window + sinks;
+    const int64_t tile = dim == 64 ? Shape<64>::kTile : dim == 128 ? Shape<128>::kTile : Shape<256>::kTile;
+    const int64_t tiles = (most + tile - 1) / tile;
+    cluster = choose_cluster(segments, tiles, resident);
+  }
+  if (batch > 65535 || p.segments_per_seq > 65535) cluster = 0;
+  if (cluster == 0) {
+    const int64_t ctas = (int64_t)p.groups * p.lanes, need = ctas * (16 + 2 * p.rows * (dim + 2) * 4);
+    if (!work || work_bytes < need) return (int)need;
+    p.jobs = static_cast<int4*>(work);
+    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ctas * 16);
+  } else {
+    p.lanes = p.turns = 1;   // (a CTA's lane is its block's y)
+  }
+  if (cluster != 0 && cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) {
+    return refuse("a cluster has 1, 2, 4 or 8 CTAs");
+  }
   p.q = static_cast<const uint8_t*>(q);
   p.table = static_cast<const int*>(table);
   p.lens = static_cast<const int*>(lens);
@@ -1121,45 +1181,12 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
   p.table_pitch = table_pitch;
   p.out_batch = out_batch * 2, p.out_head = out_head * 2;
   p.lse_batch = lse_batch;
-  p.batch = (int)batch;
-  p.group = (int)(heads / kv_heads);
-  p.row_tiles = (p.group + kRows - 1) / kRows;
-  p.segments_per_seq = (int)kv_heads * p.row_tiles;
   p.pages = (int)pages;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   p.wide = (int)wide;
   p.window = window < 0x7fffffff ? (int)window : 0x7fffffff;
   p.sinks = sinks < 0x7fffffff ? (int)sinks : 0x7fffffff;
   p.scale_log2 = scale_log2;
-  p.rows = p.group < kRows ? p.group : kRows;
-  // lanes: as many of a sequence's segments side by side as leave no more than one CTA in 32 without work
-  const int resident = sms * 2;
-  p.lanes = 1;
-  for (int n = 2; n <= p.segments_per_seq && n <= resident; ++n)
-    if (p.segments_per_seq % n == 0 && resident / n * n * 32 >= resident * 31) p.lanes = n;
-  p.turns = p.segments_per_seq / p.lanes;
-  p.groups = resident / p.lanes;
-  const int64_t segments = batch * p.segments_per_seq;
-  if (cluster < 0) {
-    int64_t most = wide * (int64_t)page_size;
-    if (longest > 0 && longest < most) most = longest;
-    if (window > 0 && window < most && window + sinks < most) most = window + sinks;
-    const int64_t tile = dim == 64 ? Shape<64>::kTile : dim == 128 ? Shape<128>::kTile : Shape<256>::kTile;
-    const int64_t tiles = (most + tile - 1) / tile;
-    cluster = choose_cluster(segments, tiles, resident);
-  }
-  if (batch > 65535 || p.segments_per_seq > 65535) cluster = 0;
-  if (cluster == 0) {
-    const int64_t ctas = (int64_t)p.groups * p.lanes, need = ctas * (16 + 2 * p.rows * (dim + 2) * 4);
-    if (!work || work_bytes < need) return (int)need;
-    p.jobs = static_cast<int4*>(work);
-    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ctas * 16);
-  } else {
-    p.lanes = p.turns = 1;   // (a CTA's lane is its block's y)
-  }
-  if (cluster != 0 && cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) {
-    return refuse("a cluster has 1, 2, 4 or 8 CTAs");
-  }
   const auto st = static_cast<cudaStream_t>(stream);
   if (dim == 64) return dtype ? launch_paged<64, true>(p, (int)cluster, (int)device, st) : launch_paged<64, false>(p, (int)cluster, (int)device, st);
   if (dim == 128) return dtype ? launch_paged<128, true>(p, (int)cluster, (int)device, st) : launch_paged<128, false>(p, (int)cluster, (int)device, st);

@@ -82,7 +82,7 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
 // token; block (x, y): tokens x * (groups / spread) on, heads y * spread * HEADS on.  (64 registers, four blocks to an SM, although
 // that spills a little: 16384 tokens of 96 heads of 128, 181 us with 78 registers, 173 with 64; two heads to a lane 195.)
 template <int LANES, bool F16, bool INTERLEAVED, int HEADS>
-__global__ void __launch_bounds__(kThreads, HEADS == 1 ? 6 : 4) qk_norm_rope_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, HEADS == 1 ? 5 : 4) qk_norm_rope_kernel(const __grid_constant__ Params p) {
   constexpr int kGroups = kThreads / LANES, kHeads = HEADS;
   grid_dependency_wait();
   grid_dependency_launch();

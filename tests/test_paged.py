@@ -194,6 +194,19 @@ def test_attention_lengths_outside_the_table_are_cut():
 
 
 @gpu
+@pytest.mark.parametrize("page", [4, 8, 16, 64])
+@pytest.mark.parametrize("which", ["values first", "one tensor"])
+def test_attention_places_of_the_caches(which, page):
+    """The values' cache in front of the keys' in memory, and one tensor for both."""
+    case = Case([100, 33], 4, 2, 128, page, torch.bfloat16)
+    if which == "values first":
+        case.k, case.v = case.v, case.k
+    else:
+        case.v = case.k
+    case.run().check()
+
+
+@gpu
 def test_attention_offsets_beyond_32_bits():
     """A cache of more than 4 GiB whose last pages are used (strides that pass 2^31 elements)."""
     pages, page, kv, dim = 70000, 64, 4, 128                         # 2.3e9 elements each: keys and values alias, 4.6 GB
