@@ -76,12 +76,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     strides = page, slot, head, one = k_cache.stride()
     if one != 1 or q_one != 1 or out_one != 1 or (v_cache.stride() != strides and not same_strides(k_cache, v_cache)):
         raise ValueError("k_cache and v_cache must have the same strides, and all heads be contiguous")
-    table_shape = block_table.shape
-    if block_table.dtype is not torch.int32 or len(table_shape) != 2 or table_shape[0] != batch:
-        raise ValueError(f"block_table must be int32 [{batch}, pages of a sequence]")
-    table_pitch, table_one = block_table.stride()
-    if lens.dtype is not torch.int32 or lens.shape != (batch,) or not lens.is_contiguous() or (table_one != 1 and table_shape[1] > 1):
-        raise ValueError(f"lens must be int32 [{batch}], and it and the rows of block_table contiguous")
+    (rows, wide), (table_pitch, table_one) = block_table.shape, block_table.stride()
+    if (block_table.dtype is not torch.int32 or rows != batch or (table_one != 1 and wide > 1) or lens.dtype is not torch.int32 or
+            lens.nbytes != 4 * batch or not lens.is_contiguous()):
+        raise ValueError(f"block_table must be int32 [{batch}, pages of a sequence] with contiguous rows, lens contiguous int32 [{batch}]")
     if (batch > 1 and out_batch < dim) or (heads > 1 and out_head < dim):
         raise ValueError("rows of out must not overlap")
     device = q.get_device()
@@ -89,11 +87,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             block_table.get_device() == device and lens.get_device() == device)
     lse_ptr = lse_batch = status_ptr = 0
     if lse is not None:
-        if lse.dtype is not torch.float32 or lse.shape != (batch, heads):
-            raise ValueError(f"lse must be fp32 [{batch}, {heads}]")
-        lse_batch, lse_one = lse.stride()
-        if (lse_one != 1 and heads > 1) or (batch > 1 and lse_batch < heads):
-            raise ValueError("rows of lse must be contiguous and not overlap")
+        (lse_batch, lse_one) = lse.stride()
+        if (lse.dtype is not torch.float32 or lse.shape != (batch, heads) or (lse_one != 1 and heads > 1) or
+                (batch > 1 and lse_batch < heads)):
+            raise ValueError(f"lse must be fp32 [{batch}, {heads}], with rows that are contiguous and do not overlap")
         same = same and lse.get_device() == device
         lse_ptr = lse.data_ptr()
     if status is not None:
@@ -116,7 +113,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         rc = fn(_ATTENTION.pack(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lens.data_ptr(), out.data_ptr(), lse_ptr,
             work_ptr, status_ptr, current if stream is None else stream, q_batch, q_head, page, slot, head, table_pitch, out_batch,
-            out_head, lse_batch, batch, heads, dim, pages, size, kv_heads, table_shape[1], _DT[dtype], window, sinks, longest or 0,
+            out_head, lse_batch, batch, heads, dim, pages, size, kv_heads, wide, _DT[dtype], window, sinks, longest or 0,
             -1, work_bytes, device, int(timeout_ms * 1e6), dim ** -0.5 if scale is None else scale))
         if rc <= 0 or work_bytes:
             break
@@ -148,27 +145,29 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     A request for which the free pages do not last (nor for any later one that lacks a page), whose tokens do not fit its row of
     the table, or have not enough rows, gets nothing: its length stays, its rows get -1.  All tensors int32.
     """
-    i32, shape, rows = torch.int32, lens.shape, slots.shape
+    # (every look at a tensor costs the host 0.06 to 0.12 us, on a path of 7: sizes in bytes and straight chains, not shapes and loops)
+    i32 = torch.int32
     lens_out = lens if lens_out is None else lens_out
     free_count_out = free_count if free_count_out is None else free_count_out
-    for t in (lens, new_lens, free_pages, free_count, slots, positions, lens_out, free_count_out):
-        if t.dtype is not i32 or not t.is_contiguous():
-            raise ValueError("all tensors must be int32 and contiguous (block_table: its rows)")
-    if len(shape) != 1 or new_lens.shape != shape or lens_out.shape != shape:
-        raise ValueError(f"lens, new_lens and lens_out must be 1-D and of one length, got {list(shape)}, {list(new_lens.shape)} and "
-                         f"{list(lens_out.shape)}")
-    if len(rows) != 1 or positions.shape != rows or free_pages.dim() != 1 or free_count.shape != (1,) or free_count_out.shape != (1,):
-        raise ValueError("slots, positions and free_pages must be 1-D, the first two of one length, and the counts of one element")
-    batch, tokens = shape[0], rows[0]
+    if not (lens.dtype is i32 and new_lens.dtype is i32 and free_pages.dtype is i32 and free_count.dtype is i32 and
+            slots.dtype is i32 and positions.dtype is i32 and lens_out.dtype is i32 and free_count_out.dtype is i32 and
+            lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous() and slots.is_contiguous() and
+            positions.is_contiguous() and lens_out.is_contiguous()):
+        raise ValueError("all tensors must be int32 and contiguous (block_table: its rows)")
+    size, rows = lens.nbytes, slots.nbytes
+    if new_lens.nbytes != size or lens_out.nbytes != size or positions.nbytes != rows or free_count.nbytes != 4 or free_count_out.nbytes != 4:
+        raise ValueError("lens, new_lens and lens_out must be of one length, as slots and positions, and the counts of one element")
+    batch, tokens = size // 4, rows // 4
     table_shape, (pitch, one) = _rows(block_table, batch)
     if page_size < 1 or page_size & (page_size - 1):
         raise ValueError("page_size must be a power of two")
     if row_stride < 0 or tokens < batch * row_stride:
         raise ValueError(f"{tokens} rows do not hold {batch} requests of {row_stride}")
     device = lens.get_device()
-    for t in (new_lens, block_table, free_pages, free_count, slots, positions, lens_out, free_count_out):
-        if t.get_device() != device:
-            raise ValueError("all tensors must be on one device")
+    if not (new_lens.get_device() == device and block_table.get_device() == device and free_pages.get_device() == device and
+            free_count.get_device() == device and slots.get_device() == device and positions.get_device() == device and
+            lens_out.get_device() == device and free_count_out.get_device() == device):
+        raise ValueError("all tensors must be on one device")
     if batch == 0 or table_shape[1] == 0:
         raise ValueError("no requests, or no room in the block table")
     if device != _native.current_device(device):
@@ -178,7 +177,7 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     rc = _native.entry("iris_k_reserve_slots")(_RESERVE.pack(
         lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
         slots.data_ptr(), positions.data_ptr(), lens_out.data_ptr(), free_count_out.data_ptr(),
-        torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, pitch, table_shape[1], free_pages.shape[0],
+        torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, pitch, table_shape[1], free_pages.nbytes // 4,
         page_size, batch, tokens, row_stride))
     if rc:
         _raise("reserve_slots", rc)
