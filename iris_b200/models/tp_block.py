@@ -147,6 +147,8 @@ class TPDecoder:
             raise ValueError("key heads must divide the query heads, and by the number of ranks")
         if cfg.hidden != cfg.n_heads * cfg.head_dim and not cfg.plain:
             raise ValueError("the hidden size must be that of all heads")
+        if cfg.rope_theta and cfg.positions and cfg.positions < cfg.seq:
+            raise ValueError("fewer positions than rows of a sequence")
         if weights is not None and (weights.ranks != self.ranks or len(weights.layers) != cfg.n_layers or any(
                 getattr(weights.cfg, f) != getattr(cfg, f)
                 for f in ("hidden", "n_heads", "head_dim", "intermediate", "kv_heads", "qk_norm"))):

@@ -14,6 +14,7 @@ from typing import Optional
 import torch
 
 from .. import _native
+from .paged import may_overlap
 
 HEAD_DIM = 128
 _DT = {torch.bfloat16: 0, torch.float16: 1}
@@ -59,7 +60,7 @@ def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: 
 
     ``qkv`` is ``[batch * seq, (heads + 2 * kv_heads) * 128]`` with the Q, K and V column blocks side by side, query head ``h``
     reading key head ``h // (heads // kv_heads)``; ``out`` is ``[batch * seq, heads * 128]``; rows may be strided views.
-    ``seq``: any length.  ``status``: as for :func:`attention_fwd`.  A masked key weighs exactly nothing; a masked *value* that
+    ``seq``: any length.  ``out`` may be the query columns of ``qkv`` themselves.  ``status``: as for :func:`attention_fwd`.  A masked key weighs exactly nothing; a masked *value* that
     is infinite or NaN still reaches the queries of its sequence whose window shares its tile of 128 keys (zero times it), so
     the rows of padding have to be finite.
     """
@@ -81,14 +82,18 @@ def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: 
     device = qkv.get_device()
     if out.get_device() != device or (status is not None and status.get_device() != device):
         raise ValueError("all tensors must be on one device")
-    if batch * seq == 0:
+    rows = batch * seq
+    if rows == 0:
         return out
+    kv_ptr, out_ptr = qkv.data_ptr() + heads * HEAD_DIM * 2, out.data_ptr()
+    if rows > 1 and ld_out < heads * HEAD_DIM or may_overlap(rows, kv_ptr, ld_in, 2 * kv_heads * HEAD_DIM, out_ptr, ld_out, heads * HEAD_DIM):
+        raise ValueError("rows of out must not overlap, nor lie over keys or values")
     if device != _native.current_device(device):
         with torch.cuda.device(device):
             return attention_window_fwd(qkv, out, batch, seq, heads, kv_heads, window=window, sinks=sinks, status=status,
                                         timeout_ms=timeout_ms, stream=stream)
     rc = _native.entry("iris_k_attention_window_fwd")(_WINDOW_ARGS.pack(
-        qkv.data_ptr(), out.data_ptr(), 0 if status is None else status.data_ptr(),
+        kv_ptr - heads * HEAD_DIM * 2, out_ptr, 0 if status is None else status.data_ptr(),
         torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, ld_in, ld_out, batch, seq, heads, kv_heads,
         window, sinks, _DT[dtype], int(timeout_ms * 1e6)))
     if rc != 0:

@@ -43,6 +43,17 @@ def same_strides(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.stride() == b.stride() or all(x == y or n < 2 for x, y, n in zip(a.stride(), b.stride(), a.shape))
 
 
+def may_overlap(rows: int, a: int, a_pitch: int, a_width: int, b: int, b_pitch: int, b_width: int) -> bool:
+    """Whether two matrices of 16-bit elements (address, pitch and width in elements) share memory; column blocks of one matrix,
+    with its pitch, do not."""
+    if a + ((rows - 1) * a_pitch + a_width) * 2 <= b or b + ((rows - 1) * b_pitch + b_width) * 2 <= a:
+        return False
+    if a_pitch == b_pitch and rows > 1:
+        off = (b - a) % (a_pitch * 2) if a_pitch else 0
+        return off < a_width * 2 or off + b_width * 2 > a_pitch * 2
+    return True
+
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                     lens: torch.Tensor, out: torch.Tensor, *, window: int = 0, sinks: int = 0, scale: Optional[float] = None,
                     lse: Optional[torch.Tensor] = None, longest: Optional[int] = None, status: Optional[torch.Tensor] = None,
@@ -57,7 +68,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``window`` the token sees the last ``window`` keys (its own among them) and the first ``sinks``.  ``scale`` defaults to
     ``head_dim ** -0.5``.  ``lse`` fp32 ``[batch, heads]``: receives the logarithm of the softmax's sum.
 
-    A sequence of no keys gets zeros (and minus infinity in ``lse``).  Memory behind a sequence's last key is not looked at.  A
+    A sequence of no keys gets zeros (and minus infinity in ``lse``); a length beyond the table's width is cut to it, a negative
+    one counts as 0.  Keys and values behind a sequence's last key, or out of its window, reach nothing, NaN or not.  A
     key whose table entry is no page is left out and recorded in ``status`` (an ``Iris`` context's status block) if that is
     given, as is a bounded wait of the kernel that ran out.  ``longest``: what the lengths are expected not to exceed, where that is much less than the table's width; it is
     for speed alone.
@@ -108,7 +120,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                    longest=longest, status=status, timeout_ms=timeout_ms, stream=stream)
     fn = _native.entry("iris_k_paged_attention")
     current = torch._C._cuda_getCurrentRawStream(device)
-    work, work_ptr, work_bytes = None, 0, 0
+    work_ptr = work_bytes = 0
     while True:
         rc = fn(_ATTENTION.pack(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lens.data_ptr(), out.data_ptr(), lse_ptr,
@@ -117,15 +129,17 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             -1, work_bytes, device, int(timeout_ms * 1e6), dim ** -0.5 if scale is None else scale))
         if rc <= 0 or work_bytes:
             break
-        # sums of sequences that several CTAs share, of this call alone
-        work, work_bytes = torch.empty(rc, dtype=torch.uint8, device=q.device), rc
-        work_ptr = work.data_ptr()
+        # sums of sequences that several CTAs share: memory of this call alone, and of the stream that it runs on
+        if stream is None or stream == current:
+            work = torch.empty(rc, dtype=torch.uint8, device=q.device)
+        else:
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=q.device)):
+                work = torch.empty(rc, dtype=torch.uint8, device=q.device)
+        work_ptr, work_bytes = work.data_ptr(), rc
     if rc:
         lib = _native.kernels()
         lib.iris_paged_attention_last_error.restype = ctypes.c_char_p
         raise RuntimeError(lib.iris_paged_attention_last_error().decode() or f"paged attention failed ({rc})")
-    if work is not None and stream is not None and stream != current:
-        work.record_stream(torch.cuda.ExternalStream(stream, device=device))
     return out
 
 

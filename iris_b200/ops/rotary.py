@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from .paged import same_strides
+from .paged import may_overlap, same_strides
 
 _DT = {torch.bfloat16: 0, torch.float16: 1}
 _ARGS = struct.Struct("@28qd")
@@ -56,17 +56,6 @@ def _weight(w: torch.Tensor, head_dim: int, dtype: torch.dtype) -> int:
     if w.dtype is not dtype or w.nbytes != 2 * head_dim or not w.is_contiguous():
         raise ValueError(f"norm weights must be contiguous [{head_dim}] of the type of qkv")
     return w.data_ptr()
-
-
-def _may_overlap(rows: int, a: int, a_pitch: int, a_width: int, b: int, b_pitch: int, b_width: int) -> bool:
-    """Whether two matrices of 16-bit elements (address, pitch and width in elements) share memory; column blocks of one matrix,
-    with its pitch, do not."""
-    if a + ((rows - 1) * a_pitch + a_width) * 2 <= b or b + ((rows - 1) * b_pitch + b_width) * 2 <= a:
-        return False
-    if a_pitch == b_pitch and rows > 1:
-        off = (b - a) % (a_pitch * 2) if a_pitch else 0
-        return off < a_width * 2 or off + b_width * 2 > a_pitch * 2
-    return True
 
 
 def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, table: Optional[torch.Tensor], heads: int, kv_heads: int,
@@ -148,7 +137,7 @@ def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, 
     in_place = out_ptr == qkv_ptr and ld_out == ld_in
     if tokens > 1 and ld_out < out_width:
         raise ValueError("rows of out must not overlap")
-    if not in_place and _may_overlap(tokens, qkv_ptr, ld_in, width, out_ptr, ld_out, out_width):
+    if not in_place and may_overlap(tokens, qkv_ptr, ld_in, width, out_ptr, ld_out, out_width):
         raise ValueError("out must be qkv itself, or share no memory with it")
     if device != _native.current_device(device):
         with torch.cuda.device(device):

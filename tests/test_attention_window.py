@@ -150,6 +150,16 @@ def test_in_a_graph_and_on_another_stream():
 
 
 @gpu
+@pytest.mark.parametrize("batch,seq,heads,kv", [(2, 300, 4, 2), (3, 640, 40, 8)])
+def test_output_over_the_queries(batch, seq, heads, kv):
+    qkv, _, out = _inputs(batch, seq, heads, kv, torch.bfloat16)
+    A.attention_window_fwd(qkv, out, batch, seq, heads, kv, window=100, sinks=2)
+    over = qkv[:, :heads * 128]
+    A.attention_window_fwd(qkv, over, batch, seq, heads, kv, window=100, sinks=2)
+    assert torch.equal(over, out)
+
+
+@gpu
 def test_no_rows():
     qkv, _, out = _inputs(1, 4, 2, 1, torch.bfloat16)
     assert A.attention_window_fwd(qkv[:0], out[:0], 0, 4, 2, 1, window=4).shape == (0, 256)
@@ -164,8 +174,13 @@ def test_refusals():
                 dict(sinks=-1), dict(qkv=qkv.t().contiguous().t()), dict(out=out[:, :128]), dict(qkv=qkv[None])):
         with pytest.raises(ValueError):
             A.attention_window_fwd(**{**ok, **bad})
-    with pytest.raises(ValueError, match="CUDA device"):
-        A.attention_window_fwd(**ok)
+    wide = torch.zeros((20, 2000), dtype=torch.bfloat16)
+    for bad in (wide[:, 512:1024], wide[:, 800:1312], wide[:1, :512].expand(20, -1)):      # over the keys; over the values; one row
+        with pytest.raises(ValueError, match="overlap"):
+            A.attention_window_fwd(**{**ok, "qkv": wide[:, :1024], "out": bad})
+    for fine in (out, wide[:, :512], wide[:, 1024:1536]):                                # of its own; the queries; beside them
+        with pytest.raises(ValueError, match="CUDA device"):
+            A.attention_window_fwd(**{**ok, "qkv": wide[:, :1024], "out": fine})
 
 
 @gpu

@@ -255,6 +255,36 @@ def test_attention_on_another_stream_and_in_two_graphs():
 
 
 @gpu
+def test_attention_over_its_queries():
+    """The output may take the queries' place, in both forms."""
+    for wide in (None, 4000):
+        case = Case([3000, 10, 0, 800], 8, 2, 128, 16, torch.bfloat16, wide=wide)
+        case.run()
+        P.paged_attention(case.q, case.k, case.v, case.table, case.len_t, case.q)
+        assert torch.equal(case.q, case.out)
+
+
+@gpu
+def test_attention_workspace_on_another_stream_is_its_own():
+    """Memory that the current stream still works on is not what a call on another stream gets for its workspace: calls on a side
+    stream, between long-running kernels of the current one whose memory has been let go of, give the right answer."""
+    case = Case([3000, 10, 800], 8, 2, 128, 16, torch.bfloat16, wide=4000)
+    case.run().check()
+    want, side = case.out.clone(), torch.cuda.Stream()
+    for _ in range(10):
+        for n in (1, 2, 4):
+            t = torch.full((n << 20,), 7.0, device="cuda")
+            for _ in range(20):
+                t.mul_(1.0001)
+            del t
+        P.paged_attention(case.q, case.k, case.v, case.table, case.len_t, case.out, stream=side.cuda_stream)
+        side.synchronize()
+        assert torch.equal(case.out, want)
+        case.out.zero_()
+        torch.cuda.synchronize()
+
+
+@gpu
 def test_attention_empty_batch():
     c = Case([5], 2, 1, 64, 16, torch.bfloat16)
     out = c.out[:0]
