@@ -6,16 +6,72 @@ Column-parallel projections run as fused all-gather->GEMM, row-parallel ones as 
 reference, whose fused kernels are the ingredients.
 
     python -m iris_b200.launch -np 8 examples/10_tp_block/tp_block.py -v -b
+    python examples/10_tp_block/tp_block.py --decode 64 --kv_heads 8 --rope_theta 10000 --qk_norm --window 1024 --sinks 4
+
+``--decode N``: the same sequences as prompts followed by N single tokens each over a paged cache (one step captured into a CUDA
+graph), instead of the comparison with the library stack.
 """
 import argparse
 import json
 import os
 import sys
+from dataclasses import replace
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."))
 from common.harness import device_barrier, iris, reduce_ranks, time_kernel_ms, torch  # noqa: E402
 
 from iris_b200.models.tp_block import TPConfig, TPDecoder, TPDecoderBaseline, reference_forward  # noqa: E402
+
+
+def decode(ctx, cfg, prefill, args):
+    """Prompts through `prefill`, then `args.decode` tokens of every sequence one by one.  The rows are random ones, as in the
+    other runs (there is no vocabulary here); with -v they are compared with the oracle's rows of the whole sequences."""
+    rank, world, dev = ctx.get_rank(), ctx.get_num_ranks(), ctx.get_device()
+    total = cfg.seq + args.decode
+    one = TPDecoder(ctx, replace(cfg, seq=1, positions=total), variant=args.variant, weights=prefill)
+    cache = prefill.make_cache(cfg.batch * -(-total // args.page_size), args.page_size, cfg.batch, total)
+    g = torch.Generator(device=dev).manual_seed(cfg.seed)
+    x = torch.randn((cfg.batch, total, cfg.hidden), generator=g, device=dev).to(torch.bfloat16)
+
+    def shard(rows):
+        n = rows.shape[0] // world
+        return rows[rank * n:(rank + 1) * n]
+    prompts = shard(x[:, :cfg.seq].reshape(-1, cfg.hidden)).clone()
+    new = torch.full((cfg.batch,), cfg.seq, dtype=torch.int32, device=dev)
+    prefill.forward([prompts], cache=cache, new_lens=new)
+    prefill.check()
+    new.fill_(1)
+    row = shard(x[:, 0]).clone()
+    graph = one.capture([row], cache=cache, new_lens=new)
+    outs, times = [], []
+    for i in range(args.decode):
+        row.copy_(shard(x[:, cfg.seq + i]))
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        ctx.barrier()
+        begin.record()
+        graph.replay()
+        end.record()
+        outs.append(row.clone())
+        one.check()
+        times.append(begin.elapsed_time(end) * 1e3)
+    us = reduce_ranks(ctx, sorted(times)[len(times) // 2], "max")
+    if rank == 0:
+        print(f"decode x{cfg.n_layers} layers, W={world}, {cfg.batch} sequences of {cfg.seq} to {total} tokens: {us:.0f} us a step",
+              flush=True)
+    ok = bool(torch.isfinite(torch.stack(outs).float()).all()) and cache[0].lens.tolist() == [total] * cfg.batch
+    if args.validate:
+        want = reference_forward(x.reshape(-1, cfg.hidden), replace(cfg, seq=total)).view(cfg.batch, total, -1)
+        pairs = [(prompts, shard(want[:, :cfg.seq].reshape(-1, cfg.hidden)))]
+        pairs += [(o, shard(want[:, cfg.seq + i])) for i, o in enumerate(outs)]
+        worst = max(((o.float() - w).norm() / w.norm()).item() for o, w in pairs)
+        ok = ok and worst < 2e-2      # (the bf16 residual stream of four layers alone is 1.1e-2 from the oracle)
+        ctx.log(f"Validation {'successful' if ok else 'FAILED'}: relative difference from the oracle at most {worst:.4f}")
+    one.close()
+    prefill.close()
+    ctx.barrier()
+    ctx.close()
+    if not ok:
+        raise SystemExit(1)
 
 
 def main():
@@ -29,6 +85,13 @@ def main():
     ap.add_argument("--seq", type=int, default=2048)
     ap.add_argument("--attention", default="iris", choices=["iris", "sdpa"],
                     help="attention core of the fused stack: this repository's tcgen05 kernel or the library call")
+    ap.add_argument("--decode", type=int, default=0, metavar="N", help="prompts, then N tokens one by one over a paged cache")
+    ap.add_argument("--kv_heads", type=int, default=0, help="key heads (0: as many as heads)")
+    ap.add_argument("--qk_norm", action="store_true", help="norms of query and key heads")
+    ap.add_argument("--rope_theta", type=float, default=0.0, help="rotation by position (0: none)")
+    ap.add_argument("--window", type=int, default=0, help="sliding window (0: all keys)")
+    ap.add_argument("--sinks", type=int, default=0, help="first keys that stay visible behind a window")
+    ap.add_argument("--page_size", type=int, default=16)
     ap.add_argument("--variant", default="two_shot",
                     choices=["two_shot", "two_shot_push", "one_shot", "atomic", "auto", "reduce_scatter"],
                     help="row-parallel projections: an all-reduce variant, or reduce_scatter (every rank receives only its "
@@ -46,12 +109,18 @@ def main():
                     help="vmm + IRIS_NVLS=1 in the environment binds the heap to an NVLS multicast object")
     args = ap.parse_args()
     cfg = TPConfig(hidden=args.hidden, n_heads=args.heads, head_dim=args.head_dim, intermediate=args.intermediate,
-                   n_layers=args.layers, batch=args.batch, seq=args.seq)
+                   n_layers=args.layers, batch=args.batch, seq=args.seq, n_kv_heads=args.kv_heads, qk_norm=args.qk_norm,
+                   rope_theta=args.rope_theta, window=args.window, sinks=args.sinks, positions=args.seq + args.decode)
+    if not (cfg.plain or args.decode):
+        ap.error("positions, head norms, windows and grouped heads are for --decode: the library stack does not have them")
     ctx = iris.iris(args.heap_size, heap_mode=args.heap_mode)
     rank, world = ctx.get_rank(), ctx.get_num_ranks()
     dev = ctx.get_device()
     device_barrier(ctx)
     model = TPDecoder(ctx, cfg, variant=args.variant, attention=args.attention)
+    if args.decode:
+        decode(ctx, cfg, model, args)
+        return
     base = TPDecoderBaseline(cfg, rank, world, dev, scatter=args.variant == "reduce_scatter")
     g = torch.Generator(device=dev).manual_seed(cfg.seed)
     x = torch.randn((cfg.tokens, cfg.hidden), generator=g, device=dev).to(torch.bfloat16)

@@ -128,3 +128,17 @@ def test_refusals():
     with pytest.raises(ValueError):
         TPDecoderBaseline(cfg, 0, 1, "cuda")
     model.close(), ctx.close()
+
+
+def test_example_decodes():
+    """The example runs its prompts and tokens and agrees with the oracle."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    args = ("--hidden 512 --heads 4 --kv_heads 2 --intermediate 1024 --layers 2 --batch 2 --seq 60 --decode 5 --rope_theta 10000 "
+            "--qk_norm --window 30 --sinks 2 -v --heap_size 268435456").split()
+    run = subprocess.run([sys.executable, os.path.join(root, "examples", "10_tp_block", "tp_block.py"), *args], capture_output=True,
+                         text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
+    assert "us a step" in run.stdout
