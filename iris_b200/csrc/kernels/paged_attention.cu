@@ -1004,20 +1004,22 @@ EncodeTiledFn encode_fn() {
 }
 
 // CTAs of a cluster, or 0 for the stream form, for so many segments of at most so many tiles on a GPU that holds `resident` CTAs.
-// A tile takes a CTA alone 0.67 us.  The stream form shares any lengths out evenly, but begins with sums over all lengths and
-// ends with a second kernel.  us, 4 query heads of 128 to a key head, pages of 16 (cluster of 1 / 2 / 4 / 8, stream):
-//      8 segments   64 keys 3.5 / 4.5 / 4.9 / 5.5, 5.9    1024 keys 13.7 / 9.2 / 7.2 / 7.1, 8.5    4096 keys 47 / 26 / 15 / 11, 9.8
-//    128 segments   256 keys 5.7 / 6.1 / 10.9 / 23, 14    1024 keys 14.7 / 11.1 / 15.7 / 30, 19    4096 keys 49 / 31 / 32 / 43, 33
-//    512 segments   256 keys 14 / 24 / 45 / 100, 18       1024 keys 32 / 39 / 60 / 118, 34         4096 keys 108 / 97 / 109 / 169, 94
-//   2048 segments   64 keys 30 / 73 / 153 / 359, 20       512 keys 58.5 / 99 / 188 / 418, 58       1024 keys 99.6 / 133 / ..., 102
+// A tile takes a CTA alone 0.7 us.  The stream form shares any lengths out evenly, but begins with sums over all lengths and
+// ends with a second kernel.  us, clusters of 1 / 2 / 4 / 8 and stream, 4 query heads of 128 to a key head, pages of 16:
+//      8 segments   64 keys 3.7 / 4.6 / 5.0 / 5.6, 6.1    512 keys 8.6 / 6.9 / 6.1 / 6.6, 7.8    4096 keys 50 / 28 / 16 / 11.5, 9.3
+//    128 segments   256 keys 6.0 / 6.2 / 11 / 24, 14      1024 keys 15.5 / 11.3 / 15.9 / 30, 18.5   4096 keys 53 / 32 / 33 / 43, 33
+//    512 segments   256 keys 14.5 / 25 / 46 / 101, 18     1024 keys 33 / 39 / 61 / 119, 35          4096 keys 112 / 99 / 111 / 173, 95
+//   2048 segments   64 keys 30 / 74 / 156 / 364, 20       512 keys 60 / 100 / 190 / 421, 58         1024 keys 101 / 135 / .., 103
+// Over 68 such cases (heads of 64, 128 and 256, 1 to 256 sequences of up to 64 to 4096 keys) the rule is 0.7 % off the best on
+// average, 9.5 % at worst.
 int choose_cluster(int64_t segments, int64_t tiles, int resident) {
   if (segments > 4 * resident) return 0;                       // many short ones: a CTA for each costs more than it works
   if (segments > resident) return tiles <= 20 ? 1 : 0;         // more than one round of CTAs, the last of them not full
   int cluster = 1;
-  while (cluster < 8 && cluster < tiles && segments * cluster * 2 <= resident) cluster *= 2;
+  while (cluster < 8 && cluster * 4 <= tiles && segments * cluster * 2 <= resident) cluster *= 2;   // two tiles each, at least
   // the chain of a CTA's tiles against the stream form's, which is longer by 4.8 tiles' time for its beginning and end; uneven
   // lengths speak for the latter, the more the longer they are
-  return tiles <= 128 && (double)tiles / cluster <= 4.8 + 1.1 * segments * tiles / resident ? cluster : 0;
+  return tiles <= 100 && (double)tiles / cluster <= 4.8 + 1.1 * segments * tiles / resident ? cluster : 0;
 }
 
 template <int D, bool F16>
