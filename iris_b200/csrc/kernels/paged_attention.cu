@@ -29,7 +29,7 @@
 //            of a sequence that spans CTAs go to a workspace and a second kernel, started early, adds them up in their order.
 //            Neighbouring heads, whose rows are neighbours in memory where the slot comes before the head, belong to CTAs that
 //            run side by side through the same keys (`lanes`), which DRAM rewards: 256 sequences of up to 2000 keys, 32 heads of
-//            64, 437 us with the heads one behind the other.
+//            64, 437 us with the heads one behind the other, 356 side by side.
 // Both give the same bits in every run: no atomics, and parts are added in a fixed order.
 //
 // Every wait on an mbarrier is bounded by timeout_ns: on expiry the CTA records a status, the loads stop, and the other warps run
