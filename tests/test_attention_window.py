@@ -160,6 +160,28 @@ def test_output_over_the_queries(batch, seq, heads, kv):
 
 
 @gpu
+def test_offsets_beyond_32_bits():
+    """A matrix of more than 2^31 elements: the last rows of the last head are those of a short matrix with the same keys."""
+    seq, heads, window = 180000, 32, 100
+    width = 3 * heads * 128
+    qkv = torch.zeros((seq, width), dtype=torch.bfloat16, device="cuda")
+    assert qkv.numel() > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(1)
+    tail = torch.randn((256, width), generator=g, device="cuda").to(torch.bfloat16)
+    qkv[-256:] = tail
+    out = torch.empty((seq, heads * 128), dtype=torch.bfloat16, device="cuda")
+    A.attention_window_fwd(qkv, out, 1, seq, heads, window=window)
+    for h in (0, heads - 1):
+        part = torch.cat([tail[:, (n * heads + h) * 128:(n * heads + h + 1) * 128] for n in range(3)], 1)
+        ref = torch.empty((256, 128), dtype=torch.bfloat16, device="cuda")
+        A.attention_window_fwd(part, ref, 1, 256, 1, window=window)
+        # of the same keys, but grouped into other tiles: each is within the bounds of _check, the values' maximum times 2^-7
+        got = out[-256:, h * 128:(h + 1) * 128]
+        bound = 2 * 1.05 * 2.0 ** -7 * tail[:, 2 * heads * 128:].abs().max().item()
+        assert (got[window:].float() - ref[window:].float()).abs().max().item() <= bound
+
+
+@gpu
 def test_no_rows():
     qkv, _, out = _inputs(1, 4, 2, 1, torch.bfloat16)
     assert A.attention_window_fwd(qkv[:0], out[:0], 0, 4, 2, 1, window=4).shape == (0, 256)

@@ -197,6 +197,25 @@ def test_without_rotation(norm):
 
 
 @gpu
+def test_offsets_beyond_32_bits():
+    """A matrix of more than 2^31 elements, in place: its last rows have the bits of the same rows alone."""
+    tokens, heads = 180000, 32
+    width = 3 * heads * 128
+    qkv = torch.zeros((tokens, width), dtype=torch.bfloat16, device="cuda")
+    assert qkv.numel() > 2 ** 31
+    c = Case(50, heads, heads, 128, 128, torch.bfloat16)
+    qkv[-50:] = c.qkv
+    pos = torch.zeros(tokens, dtype=torch.int32, device="cuda")
+    pos[-50:] = c.pos
+    slots = torch.full((tokens,), -1, dtype=torch.int32, device="cuda")
+    slots[-50:] = c.slots
+    R.qk_norm_rope(qkv, qkv, pos, c.table, heads, heads, 128, **c.kw(), k_cache=c.k, v_cache=c.v, slots=slots)
+    c.out.copy_(qkv[-50:])
+    c.check()
+    assert bool((qkv[:-50] == 0).all())
+
+
+@gpu
 def test_no_tokens():
     c = Case(4, 2, 1, 64, 64, torch.bfloat16)
     out = c.out[:0]
