@@ -1010,8 +1010,8 @@ EncodeTiledFn encode_fn() {
 //    128 segments   256 keys 6.0 / 6.2 / 11 / 24, 14      1024 keys 15.5 / 11.3 / 15.9 / 30, 18.5   4096 keys 53 / 32 / 33 / 43, 33
 //    512 segments   256 keys 14.5 / 25 / 46 / 101, 18     1024 keys 33 / 39 / 61 / 119, 35          4096 keys 112 / 99 / 111 / 173, 95
 //   2048 segments   64 keys 30 / 74 / 156 / 364, 20       512 keys 60 / 100 / 190 / 421, 58         1024 keys 101 / 135 / .., 103
-// Over 68 such cases (heads of 64, 128 and 256, 1 to 256 sequences of up to 64 to 4096 keys) the rule is 0.7 % off the best on
-// average, 9.5 % at worst.
+// Over 68 such cases (heads of 64, 128 and 256, 1 to 256 sequences of up to 64 to 4096 keys) the rule is 0.6 % off the best on
+// average, 9 % at worst.
 int choose_cluster(int64_t segments, int64_t tiles, int resident) {
   if (segments > 4 * resident) return 0;                       // many short ones: a CTA for each costs more than it works
   if (segments > resident) return tiles <= 20 ? 1 : 0;         // more than one round of CTAs, the last of them not full
@@ -1019,7 +1019,7 @@ int choose_cluster(int64_t segments, int64_t tiles, int resident) {
   while (cluster < 8 && cluster * 4 <= tiles && segments * cluster * 2 <= resident) cluster *= 2;   // two tiles each, at least
   // the chain of a CTA's tiles against the stream form's, which is longer by 4.8 tiles' time for its beginning and end; uneven
   // lengths speak for the latter, the more the longer they are
-  return tiles <= 100 && (double)tiles / cluster <= 4.8 + 1.1 * segments * tiles / resident ? cluster : 0;
+  return tiles <= 100 && (double)tiles / cluster <= 4.8 + (double)segments * tiles / resident ? cluster : 0;
 }
 
 template <int D, bool F16>

@@ -50,37 +50,47 @@ struct Params {
   float eps;
 };
 
-template <bool F16>
-__device__ __forceinline__ void unpack8(uint4 v, float* f) {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = F16 ? __half22float2(*reinterpret_cast<const __half2*>(w + i))
-                         : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(w + i));
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 template <bool F16>
-__device__ __forceinline__ uint4 pack8(const float* f) {
-  uint4 o;
-  uint32_t* w = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (F16) {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
+__device__ __forceinline__ float2 unpack(uint32_t v) {
+  return F16 ? __half22float2(*reinterpret_cast<const __half2*>(&v)) : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack(float2 f) {
+  if (F16) {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  return o;
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// (a, b) turned by the angles whose cosines and sines are c and s.
+__device__ __forceinline__ void turn(float2& a, float2& b, float2 c, float2 s) {
+  const float2 x = fma2(mul2(b, s), make_float2(-1.f, -1.f), mul2(a, c));
+  b = fma2(a, s, mul2(b, c));
+  a = x;
 }
 
 // LANES: lanes of a head, the power of two from dim / 16 on.  HEADS: heads of a lane.  A block has `spread` groups of lanes to a
 // token; block (x, y): tokens x * (groups / spread) on, heads y * spread * HEADS on.  (64 registers, four blocks to an SM, although
-// that spills a little: 16384 tokens of 96 heads of 128, 181 us with 78 registers, 173 with 64; two heads to a lane 195.)
+// that spills a little: 16384 tokens of 96 heads of 128, 181 us with 78 registers, 173 with 64; two heads to a lane 195.  fp32
+// arithmetic two operations to an instruction: 177 -> 172 us there, 89 -> 86 with 48 heads.)
 template <int LANES, bool F16, bool INTERLEAVED, int HEADS>
 __global__ void __launch_bounds__(kThreads, HEADS == 1 ? 5 : 4) qk_norm_rope_kernel(const __grid_constant__ Params p) {
   constexpr int kGroups = kThreads / LANES, kHeads = HEADS;
@@ -119,13 +129,14 @@ __global__ void __launch_bounds__(kThreads, HEADS == 1 ? 5 : 4) qk_norm_rope_ker
   const bool keep = slot >= 0 && slot < p.cache_slots;
   const int64_t cached = keep ? (slot >> p.page_shift) * p.page_pitch + (slot & ((1 << p.page_shift) - 1)) * p.slot_pitch : 0;
 
-  float cs[8], sn[8];
+  float2 cs[4], sn[4];
   if (turns) {
     const float* row = p.table + pos * p.ld_table + lane * 8;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      *reinterpret_cast<float4*>(cs + 4 * i) = *reinterpret_cast<const float4*>(row + 4 * i);
-      *reinterpret_cast<float4*>(sn + 4 * i) = *reinterpret_cast<const float4*>(row + p.half + 4 * i);
+      const float4 c = *reinterpret_cast<const float4*>(row + 4 * i), s = *reinterpret_cast<const float4*>(row + p.half + 4 * i);
+      cs[2 * i] = make_float2(c.x, c.y), cs[2 * i + 1] = make_float2(c.z, c.w);
+      sn[2 * i] = make_float2(s.x, s.y), sn[2 * i + 1] = make_float2(s.z, s.w);
     }
   }
   uint8_t* dst = p.out + token * p.ld_out;
@@ -134,51 +145,55 @@ __global__ void __launch_bounds__(kThreads, HEADS == 1 ? 5 : 4) qk_norm_rope_ker
     const int h = head0 + u * spread;
     if (h >= all) break;                                  // (the same for all lanes of a head)
     if (h < p.heads + p.kv_heads) {
-      float a[8], b[8];
+      float2 y[2][4];                                     // the two pieces
       if (live) {
-        unpack8<F16>(x[u][0], a);
-        unpack8<F16>(x[u][1], b);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(&x[u][i]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[i][k] = unpack<F16>(w[k]);
+        }
       }
       const uint8_t* weight = h < p.heads ? p.q_weight : p.k_weight;
       if (weight) {
-        float ss = 0.f;
+        float2 ss = make_float2(0.f, 0.f);
         if (live) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+          for (int k = 0; k < 4; ++k) ss = fma2(y[0][k], y[0][k], fma2(y[1][k], y[1][k], ss));
         }
+        float sum = ss.x + ss.y;
         // (the groups of a warp may have left the loop at different heads)
         const uint32_t lanes = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1) << (threadIdx.x & 31 & ~(LANES - 1));
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(lanes, ss, o);
-        const float scale = rsqrtf(ss / (float)p.dim + p.eps);
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(lanes, sum, o);
+        const float scale = rsqrtf(sum / (float)p.dim + p.eps);
         if (live) {
-          float w[8];
-          unpack8<F16>(*reinterpret_cast<const uint4*>(weight + c0 * 2), w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) a[i] *= scale * w[i];
-          unpack8<F16>(*reinterpret_cast<const uint4*>(weight + c1 * 2), w);
+          for (int i = 0; i < 2; ++i) {
+            const uint4 w = *reinterpret_cast<const uint4*>(weight + (i ? c1 : c0) * 2);
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(&w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) b[i] *= scale * w[i];
+            for (int k = 0; k < 4; ++k) y[i][k] = mul2(y[i][k], mul2(unpack<F16>(v[k]), make_float2(scale, scale)));
+          }
         }
       }
       if (turns) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (INTERLEAVED) {
-            float* f = i < 4 ? a + 2 * i : b + 2 * i - 8;
-            const float e = f[0], d = f[1];
-            f[0] = e * cs[i] - d * sn[i];
-            f[1] = d * cs[i] + e * sn[i];
+        for (int k = 0; k < 4; ++k) {
+          if (INTERLEAVED) {     // pairs 2 k and 2 k + 1 of the lane's eight: two neighbouring words of a piece
+            float2 &f = y[k >> 1][2 * (k & 1)], &g = y[k >> 1][2 * (k & 1) + 1];
+            float2 e = make_float2(f.x, g.x), d = make_float2(f.y, g.y);
+            turn(e, d, cs[k], sn[k]);
+            f = make_float2(e.x, d.x), g = make_float2(e.y, d.y);
           } else {
-            const float e = a[i], d = b[i];
-            a[i] = e * cs[i] - d * sn[i];
-            b[i] = d * cs[i] + e * sn[i];
+            turn(y[0][k], y[1][k], cs[k], sn[k]);
           }
         }
       }
       if (live) {
-        x[u][0] = pack8<F16>(a);
-        x[u][1] = pack8<F16>(b);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          x[u][i] = make_uint4(pack<F16>(y[i][0]), pack<F16>(y[i][1]), pack<F16>(y[i][2]), pack<F16>(y[i][3]));
       }
     }
     if (!live) continue;
@@ -210,17 +225,25 @@ cudaError_t launch_as(const cudaLaunchConfig_t& cfg, const Params& p, int f16, i
                            : cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<LANES, false, false, HEADS>, p);
 }
 
+constexpr double kWorth[4] = {0., 0.80, 0.95, 1.00};   // of a place, by the heads of a lane (0.70 / 0.90 and 0.90 / 1.00: no better)
 template <int LANES>
 cudaError_t launch(Params& p, int64_t tokens, int f16, int interleaved, void* stream) {
   constexpr int kGroups = kThreads / LANES;
   const int all = p.heads + 2 * p.kv_heads;
-  // few heads: several tokens to a block; many: up to three heads to a lane, in as few blocks a token as that takes
-  p.token_shift = 0;
-  while ((kGroups >> (p.token_shift + 1)) >= all) ++p.token_shift;
-  const int passes = (all + kGroups - 1) / kGroups, blocks = (passes + 2) / 3, heads = (passes + blocks - 1) / blocks;
+  // groups of lanes to a token (a power of two, so one or more tokens to a block) and heads of a lane: the fewest places without a
+  // head, and of those the most heads to a lane.  (16384 tokens: 32 + 8 + 8 heads of 128, always 32 groups to a token 101 us, so
+  // 88; 8 + 1 + 1 heads, one head to a lane 30 us, so 22.)
+  int blocks = 0, heads = 0;
+  double best = 0.;
+  for (int shift = 0; (kGroups >> shift) > 0; ++shift)
+    for (int h = 1; h <= 3; ++h) {
+      const int places = (kGroups >> shift) * h, n = (all + places - 1) / places;
+      const double worth = (double)all / (n * places) * kWorth[h];
+      if (worth > best) best = worth, blocks = n, heads = h, p.token_shift = shift;
+    }
   p.tokens = tokens;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((tokens + (1 << p.token_shift) - 1) >> p.token_shift), (all + kGroups * heads - 1) / (kGroups * heads));
+  cfg.gridDim = dim3((unsigned)((tokens + (1 << p.token_shift) - 1) >> p.token_shift), blocks);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
