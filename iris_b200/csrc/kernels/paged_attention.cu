@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
           }
         } else {
           // pages of 8 (half of a block of which no key is seen is copied all the same, from page 0)
-#pragma unroll 1
+#pragma unroll
           for (int i = 0; i < 2 * kTB; ++i) {
             const int page = __shfl_sync(0xffffffffu, i & 1 ? now.page2 : now.page, first_lane + i / 2);
             if (one && (blocks >> i / 2 & 1)) {
@@ -425,36 +425,42 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
           for (int r = 0; r < rows; ++r) bulk_load(dst + r * S::kQPitch, src + r * p.q_head, D * 2, full(stage));
         }
       } else {
-        // pages of fewer than 8 keys: looked up a key a lane, copied a page at a time
+        // pages of fewer than 8 keys: looked up a key a lane, all blocks at once, and copied a page at a time
         const int size = 1 << p.page_shift;
-        uint32_t bytes = 0;
-        for (int pass = 0; pass < 2; ++pass) {   // count, then copy
-          for (int b = 0; b < kTB; ++b) {
-            const uint32_t m = __shfl_sync(0xffffffffu, now.mask, first_lane + b);
-            const int key = __shfl_sync(0xffffffffu, now.key, first_lane + b) + (lane & 15);
-            const bool in = m >> (lane & 15) & 1;
-            const int page = in ? p.table[l.b * p.table_pitch + (key >> p.page_shift)] : -1;
-            const bool good = in && (uint32_t)page < (uint32_t)p.pages;
-            if (pass == 0 && in && !good) record_status(p.status, kBadPointer, kSitePage, l.b, key, (uint64_t)(int64_t)page);
-            const uint32_t got = __ballot_sync(0xffffffffu, good) & 0xffffu;
-            if (pass == 0 && lane == 0) masks[stage * kTB + b] = got;
-            for (int j = 0; j < kBlock; j += size) {
-              const uint32_t part = got >> j & ((1u << size) - 1);
-              const int from = __shfl_sync(0xffffffffu, page, part ? j + __ffs(part) - 1 : 0);
-              if (!part) continue;
-              if (pass == 0) {
-                bytes += size * 128 * 2 * S::kPanels;
-              } else if (lane == 0) {
-                const uint32_t at = tile + b * S::kBlockBytes + j * 128;
-                for (int h = 0; h < S::kPanels; ++h) {
-                  tma_load_4d(at + h * S::kPanel, &p.k, h * 64, kv, 0, from, full(stage));
-                  tma_load_4d(at + h * S::kPanel + kHalfBlock, &p.v, h * 64, kv, 0, from, full(stage));
-                }
+        int page[kTB];
+        uint32_t got[kTB], bytes = 0;
+#pragma unroll
+        for (int b = 0; b < kTB; ++b) {
+          const uint32_t m = __shfl_sync(0xffffffffu, now.mask, first_lane + b);
+          const int key = __shfl_sync(0xffffffffu, now.key, first_lane + b) + (lane & 15);
+          got[b] = m >> (lane & 15) & 1;
+          page[b] = got[b] ? p.table[l.b * p.table_pitch + (key >> p.page_shift)] : -1;
+        }
+#pragma unroll
+        for (int b = 0; b < kTB; ++b) {
+          const bool good = got[b] && (uint32_t)page[b] < (uint32_t)p.pages;
+          if (got[b] && !good) record_status(p.status, kBadPointer, kSitePage, l.b, b, (uint64_t)(int64_t)page[b]);
+          got[b] = __ballot_sync(0xffffffffu, good) & 0xffffu;
+          if (lane == 0) masks[stage * kTB + b] = got[b];
+          for (int j = 0; j < kBlock; j += size)
+            if (got[b] >> j & ((1u << size) - 1)) bytes += size * 128 * 2 * S::kPanels;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(full(stage), bytes + rows * D * 2);
+#pragma unroll
+        for (int b = 0; b < kTB; ++b) {
+          for (int j = 0; j < kBlock; j += size) {
+            const uint32_t part = got[b] >> j & ((1u << size) - 1);
+            const int from = __shfl_sync(0xffffffffu, page[b], part ? j + __ffs(part) - 1 : 0);
+            if (part && lane == 0) {
+              const uint32_t at = tile + b * S::kBlockBytes + j * 128;
+#pragma unroll
+              for (int h = 0; h < S::kPanels; ++h) {
+                tma_load_4d(at + h * S::kPanel, &p.k, h * 64, kv, 0, from, full(stage));
+                tma_load_4d(at + h * S::kPanel + kHalfBlock, &p.v, h * 64, kv, 0, from, full(stage));
               }
             }
           }
-          __syncwarp();
-          if (pass == 0 && lane == 0) mbar_expect_tx(full(stage), bytes + rows * D * 2);
         }
         if (lane == 0) {
           const uint8_t* src = p.q + l.b * p.q_batch + (int64_t)(kv * p.group + r0) * p.q_head;
