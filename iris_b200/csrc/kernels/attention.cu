@@ -371,14 +371,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
           if (i + lead < it.n) load_kv(xk, key_row(i + lead));
         }
       }
-      if (*abort_flag) {   // loads in flight still write into shared memory: wait for each, bounded
-        for (int s = 0; s < kSlots; ++s) {
-          const uint32_t n = (pos + kSlots - 1 - s) / kSlots;
-          if (n > 0) mbar_wait(kv_full(s), (n - 1) & 1, 200000, never);
-        }
-        for (int x = 0; x < 2; ++x)
-          if (qn[x] > 0) mbar_wait(q_full(x), (qn[x] - 1) & 1, 200000, never);
+      // loads in flight write into shared memory, also if the other warps give up later: wait for each, bounded
+      for (int s = 0; s < kSlots; ++s) {
+        const uint32_t n = (pos + kSlots - 1 - s) / kSlots;
+        if (n > 0) mbar_wait(kv_full(s), (n - 1) & 1, 200000, never);
       }
+      for (int x = 0; x < 2; ++x)
+        if (qn[x] > 0) mbar_wait(q_full(x), (qn[x] - 1) & 1, 200000, never);
     }
   } else if (warp == 9) {
     if (elect_one()) {   // elect.sync, not a lane number: see the same place in gemm_local.cu
@@ -509,10 +508,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
         it = nx;
         have = more;
       }
-      if (*abort_flag) {   // MMAs in flight still use shared and tensor memory
-        umma_commit(drain_bar);
-        mbar_wait(drain_bar, 0, 200000, never);
-      }
+      // MMAs in flight use shared and tensor memory, also if the softmax warps give up later
+      umma_commit(drain_bar);
+      mbar_wait(drain_bar, 0, 200000, never);
     }
   } else {
     // ---- softmax: one thread per query row ----
@@ -538,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
       float m_run = -INFINITY, l_run = 0.f;
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
-        if (!mbar_wait(s_full(x), sn & 1, p.timeout_ns, abort_flag)) {
+        if (!mbar_wait_warp(s_full(x), sn & 1, p.timeout_ns, abort_flag)) {
           stop(j, 1);
           break;
         }
@@ -729,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
       };
       if (!SPLIT) {
         if (!ok) break;
-        if (!mbar_wait(o_full(x), dn & 1, p.timeout_ns, abort_flag)) {
+        if (!mbar_wait_warp(o_full(x), dn & 1, p.timeout_ns, abort_flag)) {
           stop(n, 2);
           break;
         }
@@ -758,9 +756,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
         __syncwarp();
         if (lane == 0) mbar_arrive(merge_bar);
         if (!ok) break;
-        bool w = mbar_wait(merge_bar, dn & 1, p.timeout_ns, abort_flag);
-        w = w && mbar_wait(o_full(0), dn & 1, p.timeout_ns, abort_flag);
-        if (it.nb > 0) w = w && mbar_wait(o_full(1), bn & 1, p.timeout_ns, abort_flag);
+        bool w = mbar_wait_warp(merge_bar, dn & 1, p.timeout_ns, abort_flag);
+        w = w && mbar_wait_warp(o_full(0), dn & 1, p.timeout_ns, abort_flag);
+        if (it.nb > 0) w = w && mbar_wait_warp(o_full(1), bn & 1, p.timeout_ns, abort_flag);
         if (!w) {
           stop(n, 3);
           break;

@@ -58,6 +58,7 @@ constexpr int kRows = 16;                        // query heads of a segment, at
 constexpr int kBlock = 16;                       // keys of a product
 constexpr int kHalfBlock = kBlock * 128;         // bytes of a block's keys (or values) in a panel
 constexpr int kJoinThreads = 512;
+constexpr int64_t kMostKeys = 0x7fffffff - 1023;   // of a sequence: positions are looked at up to a batch of blocks behind the last
 constexpr uint32_t kSitePage = 95, kSiteLoad = 98, kSiteTile = 99;
 
 template <int D, int COLS = 8>
@@ -355,17 +356,16 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
     };
     Cursor l = c, ahead = c;
     int ahead_left = count, in_batch = 0, stage = 0, q_buf = 0;
-    bool fresh = true, ok = true;             // fresh: the next tile is its segment's first here
+    bool fresh = true;                        // the next tile is its segment's first here
     Batch now = look_up(l, count);
     next_batch(ahead, ahead_left);
     Batch next = look_up(ahead, ahead_left);
     int issued = 0;
     for (; issued < count; ++issued) {
       const int use = issued / S::kStages;
-      if (use > 0 && !mbar_wait(empty(stage), (use - 1) & 1, p.timeout_ns, abort_flag)) {
+      if (use > 0 && !mbar_wait_warp(empty(stage), (use - 1) & 1, p.timeout_ns, abort_flag)) {
         if (lane == 0) record_status(p.status, kTimeout, kSiteLoad, blockIdx.x, issued, 0);
         *abort_flag = 1;
-        ok = false;
         break;
       }
       const int first_lane = in_batch * kTB;
@@ -479,12 +479,12 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
         next = look_up(ahead, ahead_left);
       }
     }
-    if (!ok) {   // loads in flight still write into shared memory: wait for each, bounded
-      for (int s = 0; s < S::kStages; ++s) {
-        const int n = (issued + S::kStages - 1 - s) / S::kStages;
-        if (n > 0) mbar_wait(full(s), (n - 1) & 1, 200000, never);
-      }
+    // loads in flight write into this CTA's shared memory, whether the other warps still wait for them or not: wait for each, bounded
+    for (int s = 0; s < S::kStages; ++s) {
+      const int n = (issued + S::kStages - 1 - s) / S::kStages;
+      if (n > 0) mbar_wait(full(s), (n - 1) & 1, 200000, never);
     }
+    __syncwarp();
     if (CLUSTER && gridDim.x > 1) {
       cluster_sync_all();
       cluster_sync_all();
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
 
 #pragma unroll 1
   for (int i = 0; i < count; ++i) {
-    if (ok && !mbar_wait(full(stage), parity, p.timeout_ns, abort_flag)) {
+    if (ok && !mbar_wait_warp(full(stage), parity, p.timeout_ns, abort_flag)) {
       if (lane == 0) record_status(p.status, kTimeout, kSiteTile, blockIdx.x, i, 0);
       *abort_flag = 1;
       ok = false;
@@ -743,7 +743,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
       fence_proxy_async_smem();
       __syncwarp();
     }
-    if (lane == 0) mbar_arrive(empty(stage));
+    if (lane == 0 && ok) mbar_arrive(empty(stage));   // (a warp that gave up frees none, so nothing is copied over a copy on its way)
     advance<D>(p, c);
     if (++stage == S::kStages) {
       stage = 0;
@@ -1108,6 +1108,7 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
   if (dtype != 0 && dtype != 1) return refuse("dtype must be 0 (bf16) or 1 (fp16)");
   if (page_size < 1 || (page_size & (page_size - 1))) return refuse("page size must be a power of two");
   if (pages < 1 || wide < 1 || pages > 0x7fffffff || wide > 0x7fffffff || batch > 0x7fffffff || page_size > (1 << 30)) return refuse("no pages, or too many");
+  if (wide * page_size > kMostKeys) return refuse("the block table is for more than 2^31 - 1024 keys of a sequence");
   const float scale_log2 = (float)(scale * 1.4426950408889634);
   if (window < 0 || sinks < 0 || !(scale_log2 > 0.f) || isinf(scale_log2)) return refuse("window and sinks must not be negative, scale above 0");
   // a pitch along one element says nothing
@@ -1121,6 +1122,25 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
     return refuse("rows of q, k, v and out must start on 16 bytes");
   if ((pages > 1 && page_pitch < dim) || (page_size > 1 && slot_pitch < dim) || (kv_heads > 1 && head_pitch < dim))
     return refuse("rows of the cache must not overlap");
+  const uint8_t *q8 = static_cast<const uint8_t*>(q), *out8 = static_cast<const uint8_t*>(out);
+  const auto past = [](int64_t a, int64_t pa, int64_t b, int64_t pb, int64_t c, int64_t pc, int64_t n) {   // bytes of a view
+    return ((a - 1) * pa + (b - 1) * pb + (c - 1) * pc + n) * 2;
+  };
+  const int64_t q_bytes = past(batch, q_batch, heads, q_head, 1, 0, dim), out_bytes = past(batch, out_batch, heads, out_head, 1, 0, dim);
+  const int64_t cache_bytes = past(pages, page_pitch, page_size, slot_pitch, kv_heads, head_pitch, dim);
+  for (const void* c : {k, v})
+    if (out8 < static_cast<const uint8_t*>(c) + cache_bytes && static_cast<const uint8_t*>(c) < out8 + out_bytes)
+      return refuse("out must not lie in the cache");
+  // out is q itself, or none of its heads meets one of q's
+  if (out8 < q8 + q_bytes && q8 < out8 + out_bytes && !(out8 == q8 && out_batch == q_batch && out_head == q_head)) {
+    bool apart = out_batch == q_batch && out_head == q_head;
+    for (int64_t j = 1 - heads; apart && j < heads; ++j) {
+      const int64_t off = (out8 - q8) / 2 + j * q_head, last = q_batch ? off / q_batch : 0;
+      for (int64_t i = last - 1; i <= last + 1; ++i)
+        if (i > -batch && i < batch && off - i * q_batch > -dim && off - i * q_batch < dim) apart = false;
+    }
+    if (!apart) return refuse("out must be q itself, or share no memory with it");
+  }
   const int sms = sms_of((int)device);
   if (sms < 1) return refuse("no device");
   Params p;
@@ -1141,7 +1161,7 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
   if (cluster < 0) {
     int64_t most = wide * (int64_t)page_size;
     if (longest > 0 && longest < most) most = longest;
-    if (window > 0 && window < most && window + sinks < most) most = window + sinks;
+    if (window > 0 && window < most && sinks < most - window) most = window + sinks;
     const int64_t tile = dim == 64 ? Shape<64>::kTile : dim == 128 ? Shape<128>::kTile : Shape<256>::kTile;
     const int64_t tiles = (most + tile - 1) / tile;
     cluster = choose_cluster(segments, tiles, resident);

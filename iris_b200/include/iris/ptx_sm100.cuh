@@ -63,6 +63,17 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_
     }
   }
 }
+// The same by a whole warp, whose lanes get one answer: what follows may be a collective of the warp.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, uint64_t timeout_ns,
+                                               volatile uint32_t* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = timer_ns();
+  uint32_t spins = 0;
+  for (;;) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((++spins & 63u) == 0 && __any_sync(0xffffffffu, *abort_flag || timer_ns() - t0 > timeout_ns)) return false;
+  }
+}
 
 // Whether the phase has completed, without waiting.
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {

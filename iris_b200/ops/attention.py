@@ -85,15 +85,16 @@ def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: 
     rows = batch * seq
     if rows == 0:
         return out
-    kv_ptr, out_ptr = qkv.data_ptr() + heads * HEAD_DIM * 2, out.data_ptr()
-    if rows > 1 and ld_out < heads * HEAD_DIM or may_overlap(rows, kv_ptr, ld_in, 2 * kv_heads * HEAD_DIM, out_ptr, ld_out, heads * HEAD_DIM):
-        raise ValueError("rows of out must not overlap, nor lie over keys or values")
+    qkv_ptr, out_ptr = qkv.data_ptr(), out.data_ptr()
+    if rows > 1 and ld_out < heads * HEAD_DIM or not (out_ptr == qkv_ptr and ld_out == ld_in) and may_overlap(
+            rows, qkv_ptr, ld_in, (heads + 2 * kv_heads) * HEAD_DIM, out_ptr, ld_out, heads * HEAD_DIM):
+        raise ValueError("rows of out must not overlap, nor lie over qkv but for the query columns themselves")
     if device != _native.current_device(device):
         with torch.cuda.device(device):
             return attention_window_fwd(qkv, out, batch, seq, heads, kv_heads, window=window, sinks=sinks, status=status,
                                         timeout_ms=timeout_ms, stream=stream)
     rc = _native.entry("iris_k_attention_window_fwd")(_WINDOW_ARGS.pack(
-        kv_ptr - heads * HEAD_DIM * 2, out_ptr, 0 if status is None else status.data_ptr(),
+        qkv_ptr, out_ptr, 0 if status is None else status.data_ptr(),
         torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, ld_in, ld_out, batch, seq, heads, kv_heads,
         window, sinks, _DT[dtype], int(timeout_ms * 1e6)))
     if rc != 0:

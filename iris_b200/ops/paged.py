@@ -69,10 +69,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``head_dim ** -0.5``.  ``lse`` fp32 ``[batch, heads]``: receives the logarithm of the softmax's sum.
 
     A sequence of no keys gets zeros (and minus infinity in ``lse``); a length beyond the table's width is cut to it, a negative
-    one counts as 0.  Keys and values behind a sequence's last key, or out of its window, reach nothing, NaN or not.  A
-    key whose table entry is no page is left out and recorded in ``status`` (an ``Iris`` context's status block) if that is
-    given, as is a bounded wait of the kernel that ran out.  ``longest``: what the lengths are expected not to exceed, where that is much less than the table's width; it is
-    for speed alone.
+    one counts as 0.  Keys and values behind a sequence's last key, or out of its window, reach nothing, NaN or not; a seen value
+    that is infinite makes its component infinite or NaN.  A key whose table entry is no page is left out and recorded in ``status``
+    (an ``Iris`` context's status block) if that is given, as is a bounded wait of the kernel that ran out (the output then means
+    nothing).  ``out`` may be ``q`` itself, and otherwise shares no memory with it or the cache.  ``longest``: what the lengths are
+    expected not to exceed, where that is much less than the table's width; it is for speed alone.
     """
     dtype, shape, cache_shape = q.dtype, q.shape, k_cache.shape
     if dtype not in _DT or out.dtype is not dtype or k_cache.dtype is not dtype or v_cache.dtype is not dtype:

@@ -182,6 +182,21 @@ def test_offsets_beyond_32_bits():
 
 
 @gpu
+@pytest.mark.parametrize("batch,seq,heads,kv", [(2, 300, 4, 2), (3, 640, 40, 8)])
+def test_waits_that_may_run_out(batch, seq, heads, kv):
+    """A limit of a microsecond: the call comes back, with or without having recorded that a wait ran out, with nothing left on its
+    way, and the next one is right."""
+    qkv, _, out = _inputs(batch, seq, heads, kv, torch.bfloat16)
+    status = torch.zeros(64, dtype=torch.int32, device="cuda")
+    for _ in range(20):
+        A.attention_window_fwd(qkv, out, batch, seq, heads, kv, window=100, timeout_ms=1e-3, status=status)
+    torch.cuda.synchronize()
+    assert status[0].item() in (0, 1), status[:8]
+    A.attention_window_fwd(qkv, out, batch, seq, heads, kv, window=100)
+    _check(qkv, out, batch, seq, heads, kv, 100, 0)
+
+
+@gpu
 def test_no_rows():
     qkv, _, out = _inputs(1, 4, 2, 1, torch.bfloat16)
     assert A.attention_window_fwd(qkv[:0], out[:0], 0, 4, 2, 1, window=4).shape == (0, 256)
@@ -200,6 +215,9 @@ def test_refusals():
     for bad in (wide[:, 512:1024], wide[:, 800:1312], wide[:1, :512].expand(20, -1)):      # over the keys; over the values; one row
         with pytest.raises(ValueError, match="overlap"):
             A.attention_window_fwd(**{**ok, "qkv": wide[:, :1024], "out": bad})
+    tall = torch.zeros((21, 1024), dtype=torch.bfloat16)                                 # the queries of the next token
+    with pytest.raises(ValueError, match="overlap"):
+        A.attention_window_fwd(**{**ok, "qkv": tall[:20], "out": tall[1:, :512]})
     for fine in (out, wide[:, :512], wide[:, 1024:1536]):                                # of its own; the queries; beside them
         with pytest.raises(ValueError, match="CUDA device"):
             A.attention_window_fwd(**{**ok, "qkv": wide[:, :1024], "out": fine})

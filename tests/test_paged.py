@@ -1,11 +1,13 @@
 """The paged cache's operators against plain implementations in 64 bits: attention of one new token, pages taken and given
 back, and the refusals of both."""
+import ctypes
 import math
 import random
 
 import pytest
 import torch
 
+from iris_b200 import _native
 from iris_b200.ops import paged as P
 
 gpu = pytest.mark.gpu
@@ -335,6 +337,58 @@ def test_attention_refusals_of_the_native_entry():
         P.paged_attention(c.q, c.k, c.v, c.table, c.len_t, c.out, scale=0.0)
     with pytest.raises(ValueError, match="one device"):
         P.paged_attention(c.q, c.k, c.v, c.table.cpu(), c.len_t, c.out)
+
+
+def _native_refusal(q, k, v, table, lens, out):
+    """What the native entry says to a call that it refuses before it looks for a device (no device needed)."""
+    (batch, heads, dim), (pages, size, kv, _) = q.shape, k.shape
+    rc = _native.entry("iris_k_paged_attention")(P._ATTENTION.pack(
+        *(t.data_ptr() for t in (q, k, v, table, lens, out)), 0, 0, 0, 0, *q.stride()[:2], *k.stride()[:3], table.stride(0),
+        *out.stride()[:2], 0, batch, heads, dim, pages, size, kv, table.shape[1], 0, 0, 0, 0, -1, 0, -1, 0, dim ** -0.5))
+    lib = _native.kernels()
+    lib.iris_paged_attention_last_error.restype = ctypes.c_char_p
+    assert rc < 0
+    return lib.iris_paged_attention_last_error().decode()
+
+
+def test_attention_output_that_shares_memory_is_refused():
+    """Over a part of the queries, or over the cache; the queries' own place and places beside them are none of that."""
+    c = Case([40, 3], 4, 2, 64, 16, torch.bfloat16, device="cpu")
+    rows = torch.zeros((4, 8, 2, 64), dtype=torch.bfloat16)
+    q, fine = rows[:2, :4, 0], "no device"
+    a = (q, c.k, c.v, c.table, c.len_t)
+    assert fine in _native_refusal(*a, q)
+    assert fine in _native_refusal(*a, rows[:2, :4, 1])      # between the heads
+    assert fine in _native_refusal(*a, rows[:2, 4:, 0])      # beside them
+    assert fine in _native_refusal(*a, rows[2:, :4, 0])
+    for bad in (rows[1:3, :4, 0], rows[:2, 1:5, 0], rows.flatten(1)[:2, 32:544].unflatten(1, (4, 128))[:, :, :64],
+                rows[:2].flatten(1)[:, :256].unflatten(1, (4, 64))):
+        assert "share no memory" in _native_refusal(*a, bad)
+    flat = torch.as_strided(c.k, (c.k.numel(),), (1,), c.k.storage_offset())
+    assert "cache" in _native_refusal(*a, flat[:512].view(2, 4, 64))
+
+
+def test_attention_table_of_too_many_keys_is_refused():
+    """Positions are counted in 32 bits, up to a batch of blocks behind the last key."""
+    c = Case([40, 3], 4, 2, 64, 16, torch.bfloat16, device="cpu")
+    wide = 2 ** 27
+    table = torch.as_strided(torch.zeros(1, dtype=torch.int32), (2, wide), (0, 0))
+    assert "2^31" in _native_refusal(c.q, c.k, c.v, table, c.len_t, c.out)
+    assert "no device" in _native_refusal(c.q, c.k, c.v, table[:, :wide - 64], c.len_t, c.out)
+
+
+@gpu
+def test_attention_whose_waits_may_run_out():
+    """A limit of a microsecond: the call comes back, with or without having recorded that a wait ran out, with no copy left on its
+    way, and the next one is right."""
+    for wide, batch in ((None, 5), (8000, 5), (8000, 300)):
+        case = Case([3000, 10, 800, 0, 77] * (batch // 5), 8, 2, 128, 16, torch.bfloat16, wide=wide)
+        status = torch.zeros(64, dtype=torch.int32, device="cuda")
+        for _ in range(20):
+            P.paged_attention(case.q, case.k, case.v, case.table, case.len_t, case.out, timeout_ms=1e-3, status=status)
+        torch.cuda.synchronize()
+        assert status[0].item() in (0, 1), status[:8]
+        case.run().check()
 
 
 # ---- pages --------------------------------------------------------------------------------------------------------------
