@@ -23,11 +23,12 @@
 //   warp 9          one elected thread issues tcgen05.mma:  S = Q K^T, then O += P V (P from tensor memory, V as an
 //                   MN-major operand: V[key][d] is read as stored), alternating between the sides; the first half of a
 //                   product starts when the first half of P is there
-// What bounds it: the chain of one side, scores -> softmax -> product: 4300 - 5000 cycles per step of a pair for 2048 of MMAs
+// What bounds it: the chain of one side, scores -> softmax -> product: 4100 - 4700 cycles per step of a pair for 2048 of MMAs
 // and 2048 of ex2; in a long run the GPU's power limit takes the clock besides.  8 x 2048 tokens x 32 heads bf16, causal /
-// without a mask: from a rest, 1965 MHz, 317 / 524 us; a run of seconds, 1635 / 1612 MHz at 1010 W, 349 / 585 us.  A scale that is renewed only after a growth of 2^8 takes 287 / 467 us
-// instead, but then a row's largest weight is rounded like the others and the error against 64 bits grows by 2 to 4 %
-// (2.034e-3 -> 2.071e-3, 2.256e-3 -> 2.337e-3, both bf16).
+// without a mask: from a rest, 1965 MHz, 298 / 499 us (317 / 524 with output rows written 16 bytes at a time); a run of seconds,
+// 1582 MHz at 990 W, 338 / 575 us.  A scale that is renewed only after a growth of 2^8 saved another 30 / 57 us from a rest, but
+// then a row's largest weight is rounded like the others and the error against 64 bits grows by 2 to 4 % (2.034e-3 -> 2.071e-3,
+// 2.256e-3 -> 2.337e-3, both bf16).
 // Before: one 128-row tile per CTA, two threads per row reading the scores twice, P through shared memory, O folded
 // through registers after every tile: 659 us causal, 1091 without a mask.
 //
@@ -619,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
         } else if (__any_sync(0xffffffffu, mx > m_run + (WIN ? kGrowth : 0.f))) {
           // Each row takes its new maximum at once, so that its largest weight is exactly 1 in the 16 bits of P, and what has
           // been summed is rescaled.  These scores are complete, so the products issued before them are too, and the next
-          // one waits for P.  (32 columns at a time and two to an instruction: 317 us for 8 x 2048 x 32 causal from a rest;
+          // one waits for P.  (32 columns at a time and two to an instruction: 317 us for 8 x 2048 x 32 causal from a rest, with the output as it was then;
           // 16 at a time 328, one to an instruction 322, between the exponentials 336, two loads in flight 328.)
           // (each row by itself, so that none depends on what its neighbours in the warp see)
           const float m_new = WIN && !(mx > m_run + kGrowth) ? m_run : fmaxf(m_run, mx);
