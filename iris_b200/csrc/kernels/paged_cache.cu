@@ -315,6 +315,31 @@ int iris_k_reserve_slots(const IrisReserveArgs* args) {
   if (page_size < 1 || (page_size & (page_size - 1)) || page_size > (1 << 30)) return refuse("page size must be a power of two");
   if (batch < 1 || batch > 0x7fffffff - 4 * kThreads || wide < 1 || wide > 0x7fffffff || capacity < 0 || capacity > 0x7fffffff || tokens < 0 || row_stride < 0)
     return refuse("sizes out of range");
+  // what is written shares no memory with anything else, but for lengths and count that are updated in place
+  struct Array {
+    const void* at;
+    int64_t n;
+  };
+  const Array written[] = {{slots, tokens}, {positions, tokens}, {lens_out, batch}, {count_out, 1}};
+  const Array read[] = {{lens, batch}, {new_lens, batch}, {free, capacity}, {count, 1}};
+  const auto meet = [](const Array& a, const Array& b) {
+    const int *x = static_cast<const int*>(a.at), *y = static_cast<const int*>(b.at);
+    return a.n > 0 && b.n > 0 && x < y + b.n && y < x + a.n;
+  };
+  const auto in_table = [&](const Array& a) {   // (an array may lie between the table's rows)
+    const int *x = static_cast<const int*>(a.at), *t = static_cast<const int*>(static_cast<const void*>(table));
+    if (!meet(a, {t, (batch - 1) * table_pitch + wide})) return false;
+    return x < t || table_pitch < 1 || (x - t) % table_pitch < wide || (x - t) % table_pitch + a.n > table_pitch;
+  };
+  for (int i = 0; i < 4; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (meet(written[i], written[j])) return refuse("outputs must not share memory");
+    for (int j = 0; j < 4; ++j) {
+      const bool in_place = (i == 2 && (j == 0 ? lens_out == lens : j == 1 && lens_out == new_lens)) || (i == 3 && j == 3 && count_out == count);
+      if (!in_place && meet(written[i], read[j])) return refuse("outputs must not share memory with inputs");
+    }
+    if (in_table(written[i]) || in_table(read[i])) return refuse("the block table must not share memory with the other arrays");
+  }
   Params p;
   memset(&p, 0, sizeof(p));
   p.lens = static_cast<const int*>(lens);

@@ -155,7 +155,8 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     ``positions`` receive, for the row of every new token, page * page_size + place in the page, and the token's position in its
     request: with ``row_stride`` 0 the requests' tokens are packed one behind the other, else request ``b`` has rows
     ``b * row_stride`` on.  Rows of no token get -1 in both.  ``lens_out`` / ``free_count_out`` (default: ``lens`` and
-    ``free_count``, in place) receive the new lengths and count.  ``new_lens`` below 0 count as 0.
+    ``free_count``, in place) receive the new lengths and count; nothing else that is written may share memory.  ``new_lens`` below 0
+    count as 0.
 
     A request for which the free pages do not last (nor for any later one that lacks a page), whose tokens do not fit its row of
     the table, or have not enough rows, gets nothing: its length stays, its rows get -1.  All tensors int32.

@@ -521,6 +521,47 @@ def test_cache_lives_through_requests():
     assert refused > 0
 
 
+@pytest.mark.parametrize("name,bad", [
+    ("slots", "positions"), ("positions", "lens"), ("slots", "free_pages"), ("lens_out", "free_pages"), ("slots", "block_table"),
+    ("count_out", "new_lens"), ("lens", "block_table")])
+def test_reserve_whose_arrays_share_memory_is_refused(name, bad):
+    """By the native entry, before it looks for a device (none needed)."""
+    memory = torch.zeros(400, dtype=torch.int32)
+    sizes = dict(lens=3, new_lens=3, block_table=24, free_pages=9, free_count=1, slots=12, positions=12, lens_out=3, count_out=1)
+    at = {n: memory.data_ptr() + 160 * i for i, n in enumerate(sizes)}
+    at[name] = at[bad] + 4 * max(0, sizes[bad] - 1 - 4 * (bad == "block_table"))
+    rc = _native.entry("iris_k_reserve_slots")(P._RESERVE.pack(
+        *(at[n] for n in ("lens", "new_lens", "block_table", "free_pages", "free_count", "slots", "positions", "lens_out", "count_out")),
+        0, 8, 4, 9, 16, 3, 12, 0))
+    lib = _native.kernels()
+    lib.iris_pages_last_error.restype = ctypes.c_char_p
+    assert rc == -1 and "share memory" in lib.iris_pages_last_error().decode()
+
+
+@gpu
+def test_reserve_lengths_over_the_new_ones_and_arrays_between_the_rows():
+    """``lens_out`` may be ``new_lens``, and a count or lengths may lie in the gaps of a strided table; ``which`` may be the lengths."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    for batch in (3, 700, 2500):
+        whole = torch.full((batch, 9), -1, dtype=torch.int32, device="cuda")
+        table, count, free = whole[:, :4], whole[1, 5:6], i32(list(range(2 * batch)))
+        count.fill_(2 * batch)
+        lens, new, rows = i32([0] * batch), i32([1 + b % 2 * 4 for b in range(batch)]), sum(1 + b % 2 * 4 for b in range(batch))
+        slots, positions = i32([0] * rows), i32([0] * rows)
+        P.reserve_slots(lens, new, table, free, count, 4, slots, positions, lens_out=new)
+        assert new.tolist() == [1 + b % 2 * 4 for b in range(batch)] and not lens.any()
+        taken = sum(1 + b % 2 for b in range(batch))
+        assert count.item() == 2 * batch - taken
+        pages = []
+        for b in range(batch):   # one page, two pages, one page, ..
+            first = 3 * (b // 2) + b % 2
+            pages.append([2 * batch - 1 - i for i in range(first, first + 1 + b % 2)])
+        assert [r[:len(p)] for r, p in zip(table.tolist(), pages)] == pages
+        P.release_slots(new, new, table, free, count, 4)
+        assert count.item() == 2 * batch and not new.any() and bool((table == -1).all())
+        assert sorted(free.tolist()) == list(range(2 * batch))
+
+
 def test_reserve_refusals():
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)   # noqa: E731
     ok = dict(lens=i32(3), new_lens=i32(3), block_table=i32(3, 4), free_pages=i32(9), free_count=i32(1), page_size=16,
