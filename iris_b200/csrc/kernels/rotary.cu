@@ -303,6 +303,9 @@ int iris_k_qk_norm_rope(const IrisQkNormRopeArgs* args) {
                           reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache);
   if (bases % 16 || (ld_in | ld_out) % 8 || ld_table % 4 || (k_cache && (page_pitch | slot_pitch | head_pitch) % 8))
     return refuse("rows must start on 16 bytes");
+  if (k_cache && (k_cache == v_cache || (pages > 1 && page_pitch < dim) || (page_size > 1 && slot_pitch < dim) ||
+                  (kv_heads > 1 && head_pitch < dim)))
+    return refuse("rows of the cache must not overlap");
   Params p;
   memset(&p, 0, sizeof(p));
   p.qkv = static_cast<const uint8_t*>(qkv);

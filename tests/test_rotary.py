@@ -283,3 +283,17 @@ def test_refusals_of_the_native_entry():
     wide = torch.zeros((6, 600), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError, match="16 bytes"):
         R.qk_norm_rope(wide[:, 4:260], wide[:, 264:520], c.pos, c.table, 2, 1, 64)
+
+
+@gpu
+def test_caches_that_overlap_are_refused():
+    """Keys and values in one place, or pages that are all one page: two tokens would write to one address."""
+    c = Case(6, 2, 1, 64, 32, torch.bfloat16)
+    before = c.k.clone()
+    with pytest.raises(RuntimeError, match="overlap"):
+        R.qk_norm_rope(c.qkv, c.out, c.pos, c.table, 2, 1, 64, k_cache=c.k, v_cache=c.k, slots=c.slots)
+    one_k, one_v = (t[:1].expand(4, -1, -1, -1) for t in (c.k, c.v))
+    with pytest.raises(RuntimeError, match="overlap"):
+        R.qk_norm_rope(c.qkv, c.out, c.pos, c.table, 2, 1, 64, k_cache=one_k, v_cache=one_v, slots=c.slots)
+    torch.cuda.synchronize()
+    assert torch.equal(torch.nan_to_num(c.k.float()), torch.nan_to_num(before.float()))
