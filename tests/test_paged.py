@@ -391,6 +391,31 @@ def test_attention_whose_waits_may_run_out():
         case.run().check()
 
 
+@gpu
+@pytest.mark.parametrize("wide", [None, 5000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_weights_far_below_the_largest_count(dtype, wide):
+    """One key takes nearly all of the weight and has values of zero; 20000 others of weight exp(-18) = 2^-25.97 each make up the
+    output.  Scores are one exact product, the exponent 26 is off by a few 2^-24 of itself and a weight by ex2's 2^-22 besides, sums
+    of n equal weights in fp32 by (n / 16 + 8) 2^-22 at worst, the weights' second 16 bits leave 2^-16; the output is rounded once."""
+    n, dominant = 20000, 77
+    case = Case([n, 3], 4, 2, 64, 16, dtype, wide=wide)
+    case.q[0].zero_()
+    case.q[0, :, 0] = 8.0
+    j = torch.arange(n, device="cuda")
+    at = case.table[0].long()[j // 16], j % 16
+    case.k[at] = 0.0
+    case.v[at] = 1.0
+    page = case.table[0, dominant // 16].item()
+    case.k[page, dominant % 16, :, 0] = 18.0
+    case.v[page, dominant % 16] = 0.0
+    case.run()
+    others = (n - 1) * math.exp(-18.0)
+    want, rel = others / (1 + others), HALF[dtype] + (n / 16 + 8) * 2.0 ** -22 + 2.0 ** -16 + 2.0 ** -17
+    assert bool(((case.out[0].double() - want).abs() <= rel * want).all()), (case.out[0, 0, 0].item(), want)
+    assert bool(((case.lse[0].double() - (18.0 + math.log1p(others))).abs() <= 2.0 ** -22 * 20 + rel * others).all())
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------
 
 def _plain_reserve(lens, new, table, free, count, page, rows, row_stride):
