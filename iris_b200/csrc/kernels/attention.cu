@@ -85,6 +85,12 @@ constexpr int kPolyEvery = 4;
 // words of bits and rows of the output written 64 bytes at a time 266,000 -> 244,700 cycles of half the case, 8 % less.)
 constexpr float kGrowth = 8.f;
 
+// fp16 with windows: weights are made 2^kLift times as large, since fp16 has no numbers below 2^-24 (8190 keys that weigh 2^-26 of
+// the largest each, 1.2e-4 of the sum, were left out of the output).  Below 2^-14 of 2^kLift they lose bits; the largest is
+// 2^(kGrowth + kLift) but for a score's rounding, half of what fp16 holds.
+template <bool F16, bool WIN>
+constexpr float kLift = F16 && WIN ? 7.f : 0.f;
+
 // Up to so many first keys make a tile of their own width instead of a whole one (2 x 8192 tokens, 32 heads, window 1024, 4 first
 // keys: with whole tiles, and with side B going through the tile that it sees nothing of, 400 us).
 constexpr int kNarrow = 32;
@@ -552,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
 #pragma unroll
           for (int i = 0; i < kNarrow; i += 2) mx = max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
           m_run = mx * p.scale_log2;
-          const float shift = m_run == -INFINITY ? 0.f : -m_run;
+          const float shift = m_run == -INFINITY ? 0.f : kLift<F16, WIN> - m_run;
           const float2 neg = make_float2(shift, shift);
           float2 sum = make_float2(0.f, 0.f);
           uint32_t pk[kNarrow / 2];
@@ -644,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
           }
         }
         // (a row that has seen scores of minus infinity only: they weigh 0, and not the NaN of their difference)
-        const float shift = m_run == -INFINITY ? 0.f : -m_run;
+        const float shift = m_run == -INFINITY ? 0.f : kLift<F16, WIN> - m_run;
         const float2 neg = make_float2(shift, shift);
         float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll

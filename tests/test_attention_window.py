@@ -129,6 +129,34 @@ def test_nan_of_a_key_reaches_the_queries_that_see_it(batch, heads):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [1, 40])                  # keys of a query tile shared out; pairs of query tiles
+@pytest.mark.parametrize("first", [0, 4000])                # among the first keys; a key of the window
+def test_weights_far_below_the_largest_count(first, heads, dtype):
+    """One key takes nearly all of a row's weight and has values of zero; 8190 others of weight exp(-18) = 2^-25.97 each make up the
+    output.  A weight is off by half a step of its 16 bits (bf16 2^-8; fp16 as much as 2^-7 where it is that far below the largest,
+    since it has a number of its own down to 2^-32 of the row's maximum), ex2, scores and sums by less than 2^-10 together."""
+    seq = 8192
+    qkv, _, out = _inputs(1, seq, heads, heads, dtype)
+    x = qkv.unflatten(1, (3, heads, 128))
+    x[:, :2] = 0.0
+    x[:, 0, :, 0] = 128 ** 0.5
+    x[:, 0, :, 1] = 0.0
+    x[:, 2] = 1.0
+    x[first, 1, :, 0] = 18.0
+    x[first, 2] = 0.0
+    A.attention_window_fwd(qkv, out, 1, seq, heads, window=5000, sinks=1)
+    score = float(x[0, 0, 0, 0].double()) * 18.0 / 128 ** 0.5           # (the root of 128 is rounded too)
+    for row in (4500, 8191):
+        n = min(row + 1, 5000) + (1 if row >= 5000 else 0)              # keys that the row sees
+        others = (n - 1) * torch.tensor(-score, dtype=torch.float64).exp().item()
+        want = others / (1 + others)
+        rel = HALF[dtype] + 2.0 ** -7 + 2.0 ** -10
+        got = out[row].double()
+        assert bool(((got - want).abs() <= rel * want).all()), (row, got[0].item(), want)
+
+
+@gpu
 def test_in_a_graph_and_on_another_stream():
     qkv, _, out = _inputs(2, 300, 4, 2, torch.bfloat16)
     st = torch.cuda.Stream()
