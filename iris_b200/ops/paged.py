@@ -19,7 +19,7 @@ from .. import _native
 
 _DT = {torch.bfloat16: 0, torch.float16: 1}
 _P, _L, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
-_ATTENTION, _RESERVE = struct.Struct("@34qd"), struct.Struct("@17q")
+_ATTENTION, _RESERVE, _LIMITS = struct.Struct("@34qd"), struct.Struct("@17q"), struct.Struct("@q")
 _RELEASE = [_P, _P, _P, _L, _L, _P, _L, _P, _I, _L, _P]
 
 
@@ -147,7 +147,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                   free_count: torch.Tensor, page_size: int, slots: torch.Tensor, positions: torch.Tensor, *,
                   row_stride: int = 0, lens_out: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None,
-                  stream=None) -> None:
+                  max_len: Optional[int] = None, stream=None) -> None:
     """Takes pages for ``new_lens[b]`` further tokens of every request ``b``, and says where those tokens go.
 
     Request ``b`` holds ``lens[b]`` tokens in pages ``block_table[b, :]``.  In the requests' order, each takes the pages it lacks
@@ -159,7 +159,8 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     count as 0.
 
     A request for which the free pages do not last (nor for any later one that lacks a page), whose tokens do not fit its row of
-    the table, or have not enough rows, gets nothing: its length stays, its rows get -1.  All tensors int32.
+    the table, or have not enough rows, or which would hold more than ``max_len`` tokens, gets nothing: its length stays, its rows
+    get -1.  All tensors int32.
     """
     # (every look at a tensor costs the host 0.06 to 0.12 us, on a path of 7: sizes in bytes and straight chains, not shapes and loops)
     i32 = torch.int32
@@ -179,6 +180,8 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
         raise ValueError("page_size must be a power of two")
     if row_stride < 0 or tokens < batch * row_stride:
         raise ValueError(f"{tokens} rows do not hold {batch} requests of {row_stride}")
+    if max_len is not None and max_len < 0:
+        raise ValueError("max_len must not be negative")
     device = lens.get_device()
     if not (new_lens.get_device() == device and block_table.get_device() == device and free_pages.get_device() == device and
             free_count.get_device() == device and slots.get_device() == device and positions.get_device() == device and
@@ -189,12 +192,17 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     if device != _native.current_device(device):
         with torch.cuda.device(device):
             return reserve_slots(lens, new_lens, block_table, free_pages, free_count, page_size, slots, positions,
-                                 row_stride=row_stride, lens_out=lens_out, free_count_out=free_count_out, stream=stream)
-    rc = _native.entry("iris_k_reserve_slots")(_RESERVE.pack(
+                                 row_stride=row_stride, lens_out=lens_out, free_count_out=free_count_out, max_len=max_len,
+                                 stream=stream)
+    args = _RESERVE.pack(
         lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
         slots.data_ptr(), positions.data_ptr(), lens_out.data_ptr(), free_count_out.data_ptr(),
         torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, pitch, table_shape[1], free_pages.nbytes // 4,
-        page_size, batch, tokens, row_stride))
+        page_size, batch, tokens, row_stride)
+    if max_len is None:
+        rc = _native.entry("iris_k_reserve_slots")(args)
+    else:
+        rc = _native.entry("iris_k_reserve_slots_within")(args + _LIMITS.pack(max_len))
     if rc:
         _raise("reserve_slots", rc)
 
@@ -240,7 +248,8 @@ def _raise(what: str, rc: int):
 
 class PagedCache:
     """Keys and values of up to ``max_batch`` requests in pages that all layers share out alike: page ``i`` of the list is page
-    ``i`` in every layer.  ``k(layer)`` / ``v(layer)``: ``[pages, page_size, kv_heads, head_dim]``."""
+    ``i`` in every layer.  ``k(layer)`` / ``v(layer)``: ``[pages, page_size, kv_heads, head_dim]``.  No request gets more than
+    ``max_len`` tokens, whatever room its last page has."""
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, max_batch: int, max_len: int,
                  dtype: torch.dtype = torch.bfloat16, device=None):
@@ -265,9 +274,9 @@ class PagedCache:
 
     def reserve(self, new_lens: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, row_stride: int = 0,
                 stream=None) -> None:
-        """:func:`reserve_slots` on this cache's requests, lengths and free pages updated in place."""
+        """:func:`reserve_slots` on this cache's requests, up to ``max_len`` tokens each; lengths and free pages are updated in place."""
         reserve_slots(self.lens, new_lens, self.block_table, self.free_pages, self.free_count, self.page_size, slots, positions,
-                      row_stride=row_stride, stream=stream)
+                      row_stride=row_stride, max_len=self.max_len, stream=stream)
 
     def release(self, which: torch.Tensor, stream=None) -> None:
         """:func:`release_slots` on this cache's requests."""

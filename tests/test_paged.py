@@ -587,6 +587,33 @@ def test_reserve_lengths_over_the_new_ones_and_arrays_between_the_rows():
         assert sorted(free.tolist()) == list(range(2 * batch))
 
 
+@gpu
+@pytest.mark.parametrize("row_stride", [0, 40])
+def test_reserve_stops_at_the_longest_length(row_stride):
+    """``max_len`` binds although the last page has room for more, and a request beyond it is in nobody's way."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    cache = P.PagedCache(1, 20, 16, 1, 64, 3, 35, device="cuda")
+    slots, positions = i32([0] * 120), i32([0] * 120)
+    cache.reserve(i32([35, 34, 36]), slots, positions, row_stride=row_stride)
+    assert cache.lens.tolist() == [35, 34, 0] and cache.free_count.item() == 14
+    cache.reserve(i32([1, 1, 35]), slots, positions, row_stride=row_stride)
+    assert cache.lens.tolist() == [35, 35, 35] and cache.free_count.item() == 11
+    first = row_stride or 1
+    assert positions[0].item() == -1 and slots[0].item() == -1 and positions[first].item() == 34
+    cache.reserve(i32([1, 0, 2]), slots, positions, row_stride=row_stride)
+    assert cache.lens.tolist() == [35, 35, 35] and bool((positions == -1).all())
+    table, lens, count = i32([[-1] * 4]), i32([0]), i32([9])
+    for limit, want in ((3, 0), (4, 4), (None, 8)):
+        P.reserve_slots(lens, i32([4]), table, i32(list(range(9))), count, 4, slots, positions, max_len=limit)
+        assert lens.item() == want
+
+
+def test_reserve_refuses_a_negative_longest_length():
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)   # noqa: E731
+    with pytest.raises(ValueError, match="max_len"):
+        P.reserve_slots(i32(3), i32(3), i32(3, 4), i32(9), i32(1), 16, i32(12), i32(12), max_len=-1)
+
+
 def test_reserve_refusals():
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)   # noqa: E731
     ok = dict(lens=i32(3), new_lens=i32(3), block_table=i32(3, 4), free_pages=i32(9), free_count=i32(1), page_size=16,

@@ -109,6 +109,31 @@ def test_prompts_then_single_tokens(kind, world, batch, seq, steps, graph):
     ranks[0].close()
 
 
+def _forward(model, rows, cache, new):
+    shards = [rows.clone()]
+    model.forward(shards, cache=cache, new_lens=torch.tensor(new, dtype=torch.int32, device="cuda"))
+    model.check()
+    return shards[0]
+
+
+def test_a_request_stops_at_the_caches_longest_length():
+    """Angles for 71 positions, a cache of requests of up to 71 tokens, pages of 16: the 72nd token is not taken, and its request
+    answers as before, whoever had the rest of its page earlier."""
+    more = dict(SIZES, **KINDS["grouped"], positions=71)
+    ctx = iris.iris(192 << 20)
+    prefill = TPDecoder(ctx, TPConfig(batch=2, seq=70, **more))
+    decode = TPDecoder(ctx, TPConfig(batch=2, seq=1, **more), weights=prefill)
+    cache = prefill.make_cache(10, 16, 2, 71)
+    x = _inputs(2, 71)
+    want = reference_forward(x.view(142, -1), TPConfig(batch=2, seq=71, **more)).view(2, 71, -1)
+    _forward(prefill, x[:, :70].reshape(140, -1), cache, [70, 70])
+    _near(_forward(decode, x[:, 70].contiguous(), cache, [1, 1]), want[:, 70])
+    for _ in range(3):
+        _forward(decode, x[:, 70].contiguous(), cache, [1, 1])              # (and check() finds nothing recorded)
+        assert cache[0].lens.tolist() == [71, 71] and decode.cache_positions.tolist() == [-1, -1]
+    prefill.close(), decode.close(), ctx.close()
+
+
 def test_refusals():
     ctx = iris.iris(192 << 20)
     cfg = TPConfig(batch=2, seq=64, **SIZES, **KINDS["grouped"])
