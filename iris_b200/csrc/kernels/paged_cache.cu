@@ -6,10 +6,10 @@
 //   need_b = ceil((lens[b] + new_lens[b]) / page_size) - ceil(lens[b] / page_size),   first_b = need_0 + .. + need_{b-1}
 //   block_table[b, held_b + i] = free[count - 1 - (first_b + i)],   0 <= i < need_b
 //
-// as long as they last: a request with first_b + need_b > count, too long for its row of the table or for the caller's limit, or
-// with more tokens than rows were left for them, gets nothing.  Every new token gets its position and its slot,
-// page * page_size + position % page_size.  release: pages of chosen requests go back to
-// the end of the list.  No counterpart in the reference.
+// as long as they last: a request with first_b + need_b > count, too long for its row of the table or for the caller's limit, with
+// more tokens than rows were left for them, or that holds tokens although only empty ones are asked for, gets nothing.  Every new
+// token gets its position and its slot, page * page_size + position % page_size.  release: pages of chosen requests go back to the
+// end of the list.  No counterpart in the reference.
 //
 // A call's time is its launch and a few passes through memory in a row (lengths, prefix sums, free list or table, output), so
 // it is one launch: every CTA of one cluster makes the prefix sums for itself, in chunks of a few requests per thread, and the
@@ -44,6 +44,7 @@ struct Params {
   int64_t table_pitch, tokens, row_stride;
   int64_t most;              // tokens of a request
   int batch, wide, page_shift, capacity;
+  int most_held;             // that a request may hold already
 };
 
 // A chunk of requests, PER a thread, and the sums over them, for every thread to search.  One a thread up to 512 requests, else
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__
         if (granted[u]) need[u] = min(held_of(len[u]), p.wide);
       } else {
         const int64_t end = (int64_t)len[u] + more[u];
-        granted[u] = granted[u] && end <= p.most &&
+        granted[u] = granted[u] && end <= p.most && (len[u] <= p.most_held || more[u] == 0) &&
                      (p.row_stride ? more[u] <= p.row_stride : tokens + t_upto[u] <= p.tokens);
         if (granted[u]) need[u] = ((end + mask) >> p.page_shift) - held_of(len[u]);
       }
@@ -308,7 +309,7 @@ struct IrisReserveArgs {
   int64_t table_pitch, wide, capacity, page_size, batch, tokens, row_stride;
 };
 
-static int reserve(const IrisReserveArgs* args, int64_t max_len) {
+static int reserve(const IrisReserveArgs* args, int64_t max_len, bool fresh) {
   using namespace iris::pages;
   g_err[0] = 0;
   const auto [lens, new_lens, table, free, count, slots, positions, lens_out, count_out, stream, table_pitch, wide, capacity,
@@ -357,17 +358,19 @@ static int reserve(const IrisReserveArgs* args, int64_t max_len) {
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   p.most = wide << p.page_shift < 0x7fffffff ? wide << p.page_shift : 0x7fffffff;
   if (max_len < p.most) p.most = max_len;
+  p.most_held = fresh ? 0 : 0x7fffffff;
   return launch<false>(p, tokens, stream);
 }
 
-int iris_k_reserve_slots(const IrisReserveArgs* args) { return reserve(args, INT64_MAX); }
+int iris_k_reserve_slots(const IrisReserveArgs* args) { return reserve(args, INT64_MAX, false); }
 
-// The same with a limit to the tokens of a request, below what its row of the table has room for.
+// The same with a limit to the tokens of a request, below what its row of the table has room for; fresh: not 0 for requests that
+// hold nothing alone.
 struct IrisReserveWithinArgs {
   IrisReserveArgs all;
-  int64_t max_len;
+  int64_t max_len, fresh;
 };
-int iris_k_reserve_slots_within(const IrisReserveWithinArgs* args) { return reserve(&args->all, args->max_len); }
+int iris_k_reserve_slots_within(const IrisReserveWithinArgs* args) { return reserve(&args->all, args->max_len, args->fresh != 0); }
 
 // which [batch]: not 0 for the requests whose pages go back; their length becomes 0 and their entries of the table -1.
 int iris_k_release_slots(void* lens, const void* which, void* table, int64_t table_pitch, int64_t wide, void* free,

@@ -222,10 +222,10 @@ class TPDecoder:
 
         ``cache``: one paged cache per local rank (:meth:`make_cache`), of ``batch`` requests.  ``new_lens`` int32 [batch] says how
         many of each request's ``seq`` rows are tokens (the first ones); the cache takes pages for them and their keys and
-        values.  With ``seq`` rows and more than one, these are whole prompts of requests that hold nothing yet; with ``seq=1``
-        the newest token of each request attends over its pages (with peers, ``batch`` is a multiple of 128 per rank, as the rows of
-        every fused all-gather -> GEMM).  Rows of no token, and of requests that got no pages (their
-        length in the cache stays), give no meaningful output."""
+        values.  With ``seq`` rows and more than one, these are whole prompts, which attend over their own rows alone, so that a
+        request that holds tokens already gets nothing; with ``seq=1`` the newest token of each request attends over its pages
+        (with peers, ``batch`` is a multiple of 128 per rank, as the rows of every fused all-gather -> GEMM).  Rows of no token,
+        and of requests that got nothing (:func:`iris_b200.ops.paged.reserve_slots`; their length in the cache stays), give no meaningful output."""
         cfg, nl = self.cfg, len(self.ctxs)
         n = 0
         tick = timers if timers is not None else (lambda name: None)
@@ -239,7 +239,7 @@ class TPDecoder:
                 raise ValueError("the cache holds more positions than there are angles for (TPConfig.positions)")
             tick("reserve")
             for l in range(nl):
-                cache[l].reserve(new_lens, self.slots, self.cache_positions, row_stride=cfg.seq)
+                cache[l].reserve(new_lens, self.slots, self.cache_positions, row_stride=cfg.seq, fresh=cfg.seq > 1)
             n += nl
         pending = None   # output of the previous layer's down projection, not yet added to the residual stream
         for layer, ops in enumerate(self.layers):

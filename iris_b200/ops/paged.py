@@ -19,7 +19,7 @@ from .. import _native
 
 _DT = {torch.bfloat16: 0, torch.float16: 1}
 _P, _L, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
-_ATTENTION, _RESERVE, _LIMITS = struct.Struct("@34qd"), struct.Struct("@17q"), struct.Struct("@q")
+_ATTENTION, _RESERVE, _LIMITS = struct.Struct("@34qd"), struct.Struct("@17q"), struct.Struct("@2q")
 _RELEASE = [_P, _P, _P, _L, _L, _P, _L, _P, _I, _L, _P]
 
 
@@ -147,7 +147,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                   free_count: torch.Tensor, page_size: int, slots: torch.Tensor, positions: torch.Tensor, *,
                   row_stride: int = 0, lens_out: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None,
-                  max_len: Optional[int] = None, stream=None) -> None:
+                  max_len: Optional[int] = None, fresh: bool = False, stream=None) -> None:
     """Takes pages for ``new_lens[b]`` further tokens of every request ``b``, and says where those tokens go.
 
     Request ``b`` holds ``lens[b]`` tokens in pages ``block_table[b, :]``.  In the requests' order, each takes the pages it lacks
@@ -160,7 +160,7 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
 
     A request for which the free pages do not last (nor for any later one that lacks a page), whose tokens do not fit its row of
     the table, or have not enough rows, or which would hold more than ``max_len`` tokens, gets nothing: its length stays, its rows
-    get -1.  All tensors int32.
+    get -1.  With ``fresh`` neither does a request that holds tokens already.  All tensors int32.
     """
     # (every look at a tensor costs the host 0.06 to 0.12 us, on a path of 7: sizes in bytes and straight chains, not shapes and loops)
     i32 = torch.int32
@@ -193,16 +193,16 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
         with torch.cuda.device(device):
             return reserve_slots(lens, new_lens, block_table, free_pages, free_count, page_size, slots, positions,
                                  row_stride=row_stride, lens_out=lens_out, free_count_out=free_count_out, max_len=max_len,
-                                 stream=stream)
+                                 fresh=fresh, stream=stream)
     args = _RESERVE.pack(
         lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
         slots.data_ptr(), positions.data_ptr(), lens_out.data_ptr(), free_count_out.data_ptr(),
         torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, pitch, table_shape[1], free_pages.nbytes // 4,
         page_size, batch, tokens, row_stride)
-    if max_len is None:
+    if max_len is None and not fresh:
         rc = _native.entry("iris_k_reserve_slots")(args)
     else:
-        rc = _native.entry("iris_k_reserve_slots_within")(args + _LIMITS.pack(max_len))
+        rc = _native.entry("iris_k_reserve_slots_within")(args + _LIMITS.pack(0x7fffffff if max_len is None else max_len, fresh))
     if rc:
         _raise("reserve_slots", rc)
 
@@ -273,10 +273,10 @@ class PagedCache:
         return self.data[layer, 1]
 
     def reserve(self, new_lens: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, row_stride: int = 0,
-                stream=None) -> None:
+                fresh: bool = False, stream=None) -> None:
         """:func:`reserve_slots` on this cache's requests, up to ``max_len`` tokens each; lengths and free pages are updated in place."""
         reserve_slots(self.lens, new_lens, self.block_table, self.free_pages, self.free_count, self.page_size, slots, positions,
-                      row_stride=row_stride, max_len=self.max_len, stream=stream)
+                      row_stride=row_stride, max_len=self.max_len, fresh=fresh, stream=stream)
 
     def release(self, which: torch.Tensor, stream=None) -> None:
         """:func:`release_slots` on this cache's requests."""

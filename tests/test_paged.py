@@ -614,6 +614,27 @@ def test_reserve_refuses_a_negative_longest_length():
         P.reserve_slots(i32(3), i32(3), i32(3, 4), i32(9), i32(1), 16, i32(12), i32(12), max_len=-1)
 
 
+@gpu
+@pytest.mark.parametrize("batch", [4, 700])
+def test_reserve_for_requests_that_hold_nothing(batch):
+    """``fresh``: a request that holds tokens gets nothing, takes no page, and is in nobody's way."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    held = [b % 2 * 5 for b in range(batch)]
+    table = [[b, -1] if held[b] else [-1, -1] for b in range(batch)]
+    lens, table_t, count = i32(held), i32(table), i32([batch])
+    slots, positions = i32([7] * 6 * batch), i32([7] * 6 * batch)
+    new = [6 - b % 4 // 2 * 6 for b in range(batch)]            # 6, 6, 0, 0, ..
+    P.reserve_slots(lens, i32(new), table_t, i32(list(range(batch, 2 * batch))), count, 8, slots, positions, row_stride=6, fresh=True)
+    given = [b for b in range(batch) if new[b] and not held[b]]
+    assert lens.tolist() == [6 if b in given else held[b] for b in range(batch)]
+    assert count.item() == batch - len(given)
+    pages = {b: 2 * batch - 1 - i for i, b in enumerate(given)}
+    assert table_t.tolist() == [[pages[b], -1] if b in pages else table[b] for b in range(batch)]
+    want = [[pages[b] * 8 + j if b in pages else -1 for j in range(6)] for b in range(batch)]
+    assert slots.view(batch, 6).tolist() == want
+    assert positions.view(batch, 6).tolist() == [list(range(6)) if b in pages else [-1] * 6 for b in range(batch)]
+
+
 def test_reserve_refusals():
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)   # noqa: E731
     ok = dict(lens=i32(3), new_lens=i32(3), block_table=i32(3, 4), free_pages=i32(9), free_count=i32(1), page_size=16,

@@ -134,6 +134,26 @@ def test_a_request_stops_at_the_caches_longest_length():
     prefill.close(), decode.close(), ctx.close()
 
 
+@pytest.mark.parametrize("kind", ["plain", "grouped", "window"])
+def test_a_prompt_for_a_request_that_holds_tokens_gets_nothing(kind):
+    """A prompt attends over its own rows alone, so a request that goes on takes single tokens; others in the call are served."""
+    more = dict(SIZES, **KINDS[kind], positions=64)
+    ctx = iris.iris(192 << 20)
+    prefill = TPDecoder(ctx, TPConfig(batch=2, seq=40, **more))
+    decode = TPDecoder(ctx, TPConfig(batch=2, seq=1, **more), weights=prefill)
+    cache = prefill.make_cache(16, 16, 2, 64)
+    x = _inputs(2, 40)
+    want = reference_forward(x.view(80, -1), TPConfig(batch=2, seq=40, **more)).view(2, 40, -1)
+    got = _forward(prefill, x.view(80, -1), cache, [12, 0]).view(2, 40, -1)
+    _near(got[0, :12], want[0, :12])
+    free = cache[0].free_count.item()
+    got = _forward(prefill, x.view(80, -1), cache, [9, 30]).view(2, 40, -1)
+    assert cache[0].lens.tolist() == [12, 30] and cache[0].free_count.item() == free - 2
+    _near(got[1, :30], want[1, :30])
+    _near(_forward(decode, x[torch.arange(2), [12, 30]], cache, [1, 1]), want[torch.arange(2), [12, 30]])
+    prefill.close(), decode.close(), ctx.close()
+
+
 def test_refusals():
     ctx = iris.iris(192 << 20)
     cfg = TPConfig(batch=2, seq=64, **SIZES, **KINDS["grouped"])
