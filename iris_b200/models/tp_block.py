@@ -225,7 +225,7 @@ class TPDecoder:
         values.  With ``seq`` rows and more than one, these are whole prompts, which attend over their own rows alone, so that a
         request that holds tokens already gets nothing; with ``seq=1`` the newest token of each request attends over its pages
         (with peers, ``batch`` is a multiple of 128 per rank, as the rows of every fused all-gather -> GEMM).  Rows of no token,
-        and of requests that got nothing (:func:`iris_b200.ops.paged.reserve_slots`; their length in the cache stays), give no meaningful output."""
+        and of requests that got nothing (:func:`iris_b200.ops.paged.reserve_slots`; their length in the cache stays) may hold anything and give no meaningful output."""
         cfg, nl = self.cfg, len(self.ctxs)
         n = 0
         tick = timers if timers is not None else (lambda name: None)
@@ -241,6 +241,11 @@ class TPDecoder:
             for l in range(nl):
                 cache[l].reserve(new_lens, self.slots, self.cache_positions, row_stride=cfg.seq, fresh=cfg.seq > 1)
             n += nl
+            if cfg.seq > 1:
+                # A prompt's padding may hold anything, and infinity or NaN would reach the tokens that share its tile of keys with
+                # a weight of zero (single tokens share no tile): zeros stay finite through all layers.
+                for l in range(nl):
+                    x_shards[l].masked_fill_((self.cache_positions[self.rows(l)] < 0)[:, None], 0)
         pending = None   # output of the previous layer's down projection, not yet added to the residual stream
         for layer, ops in enumerate(self.layers):
             tick("norm")

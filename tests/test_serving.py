@@ -154,6 +154,33 @@ def test_a_prompt_for_a_request_that_holds_tokens_gets_nothing(kind):
     prefill.close(), decode.close(), ctx.close()
 
 
+@pytest.mark.parametrize("kind,seq,attention", [
+    ("plain", 128, "iris"), ("plain", 96, "iris"), ("grouped", 96, "iris"), ("window", 128, "iris"), ("plain", 128, "sdpa")])
+@pytest.mark.parametrize("rubbish", [float("nan"), float("inf"), 3.0e38])
+def test_rows_of_no_token_reach_nothing(kind, seq, attention, rubbish):
+    """A prompt's padding may hold anything, NaN and infinity too."""
+    more = dict(SIZES, **KINDS[kind], positions=seq)
+    cfg = TPConfig(batch=3, seq=seq, **more)
+    ctx = iris.iris(192 << 20)
+    prefill = TPDecoder(ctx, cfg, attention=attention)
+    decode = TPDecoder(ctx, TPConfig(batch=3, seq=1, **more), weights=prefill)
+    cache = prefill.make_cache(3 * 8, 16, 3, seq)
+    x, lens = _inputs(3, seq), [seq - 30, 1, 0]
+    want = reference_forward(x.view(3 * seq, -1), cfg).view(3, seq, -1)
+    padded = x.clone()
+    for b, n in enumerate(lens):
+        padded[b, n:] = rubbish
+    got = _forward(prefill, padded.view(3 * seq, -1), cache, lens).view(3, seq, -1)
+    for b, n in enumerate(lens):
+        if n:
+            _near(got[b, :n], want[b, :n])
+    step = x[torch.arange(3), lens].clone()
+    step[1] = rubbish                                                       # no token either
+    got = _forward(decode, step, cache, [1, 0, 1])
+    _near(got[[0, 2]], want[torch.arange(3), lens][[0, 2]])
+    prefill.close(), decode.close(), ctx.close()
+
+
 def test_refusals():
     ctx = iris.iris(192 << 20)
     cfg = TPConfig(batch=2, seq=64, **SIZES, **KINDS["grouped"])
