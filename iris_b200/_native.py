@@ -141,5 +141,13 @@ def current_device(expected: int) -> int:
     return torch._C._cuda_getDevice()
 
 
+def status_block(t, device: int) -> int:
+    """Address of a status block (an ``Iris`` context's, or memory like it) on CUDA device ``device``, which kernels write a record
+    of 32 bytes into."""
+    if t.get_device() != device or t.nbytes < 32 or not t.is_contiguous() or t.data_ptr() % 8:
+        raise ValueError("status must be at least 32 contiguous bytes, on 8 of them, on the device of the other tensors")
+    return t.data_ptr()
+
+
 def kernels_available() -> bool:
     return lib_path("kernels").exists()

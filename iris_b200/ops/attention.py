@@ -80,8 +80,9 @@ def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: 
     if window < 1 or sinks < 0:
         raise ValueError("a window has at least one key, the number of first keys is not negative")
     device = qkv.get_device()
-    if out.get_device() != device or (status is not None and status.get_device() != device):
+    if out.get_device() != device:
         raise ValueError("all tensors must be on one device")
+    status_ptr = 0 if status is None else _native.status_block(status, device)
     rows = batch * seq
     if rows == 0:
         return out
@@ -94,7 +95,7 @@ def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: 
             return attention_window_fwd(qkv, out, batch, seq, heads, kv_heads, window=window, sinks=sinks, status=status,
                                         timeout_ms=timeout_ms, stream=stream)
     rc = _native.entry("iris_k_attention_window_fwd")(_WINDOW_ARGS.pack(
-        qkv_ptr, out_ptr, 0 if status is None else status.data_ptr(),
+        qkv_ptr, out_ptr, status_ptr,
         torch._C._cuda_getCurrentRawStream(device) if stream is None else stream, ld_in, ld_out, batch, seq, heads, kv_heads,
         window, sinks, _DT[dtype], int(timeout_ms * 1e6)))
     if rc != 0:

@@ -106,11 +106,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             raise ValueError(f"lse must be fp32 [{batch}, {heads}], with rows that are contiguous and do not overlap")
         same = same and lse.get_device() == device
         lse_ptr = lse.data_ptr()
-    if status is not None:
-        same = same and status.get_device() == device
-        status_ptr = status.data_ptr()
     if not same:
         raise ValueError("all tensors must be on one device")
+    if status is not None:
+        status_ptr = _native.status_block(status, device)
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
     if batch == 0:

@@ -126,11 +126,10 @@ def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, 
     elif out_width != width:
         raise ValueError("an output of queries alone needs a cache for the keys and values")
     status_ptr = 0
-    if status is not None:
-        same = same and status.get_device() == device
-        status_ptr = status.data_ptr()
     if not same:
         raise ValueError("all tensors must be on one device")
+    if status is not None:
+        status_ptr = _native.status_block(status, device)
     if tokens == 0:
         return out
     qkv_ptr, out_ptr = qkv.data_ptr(), out.data_ptr()

@@ -251,6 +251,17 @@ def test_refusals():
             A.attention_window_fwd(**{**ok, "qkv": wide[:, :1024], "out": fine})
 
 
+def test_a_status_that_is_no_block_is_refused():
+    """A record has 32 bytes; what is smaller, strided or misaligned would be written past."""
+    qkv, _, out = _inputs(2, 10, 4, 2, torch.bfloat16, device="cpu")
+    memory = torch.zeros(17, dtype=torch.int32)
+    for bad in (memory[:1], memory[:7], memory[1:], memory[::2][:8]):
+        with pytest.raises(ValueError, match="status"):
+            A.attention_window_fwd(qkv, out, 2, 10, 4, 2, window=4, status=bad)
+    with pytest.raises(ValueError, match="CUDA device"):
+        A.attention_window_fwd(qkv, out, 2, 10, 4, 2, window=4, status=memory[:8])
+
+
 @gpu
 def test_refusals_of_the_native_entry():
     wide = torch.zeros((20, 2000), dtype=torch.bfloat16, device="cuda")

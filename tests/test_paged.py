@@ -325,6 +325,17 @@ def test_attention_refusals():
         call()
 
 
+def test_attention_refuses_a_status_that_is_no_block():
+    """A record has 32 bytes; what is smaller, strided or misaligned would be written past."""
+    c = Case([40, 3], 4, 2, 64, 16, torch.bfloat16, device="cpu")
+    memory = torch.zeros(17, dtype=torch.int32)
+    for bad in (memory[:1], memory[:7], memory[1:], memory[::2][:8]):
+        with pytest.raises(ValueError, match="status"):
+            P.paged_attention(c.q, c.k, c.v, c.table, c.len_t, c.out, status=bad)
+    with pytest.raises(ValueError, match="CUDA device"):
+        P.paged_attention(c.q, c.k, c.v, c.table, c.len_t, c.out, status=memory[:8])
+
+
 @gpu
 def test_attention_refusals_of_the_native_entry():
     c = Case([40, 3], 4, 2, 64, 16, torch.bfloat16)

@@ -275,6 +275,17 @@ def test_refusals():
             R.rotary_table(**{**dict(positions=4, rotary_dim=32), **bad})
 
 
+def test_a_status_that_is_no_block_is_refused():
+    """A record has 32 bytes; what is smaller, strided or misaligned would be written past."""
+    c = Case(3, 2, 1, 32, 16, torch.bfloat16, device="cpu")
+    memory = torch.zeros(17, dtype=torch.int32)
+    for bad in (memory[:1], memory[:7], memory[1:], memory[::2][:8]):
+        with pytest.raises(ValueError, match="status"):
+            R.qk_norm_rope(c.qkv, c.out, c.pos, c.table, 2, 1, 32, status=bad, **c.kw())
+    with pytest.raises(ValueError, match="CUDA device"):
+        R.qk_norm_rope(c.qkv, c.out, c.pos, c.table, 2, 1, 32, status=memory[:8], **c.kw())
+
+
 @gpu
 def test_refusals_of_the_native_entry():
     c = Case(6, 2, 1, 64, 32, torch.bfloat16)
