@@ -1,9 +1,11 @@
 """Head norms, rotation and cache writes against the formulas in 64 bits, the table of angles, and the refusals."""
+import ctypes
 import math
 
 import pytest
 import torch
 
+from iris_b200 import _native
 from iris_b200.ops import rotary as R
 
 gpu = pytest.mark.gpu
@@ -294,6 +296,57 @@ def test_refusals_of_the_native_entry():
     wide = torch.zeros((6, 600), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError, match="16 bytes"):
         R.qk_norm_rope(wide[:, 4:260], wide[:, 264:520], c.pos, c.table, 2, 1, 64)
+
+
+def _native_answer(qkv, out, heads, kv, dim, positions, slots, k, v, table, weights=(0, 0)):
+    """What the native entry says to a call; those it does not refuse find no device here.  (Tests without a device alone.)"""
+    out_heads = heads + kv if out.data_ptr() == qkv.data_ptr() and out.shape == qkv.shape else out.shape[1] // dim
+    pages, size = k.shape[:2]
+    lib = _native.kernels()
+    rc = _native.entry("iris_k_qk_norm_rope")(R._ARGS.pack(
+        qkv.data_ptr(), out.data_ptr(), positions.data_ptr(), table.data_ptr(), *weights, k.data_ptr(), v.data_ptr(),
+        slots.data_ptr(), 0, 0, qkv.stride(0), out.stride(0), table.stride(0), *k.stride()[:3], out_heads, *table.shape, 0,
+        pages, size, qkv.shape[0], heads, kv, dim, 0, 1e-6))
+    assert rc < 0
+    lib.iris_rotary_last_error.restype = ctypes.c_char_p
+    return lib.iris_rotary_last_error().decode()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="calls that are not refused must find no device")
+def test_memory_that_tokens_or_arguments_share_is_refused():
+    """Rows of the cache that meet, whatever pitch they meet by; keys over a part of the values; a cache in qkv or out; positions,
+    slots, weights or the table under what is written.  Column blocks side by side, and pages of keys and values in turn, are fine."""
+    tokens, heads, kv, dim, pages, size = 6, 2, 2, 64, 3, 4
+    big = torch.zeros(1 << 16, dtype=torch.bfloat16)
+    qkv, out = big[:6 * 400].view(6, 400)[:, :384], big[4096:4096 + 6 * 384].view(6, 384)
+    cache = big[8192:8192 + 2 * pages * size * kv * dim].view(2, pages, size, kv, dim)
+    positions, slots = torch.zeros(6, dtype=torch.int32), torch.arange(6, dtype=torch.int32)
+    table = torch.zeros(10, 32)
+    ok = dict(qkv=qkv, out=out, heads=heads, kv=kv, dim=dim, positions=positions, slots=slots, k=cache[0], v=cache[1], table=table)
+
+    def at(offset, pitches, shape=(pages, size, kv, dim)):
+        return torch.as_strided(big, shape, (*pitches, 1), offset)
+    turns, columns = big[16384:16384 + 2 * pages * size * kv * dim], big[24576:24576 + 2 * pages * size * kv * dim]
+    turns, columns = turns.view(pages, 2, size, kv, dim), columns.view(pages, size, kv, 2 * dim)
+    by_head = big[8192:8192 + 2 * pages * size * kv * dim].view(2, pages, kv, size, dim).transpose(2, 3)
+    for fine in (dict(), dict(k=turns[:, 0], v=turns[:, 1]), dict(k=columns[..., :dim], v=columns[..., dim:]), dict(out=qkv),
+                 dict(out=qkv[:, :128]), dict(k=by_head[0], v=by_head[1]), dict(positions=big[392:404].view(torch.int32)[:6]),
+                 dict(k=at(30000, (4096, 64, 512)), v=at(30000 + 256, (4096, 64, 512)))):
+        assert "launch" in _native_answer(**{**ok, **fine}), fine
+    ints = lambda o: big[o:o + 12].view(torch.int32)   # noqa: E731
+    for what, bad in (
+            ("overlap", dict(k=at(30000, (1024, 64, 64)), v=at(50000, (1024, 64, 64)))),       # slots and heads at one pitch
+            ("overlap", dict(k=at(30000, (64, 64, 512)), v=at(50000, (64, 64, 512)))),         # pages and slots
+            ("overlap", dict(k=at(30000, (256, 128, 64)), v=at(50000, (256, 128, 64)))),       # a page shorter than its slots
+            ("overlap", dict(v=cache[0])), ("overlap", dict(k=at(30000, (1024, 256, 128)), v=at(30064 - 8, (1024, 256, 128)))),
+            ("overlap", dict(v=at(8192 + 512, (512, 128, 64)))),                                # keys' page 1 on
+            ("overlap", dict(out=out[:1].expand(6, -1))),
+            ("qkv or out", dict(k=at(0, (512, 128, 64)), v=at(40000, (512, 128, 64)))),
+            ("qkv or out", dict(k=at(40000, (512, 128, 64)), v=at(4096, (512, 128, 64)))),
+            ("positions", dict(positions=ints(4096 + 8))), ("positions", dict(slots=ints(8192 + 64))),
+            ("positions", dict(positions=ints(8192 + 1536 + 8))), ("positions", dict(weights=(out.data_ptr() + 128, 0))),
+            ("positions", dict(table=big[4096:4096 + 640].view(torch.float32).view(10, 32)))):
+        assert what in _native_answer(**{**ok, **bad}), (what, bad)
 
 
 @gpu
