@@ -72,7 +72,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     one counts as 0.  Keys and values behind a sequence's last key, or out of its window, reach nothing, NaN or not; a seen value
     that is infinite makes its component infinite or NaN.  A key whose table entry is no page is left out and recorded in ``status``
     (an ``Iris`` context's status block) if that is given, as is a bounded wait of the kernel that ran out (the output then means
-    nothing).  ``out`` may be ``q`` itself, and otherwise shares no memory with it or the cache.  ``longest``: what the lengths are
+    nothing).  ``out`` may be ``q`` itself; otherwise what is written shares no memory with anything else.  ``longest``: what the lengths are
     expected not to exceed, where that is much less than the table's width; it is for speed alone.
     """
     dtype, shape, cache_shape = q.dtype, q.shape, k_cache.shape

@@ -379,6 +379,56 @@ def test_attention_output_that_shares_memory_is_refused():
     assert "cache" in _native_refusal(*a, flat[:512].view(2, 4, 64))
 
 
+def test_attention_outputs_that_share_memory_with_anything_are_refused():
+    """Heads of the output that meet one another, and sums or outputs over any other array; places between and beside are fine.
+    (By the native entry, before it looks for a device.)"""
+    c = Case([40, 3, 8], 4, 2, 64, 16, torch.bfloat16, device="cpu")
+    flat = torch.zeros(4096, dtype=torch.bfloat16)
+
+    def answer(q=c.q, out=c.out, lse=None, table=c.table, lens=c.len_t):
+        (batch, heads, dim), (pages, size, kv, _) = q.shape, c.k.shape
+        lse_at, lse_pitch = (0, 0) if lse is None else (lse.data_ptr(), lse.stride(0))
+        rc = _native.entry("iris_k_paged_attention")(P._ATTENTION.pack(
+            *(t.data_ptr() for t in (q, c.k, c.v, table, lens, out)), lse_at, 0, 0, 0, *q.stride()[:2], *c.k.stride()[:3],
+            table.stride(0), *out.stride()[:2], lse_pitch, batch, heads, dim, pages, size, kv, table.shape[1], 0, 0, 0, 0, -1, 0,
+            -1, 0, dim ** -0.5))
+        lib = _native.kernels()
+        lib.iris_paged_attention_last_error.restype = ctypes.c_char_p
+        assert rc < 0
+        return lib.iris_paged_attention_last_error().decode()
+    heads = lambda *pitches: torch.as_strided(flat, (3, 4, 64), (*pitches, 1), 0)   # noqa: E731
+    for fine in (heads(256, 64), heads(64, 192), heads(128, 512), heads(1024, 72)):
+        assert "no device" in answer(out=fine)
+    for bad in (heads(64, 64), heads(64, 128), heads(128, 64), heads(192, 64), heads(256, 80)):
+        assert "must not overlap" in answer(out=bad)
+    wide = torch.zeros((3, 8), dtype=torch.float32)
+    assert "no device" in answer(lse=wide[:, :4])
+    assert "must not overlap" in answer(lse=wide[:1, :4].expand(3, -1))
+    floats = lambda t: torch.as_strided(t, (t.untyped_storage().nbytes() // t.element_size(),), (1,), 0).view(torch.float32)   # noqa: E731
+    for other in (c.q, c.k, c.out):
+        at = floats(other)[other.storage_offset() // 2:][:12].view(3, 4)
+        assert "lse must share" in answer(lse=at), other.shape
+    at = floats(c.whole)[128:224].view(3, 32)[:, :4]                              # within what the views' first and last bytes span
+    assert "lse must share" in answer(lse=at)
+    gap = torch.as_strided(floats(c.whole), (3, 4), (5 * 36, 1), 4 * 36)           # behind the last head of a sequence
+    assert "no device" in answer(out=c.out[:, :, :], lse=gap.clone())
+
+
+@gpu
+def test_attention_outputs_over_the_table_or_the_lengths_are_refused():
+    c = Case([40, 3, 8], 4, 2, 64, 16, torch.bfloat16)
+    flat, wide = torch.zeros(4096, dtype=torch.bfloat16, device="cuda"), torch.zeros((3, 8), device="cuda")
+    ints, out = flat.view(torch.int32), flat[:768].view(3, 4, 64)
+    ok = dict(q=c.q, k_cache=c.k, v_cache=c.v, block_table=c.table, lens=c.len_t, out=c.out)
+    for bad in (dict(lse=torch.as_strided(c.table, (12,), (1,), 0).view(torch.float32).view(3, 4)),
+                dict(lse=wide[:, :4], lens=wide.view(torch.int32).flatten()[1:4]),
+                dict(out=out, block_table=ints[40:58].view(3, 6)), dict(out=out, lens=ints[:3])):
+        with pytest.raises(RuntimeError, match="block table or the lengths"):
+            P.paged_attention(**{**ok, **bad})
+    P.paged_attention(**{**ok, "lse": wide[:, :4], "lens": wide.view(torch.int32).flatten()[4:7]})   # between the rows: lengths of zero
+    assert not c.out.any() and bool((wide[:, :4] == -math.inf).all()) and not wide[:, 4:].any()
+
+
 def test_attention_table_of_too_many_keys_is_refused():
     """Positions are counted in 32 bits, up to a batch of blocks behind the last key."""
     c = Case([40, 3], 4, 2, 64, 16, torch.bfloat16, device="cpu")
