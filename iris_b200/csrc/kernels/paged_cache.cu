@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__
       len[u] = more[u] = 0;
       if (b < p.batch) {
         len[u] = max(p.lens[b], 0);
-        more[u] = max(p.more[b], 0);
+        more[u] = RELEASE ? p.more[b] : max(p.more[b], 0);
       }
     }
     __syncthreads();               // the chunk before has been used

@@ -579,6 +579,20 @@ def test_release_gives_everything_back(batch, page, wide):
 
 
 @gpu
+@pytest.mark.parametrize("batch", [4, 700])
+def test_release_takes_any_number_but_zero_for_yes(batch):
+    """``which`` may be the negative of a comparison, or bits."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    which = [(-1, 0, -(2 ** 31), 7)[b % 4] for b in range(batch)]
+    lens, table, free, count = i32([3] * batch), i32([[b] for b in range(batch)]), i32([-5] * batch), i32([0])
+    P.release_slots(lens, i32(which), table, free, count, 4)
+    back = [b for b in range(batch) if which[b]]
+    assert lens.tolist() == [0 if w else 3 for w in which] and count.item() == len(back)
+    assert free.tolist() == back + [-5] * (batch - len(back))
+    assert table.flatten().tolist() == [-1 if w else b for b, w in enumerate(which)]
+
+
+@gpu
 def test_release_without_room_keeps_the_request():
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
     lens, table, free, count = i32([8, 8, 8]), i32([[1, 2], [3, 4], [5, 6]]), i32([0, 9, 9, 9]), i32([1])
