@@ -21,6 +21,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include "iris/overlap.cuh"
 #include "iris/ptx_sm100.cuh"
 
 namespace iris {
@@ -266,6 +267,31 @@ int refuse(const char* what) {
   return -1;
 }
 
+// An array of a call; in_place: where else it may lie.
+struct Array {
+  iris::overlap::Rows rows;
+  bool written;
+  const void* in_place[2];
+};
+Array ints(const void* at, int64_t n, bool written = false, const void* in_place = nullptr, const void* or_in_place = nullptr) {
+  return {iris::overlap::one_row(at, n * 4), written, {in_place, or_in_place}};
+}
+Array rows_of(const void* table, int64_t batch, int64_t wide, int64_t pitch) {
+  return {iris::overlap::matrix(table, wide * 4, batch, pitch * 4), true, {nullptr, nullptr}};
+}
+// Whether what is written shares memory with anything else, but for what may be updated in place.
+template <int N>
+bool share_memory(const Array (&arrays)[N]) {
+  for (int i = 0; i < N; ++i)
+    for (int j = 0; j < i; ++j) {
+      const Array &a = arrays[i], &b = arrays[j];
+      if (!a.written && !b.written) continue;
+      if (a.rows.at == b.rows.at && a.rows.bytes == b.rows.bytes && (a.in_place[0] == b.rows.at || a.in_place[1] == b.rows.at)) continue;
+      if (meet(a.rows, b.rows)) return true;
+    }
+  return false;
+}
+
 template <bool RELEASE>
 int launch(const Params& p, int64_t items, void* stream) {
   cudaLaunchConfig_t cfg = {};
@@ -317,31 +343,10 @@ static int reserve(const IrisReserveArgs* args, int64_t max_len, bool fresh) {
   if (page_size < 1 || (page_size & (page_size - 1)) || page_size > (1 << 30)) return refuse("page size must be a power of two");
   if (batch < 1 || batch > 0x7fffffff - 4 * kThreads || wide < 1 || wide > 0x7fffffff || capacity < 0 || capacity > 0x7fffffff || tokens < 0 || row_stride < 0)
     return refuse("sizes out of range");
-  // what is written shares no memory with anything else, but for lengths and count that are updated in place
-  struct Array {
-    const void* at;
-    int64_t n;
-  };
-  const Array written[] = {{slots, tokens}, {positions, tokens}, {lens_out, batch}, {count_out, 1}};
-  const Array read[] = {{lens, batch}, {new_lens, batch}, {free, capacity}, {count, 1}};
-  const auto meet = [](const Array& a, const Array& b) {
-    const int *x = static_cast<const int*>(a.at), *y = static_cast<const int*>(b.at);
-    return a.n > 0 && b.n > 0 && x < y + b.n && y < x + a.n;
-  };
-  const auto in_table = [&](const Array& a) {   // (an array may lie between the table's rows)
-    const int *x = static_cast<const int*>(a.at), *t = static_cast<const int*>(static_cast<const void*>(table));
-    if (!meet(a, {t, (batch - 1) * table_pitch + wide})) return false;
-    return x < t || table_pitch < 1 || (x - t) % table_pitch < wide || (x - t) % table_pitch + a.n > table_pitch;
-  };
-  for (int i = 0; i < 4; ++i) {
-    for (int j = 0; j < i; ++j)
-      if (meet(written[i], written[j])) return refuse("outputs must not share memory");
-    for (int j = 0; j < 4; ++j) {
-      const bool in_place = (i == 2 && (j == 0 ? lens_out == lens : j == 1 && lens_out == new_lens)) || (i == 3 && j == 3 && count_out == count);
-      if (!in_place && meet(written[i], read[j])) return refuse("outputs must not share memory with inputs");
-    }
-    if (in_table(written[i]) || in_table(read[i])) return refuse("the block table must not share memory with the other arrays");
-  }
+  const Array arrays[] = {ints(lens, batch), ints(new_lens, batch), ints(free, capacity), ints(count, 1), rows_of(table, batch, wide, table_pitch),
+                          ints(slots, tokens, true), ints(positions, tokens, true), ints(lens_out, batch, true, lens, new_lens),
+                          ints(count_out, 1, true, count)};
+  if (share_memory(arrays)) return refuse("arrays that are written must not share memory with others");
   Params p;
   memset(&p, 0, sizeof(p));
   p.lens = static_cast<const int*>(lens);
@@ -380,6 +385,9 @@ int iris_k_release_slots(void* lens, const void* which, void* table, int64_t tab
   if (page_size < 1 || (page_size & (page_size - 1))) return refuse("page size must be a power of two");
   if (batch < 1 || batch > 0x7fffffff - 4 * kThreads || wide < 1 || wide > 0x7fffffff || capacity < 0 || capacity > 0x7fffffff)
     return refuse("sizes out of range");
+  const Array arrays[] = {ints(which, batch), ints(lens, batch, true, which), ints(free, capacity, true), ints(count, 1, true),
+                          rows_of(table, batch, wide, table_pitch)};
+  if (share_memory(arrays)) return refuse("arrays that are written must not share memory with others");
   Params p;
   memset(&p, 0, sizeof(p));
   p.lens = static_cast<const int*>(lens);

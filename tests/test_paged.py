@@ -638,6 +638,31 @@ def test_reserve_whose_arrays_share_memory_is_refused(name, bad):
     assert rc == -1 and "share memory" in lib.iris_pages_last_error().decode()
 
 
+@pytest.mark.parametrize("name,other,fine", [
+    ("free_pages", "block_table", False), ("free_pages", "lens", False), ("free_pages", "which", False), ("free_count", "free_pages", False),
+    ("lens", "block_table", False), ("which", "block_table", False), ("free_count", "lens", False), ("free_count", "gap", True),
+    ("which", "gap", True), ("lens", "gap", True), ("which", "whole lens", True), ("lens", "part of which", False)])
+@pytest.mark.skipif(torch.cuda.is_available(), reason="calls that are not refused must find no device")
+def test_release_whose_arrays_share_memory_is_refused(name, other, fine):
+    """By the native entry, before it looks for a device; places in the gaps of a strided table, and the lengths as `which`, are fine."""
+    memory = torch.zeros(400, dtype=torch.int32)
+    sizes = dict(lens=3, which=3, block_table=24, free_pages=9, free_count=1)
+    at = {n: memory.data_ptr() + 160 * i for i, n in enumerate(sizes)}
+    if other == "gap":
+        at[name] = at["block_table"] + 4 * 12                       # rows of 4 at 8 to 11 and 16 to 19
+    elif other == "whole lens":
+        at[name] = at["lens"]
+    elif other == "part of which":
+        at[name] = at["which"] + 8
+    else:
+        at[name] = at[other] + 4 * (max(0, sizes[other] - 1 - 4 * (other == "block_table")))
+    lib = _native.kernels()
+    rc = _native.typed(lib.iris_k_release_slots, P._RELEASE)(
+        at["lens"], at["which"], at["block_table"], 8, 4, at["free_pages"], 9, at["free_count"], 16, 3, 0)
+    lib.iris_pages_last_error.restype = ctypes.c_char_p
+    assert ("share memory" in lib.iris_pages_last_error().decode()) == (not fine) and rc == (-3 if fine else -1)
+
+
 @gpu
 def test_reserve_lengths_over_the_new_ones_and_arrays_between_the_rows():
     """``lens_out`` may be ``new_lens``, and a count or lengths may lie in the gaps of a strided table; ``which`` may be the lengths."""
