@@ -9,7 +9,7 @@
 // as long as they last: a request with first_b + need_b > count, too long for its row of the table or for the caller's limit, with
 // more tokens than rows were left for them, or that holds tokens although only empty ones are asked for, gets nothing.  Every new
 // token gets its position and its slot, page * page_size + position % page_size.  release: pages of chosen requests go back to the
-// end of the list.  No counterpart in the reference.
+// end of the list, in their order; negative entries of a row are passed over.  No counterpart in the reference.
 //
 // A call's time is its launch and a few passes through memory in a row (lengths, prefix sums, free list or table, output), so
 // it is one launch: every CTA of one cluster makes the prefix sums for itself, in chunks of a few requests per thread, and the
@@ -20,6 +20,8 @@
 #include <stdint.h>
 #include <stdio.h>
 #include <string.h>
+
+#include <type_traits>
 
 #include "iris/overlap.cuh"
 #include "iris/ptx_sm100.cuh"
@@ -59,6 +61,24 @@ struct Chunk {
   int64_t warp_sum[2][kWarps];
 };
 
+// The same for requests that end.
+template <int PER>
+struct Leaving {
+  static constexpr int kChunk = kThreads * PER;
+  int64_t entries_upto[kChunk];    // of their rows
+  int64_t pages_upto[kChunk];      // of these, the pages
+  int found[kChunk];               // pages in this CTA's share of the entries
+  bool leaves[kChunk];
+  int in_warp[2][kWarps];
+  int64_t warp_sum[2][kWarps];
+};
+template <int PER>
+__device__ __forceinline__ int found_by(const Leaving<PER>& c, int i, int cta) {
+  int n;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(n) : "r"(mapa_shared(smem_u32(&c.found[i]), cta)) : "memory");
+  return n;
+}
+
 // Sums of the threads before this one and this one's own.
 __device__ __forceinline__ int64_t scan(int64_t x, int64_t* warp_sum, int64_t& all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -88,18 +108,140 @@ __device__ __forceinline__ int search(const int64_t* upto, int64_t at) {
   return lo;
 }
 
-template <bool RELEASE, int PER>
-__global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__ Params p) {
+// Gives the pages of the requests that are asked for back to the list.  Negative entries of their rows are no pages (a program may
+// take pages out of a row itself, those that a window has left behind for instance): they are passed over.  So each CTA of the cluster
+// first counts the pages in its share of a chunk's entries, the CTAs put their counts together, and then each moves the entries of
+// its share, their places counted on from there.
+// (Cold caches, without the count and with it: 8 requests of 256 pages 8 and 11 us, 512 of 32 11 and 12, 512 of 256 32 and 41.)
+template <int PER>
+__device__ __forceinline__ void release(const Params& p, Leaving<PER>& c) {
+  constexpr int kPer = PER, kChunk = Leaving<PER>::kChunk, U = 4;   // U: loads under way at once
+  const int mask = (1 << p.page_shift) - 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = blockIdx.x, ctas = gridDim.x;
+  const int count = min(max(*p.count, 0), p.capacity);
+  int64_t pages = 0;               // of the chunks before, also of requests that the list had no room for
+  int64_t used = 0;                // taken back so far
+  const auto entry_of = [&](int base, int r, int64_t k) {
+    return p.table + (base + r) * p.table_pitch + (k - (r ? c.entries_upto[r - 1] : 0));
+  };
+  for (int base = 0; base < p.batch; base += kChunk) {
+    int64_t need[kPer], sum = 0, entries, all;
+    bool asked[kPer];
+    __syncthreads();               // the chunk before has been used
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int i = threadIdx.x * kPer + u, b = base + i;
+      asked[u] = b < p.batch && p.more[b] != 0;
+      need[u] = asked[u] ? min((max((int64_t)p.lens[b], (int64_t)0) + mask) >> p.page_shift, (int64_t)p.wide) : 0;
+      sum += need[u];
+      c.found[i] = 0;
+    }
+    int64_t upto = scan(sum, c.warp_sum[0], entries) - sum;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) c.entries_upto[threadIdx.x * kPer + u] = upto += need[u];
+    __syncthreads();
+    const int64_t from = entries * rank / ctas, to = entries * (rank + 1) / ctas;
+    // U tiles of entries at once, from k0 on: their requests, places and contents
+    int request[U], page[U];
+    int* entry[U];
+    auto look = [&](int64_t k0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t k = k0 + u * kThreads + threadIdx.x;
+        request[u] = search<kChunk>(c.entries_upto, min(k, to - 1));
+        entry[u] = k < to ? entry_of(base, request[u], k) : nullptr;
+        page[u] = entry[u] ? *entry[u] : -1;
+      }
+    };
+    for (int64_t k0 = from; k0 < to; k0 += kThreads * U) {
+      look(k0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t there = __ballot_sync(0xffffffffu, page[u] >= 0);
+        const int r = __shfl_sync(0xffffffffu, request[u], 0);
+        if (__all_sync(0xffffffffu, request[u] == r)) {
+          if (lane == 0 && there) atomicAdd(&c.found[r], __popc(there));
+        } else if (page[u] >= 0) {
+          atomicAdd(&c.found[request[u]], 1);
+        }
+      }
+    }
+    __syncthreads();
+    cluster_sync_all();            // every CTA has counted its share, and read the lengths
+    sum = 0;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      need[u] = 0;
+      for (int x = 0; x < ctas; ++x) need[u] += found_by(c, threadIdx.x * kPer + u, x);
+      sum += need[u];
+    }
+    upto = scan(sum, c.warp_sum[1], all) - sum;
+    const int64_t room = p.capacity - count - pages;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int i = threadIdx.x * kPer + u;
+      c.pages_upto[i] = upto += need[u];
+      asked[u] = asked[u] && (need[u] == 0 || upto <= room);
+      c.leaves[i] = asked[u];
+    }
+    __syncthreads();
+    // requests whose pages go back come before those that found no room, so pages before a request have all gone back
+    if (all == entries) {          // all entries are pages, each has its place
+      for (int64_t k0 = from; k0 < to; k0 += kThreads * U) {
+        if (to - from > kThreads * U) look(k0);                     // (else they are still there)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (entry[u] && c.leaves[request[u]]) p.free[count + pages + k0 + u * kThreads + threadIdx.x] = page[u], *entry[u] = -1;
+      }
+    } else if (from < to) {
+      const int r0 = search<kChunk>(c.entries_upto, from);
+      int64_t at = count + pages + (r0 ? c.pages_upto[r0 - 1] : 0);
+      for (int x = 0; x < rank; ++x) at += found_by(c, r0, x);
+      int turn = 0;
+      for (int64_t k0 = from; k0 < to; k0 += kThreads, turn ^= 1) {
+        const int64_t k = k0 + threadIdx.x;
+        const int r = search<kChunk>(c.entries_upto, min(k, to - 1));
+        const bool leaves = k < to && c.leaves[r];
+        int* at_entry = leaves ? entry_of(base, r, k) : nullptr;
+        const int got = leaves ? *at_entry : -1;
+        const uint32_t there = __ballot_sync(0xffffffffu, got >= 0);
+        if (lane == 0) c.in_warp[turn][warp] = __popc(there);
+        __syncthreads();
+        int before = __popc(there & ((1u << lane) - 1)), tile = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) before += c.in_warp[turn][w];
+          tile += c.in_warp[turn][w];
+        }
+        if (got >= 0) p.free[at + before] = got;
+        if (leaves) *at_entry = -1;
+        at += tile;
+      }
+    }
+    if (room > 0) {
+      const int i = all <= room ? kChunk : search<kChunk>(c.pages_upto, room);   // the first that found no room
+      used += i ? c.pages_upto[i - 1] : 0;
+    }
+    pages += all;
+    __syncthreads();
+    cluster_sync_all();            // every CTA has read the others' counts
+#pragma unroll
+    for (int u = 0; u < kPer; ++u)
+      if (rank == 0 && asked[u]) p.lens_out[base + threadIdx.x * kPer + u] = 0;
+  }
+  if (rank == 0 && threadIdx.x == 0) *p.count_out = (int)(count + used);
+}
+
+// Pages, slots and positions for new tokens (at the top of the file).
+template <int PER>
+__device__ __forceinline__ void reserve(const Params& p, Chunk<PER>& c) {
   constexpr int kPer = PER, kChunk = Chunk<PER>::kChunk;
-  __shared__ Chunk<PER> c;
-  grid_dependency_wait();
-  grid_dependency_launch();
   const int mask = (1 << p.page_shift) - 1;
   const int rank = blockIdx.x, ctas = gridDim.x;
   const int64_t at0 = (int64_t)rank * kThreads + threadIdx.x, step = (int64_t)ctas * kThreads;
   const int count = min(max(*p.count, 0), p.capacity);
   int64_t pages = 0, tokens = 0;   // of the chunks before
-  int64_t used = 0;                // pages handed out, or taken back, so far
+  int64_t used = 0;                // pages handed out so far
 
   // This thread's requests of a chunk, base + threadIdx.x * kPer on: granted or not, and the chunk's sums in shared memory.
   int len[kPer], more[kPer];
@@ -113,32 +255,25 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__
       len[u] = more[u] = 0;
       if (b < p.batch) {
         len[u] = max(p.lens[b], 0);
-        more[u] = RELEASE ? p.more[b] : max(p.more[b], 0);
+        more[u] = max(p.more[b], 0);
       }
     }
     __syncthreads();               // the chunk before has been used
-    if (!RELEASE) {
 #pragma unroll
-      for (int u = 0; u < kPer; ++u) t_upto[u] = sum += more[u];
-      const int64_t before = scan(sum, c.warp_sum[1], all_tokens) - sum;
+    for (int u = 0; u < kPer; ++u) t_upto[u] = sum += more[u];
+    const int64_t before = scan(sum, c.warp_sum[1], all_tokens) - sum;
 #pragma unroll
-      for (int u = 0; u < kPer; ++u) t_upto[u] += before;
-    }
+    for (int u = 0; u < kPer; ++u) t_upto[u] += before;
     sum = 0;
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
       const int b = base + threadIdx.x * kPer + u;
       need[u] = 0;
       granted[u] = b < p.batch;
-      if (RELEASE) {
-        granted[u] = granted[u] && more[u] != 0;
-        if (granted[u]) need[u] = min(held_of(len[u]), p.wide);
-      } else {
-        const int64_t end = (int64_t)len[u] + more[u];
-        granted[u] = granted[u] && end <= p.most && (len[u] <= p.most_held || more[u] == 0) &&
-                     (p.row_stride ? more[u] <= p.row_stride : tokens + t_upto[u] <= p.tokens);
-        if (granted[u]) need[u] = ((end + mask) >> p.page_shift) - held_of(len[u]);
-      }
+      const int64_t end = (int64_t)len[u] + more[u];
+      granted[u] = granted[u] && end <= p.most && (len[u] <= p.most_held || more[u] == 0) &&
+                   (p.row_stride ? more[u] <= p.row_stride : tokens + t_upto[u] <= p.tokens);
+      if (granted[u]) need[u] = ((end + mask) >> p.page_shift) - held_of(len[u]);
       sum += need[u];
     }
     int64_t upto = scan(sum, c.warp_sum[0], all_pages) - sum;
@@ -146,9 +281,9 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__
     for (int u = 0; u < kPer; ++u) {
       const int i = threadIdx.x * kPer + u;
       upto += need[u];
-      granted[u] = granted[u] && (need[u] == 0 || pages + upto <= (RELEASE ? p.capacity - count : count));
+      granted[u] = granted[u] && (need[u] == 0 || pages + upto <= count);
       c.pages_upto[i] = upto;
-      if (!RELEASE) c.tokens_upto[i] = t_upto[u];
+      c.tokens_upto[i] = t_upto[u];
       c.len[i] = granted[u] ? len[u] : ~len[u];
     }
     // requests that got pages come before those that did not, so the last of them has the sum
@@ -156,7 +291,7 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__
   };
   auto last_granted = [&](int64_t all) {   // pages of the chunk that were handed out
     if (all == 0) return (int64_t)0;
-    const int64_t room = (RELEASE ? p.capacity - count : count) - pages;
+    const int64_t room = count - pages;
     if (all <= room) return all;
     // the largest sum within the room
     if (room <= 0) return (int64_t)0;
@@ -172,75 +307,65 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__
     for (int64_t k = at0; k < got; k += step) {
       const int r = search<kChunk>(c.pages_upto, k);
       const int64_t i = k - (r ? c.pages_upto[r - 1] : 0);
-      int* entry = p.table + (base + r) * p.table_pitch;
-      if (RELEASE) {
-        p.free[count + pages + k] = entry[i];
-        entry[i] = -1;
-      } else {
-        entry[held_of(c.len[r]) + i] = p.free[count - 1 - (pages + k)];
-      }
+      p.table[(base + r) * p.table_pitch + held_of(c.len[r]) + i] = p.free[count - 1 - (pages + k)];
     }
-    if (!RELEASE) {
-      // token rows of this chunk's requests: packed one request behind the other, or row_stride rows to a request
-      const int n = min(kChunk, p.batch - base);
-      const int64_t row0 = p.row_stride ? base * p.row_stride : tokens;
-      const int64_t row1 = min(p.tokens, p.row_stride ? (base + n) * p.row_stride : tokens + all_tokens);
-      // Many rows: four in a row to a thread, one search, and a page looked up once for the rows that lie in it (32 prompts,
-      // 65536 rows: 9.3 -> 7.8 us).  Few: one to a thread (512 requests of one token: 4.1 us, 5.5 with four).
-      const int width = row1 - row0 > 2 * step ? 4 : 1;
-      for (int64_t at = row0 + width * at0; at < row1; at += width * step) {
-        int r;
-        int64_t j;
-        if (p.row_stride) {
-          r = (int)((at - row0) / p.row_stride);
-          j = at - row0 - r * p.row_stride;
-        } else {
-          r = search<kChunk>(c.tokens_upto, at - row0);
-          j = at - row0 - (r ? c.tokens_upto[r - 1] : 0);
-        }
-        int slot[4], position[4], known = -1, page = -1;
-        int64_t more_here = c.tokens_upto[r] - (r ? c.tokens_upto[r - 1] : 0);
-        const int n4 = (int)min((int64_t)width, row1 - at);
+    // token rows of this chunk's requests: packed one request behind the other, or row_stride rows to a request
+    const int n = min(kChunk, p.batch - base);
+    const int64_t row0 = p.row_stride ? base * p.row_stride : tokens;
+    const int64_t row1 = min(p.tokens, p.row_stride ? (base + n) * p.row_stride : tokens + all_tokens);
+    // Many rows: four in a row to a thread, one search, and a page looked up once for the rows that lie in it (32 prompts,
+    // 65536 rows: 9.3 -> 7.8 us).  Few: one to a thread (512 requests of one token: 4.1 us, 5.5 with four).
+    const int width = row1 - row0 > 2 * step ? 4 : 1;
+    for (int64_t at = row0 + width * at0; at < row1; at += width * step) {
+      int r;
+      int64_t j;
+      if (p.row_stride) {
+        r = (int)((at - row0) / p.row_stride);
+        j = at - row0 - r * p.row_stride;
+      } else {
+        r = search<kChunk>(c.tokens_upto, at - row0);
+        j = at - row0 - (r ? c.tokens_upto[r - 1] : 0);
+      }
+      int slot[4], position[4], known = -1, page = -1;
+      int64_t more_here = c.tokens_upto[r] - (r ? c.tokens_upto[r - 1] : 0);
+      const int n4 = (int)min((int64_t)width, row1 - at);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          slot[u] = position[u] = -1;
-          if (u >= n4) break;
-          while (p.row_stride ? j >= p.row_stride : j >= more_here) {   // on to the next request (that has a token)
-            ++r;
-            j = 0;
-            known = -1;
-            more_here = c.tokens_upto[r] - c.tokens_upto[r - 1];
-          }
-          if (c.len[r] >= 0 && j < more_here) {
-            const int pos = (int)(c.len[r] + j), i = pos >> p.page_shift, fresh = i - held_of(c.len[r]);
-            if (i != known) {
-              known = i;
-              page = fresh < 0 ? p.table[(base + r) * p.table_pitch + i]
-                               : p.free[count - 1 - (pages + (r ? c.pages_upto[r - 1] : 0) + fresh)];
-            }
-            const int64_t s = ((int64_t)page << p.page_shift) + (pos & mask);
-            position[u] = pos;
-            slot[u] = page < 0 || s > 0x7fffffff ? -1 : (int)s;   // an entry that is no page: as a token that is not kept
-          }
-          ++j;
+      for (int u = 0; u < 4; ++u) {
+        slot[u] = position[u] = -1;
+        if (u >= n4) break;
+        while (p.row_stride ? j >= p.row_stride : j >= more_here) {   // on to the next request (that has a token)
+          ++r;
+          j = 0;
+          known = -1;
+          more_here = c.tokens_upto[r] - c.tokens_upto[r - 1];
         }
-        if (n4 == 4 && !((reinterpret_cast<uintptr_t>(p.slots + at) | reinterpret_cast<uintptr_t>(p.positions + at)) & 15)) {
-          *reinterpret_cast<int4*>(p.slots + at) = make_int4(slot[0], slot[1], slot[2], slot[3]);
-          *reinterpret_cast<int4*>(p.positions + at) = make_int4(position[0], position[1], position[2], position[3]);
-        } else {
+        if (c.len[r] >= 0 && j < more_here) {
+          const int pos = (int)(c.len[r] + j), i = pos >> p.page_shift, fresh = i - held_of(c.len[r]);
+          if (i != known) {
+            known = i;
+            page = fresh < 0 ? p.table[(base + r) * p.table_pitch + i]
+                             : p.free[count - 1 - (pages + (r ? c.pages_upto[r - 1] : 0) + fresh)];
+          }
+          const int64_t s = ((int64_t)page << p.page_shift) + (pos & mask);
+          position[u] = pos;
+          slot[u] = page < 0 || s > 0x7fffffff ? -1 : (int)s;   // an entry that is no page: as a token that is not kept
+        }
+        ++j;
+      }
+      if (n4 == 4 && !((reinterpret_cast<uintptr_t>(p.slots + at) | reinterpret_cast<uintptr_t>(p.positions + at)) & 15)) {
+        *reinterpret_cast<int4*>(p.slots + at) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        *reinterpret_cast<int4*>(p.positions + at) = make_int4(position[0], position[1], position[2], position[3]);
+      } else {
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (u < n4) p.slots[at + u] = slot[u], p.positions[at + u] = position[u];
-        }
+        for (int u = 0; u < 4; ++u)
+          if (u < n4) p.slots[at + u] = slot[u], p.positions[at + u] = position[u];
       }
     }
     pages += all_pages;
     tokens += all_tokens;
   }
-  if (!RELEASE) {
-    const int64_t end = p.row_stride ? p.batch * p.row_stride : tokens;
-    for (int64_t row = end + at0; row < p.tokens; row += step) p.slots[row] = p.positions[row] = -1;
-  }
+  const int64_t end = p.row_stride ? p.batch * p.row_stride : tokens;
+  for (int64_t row = end + at0; row < p.tokens; row += step) p.slots[row] = p.positions[row] = -1;
   cluster_sync_all();   // every CTA has read the lengths and the count
   if (rank != 0) return;
   for (int base = 0; base < p.batch; base += kChunk) {
@@ -254,10 +379,19 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
       const int b = base + threadIdx.x * kPer + u;
-      if (b < p.batch) p.lens_out[b] = !granted[u] ? p.lens[b] : RELEASE ? 0 : len[u] + more[u];
+      if (b < p.batch) p.lens_out[b] = !granted[u] ? p.lens[b] : len[u] + more[u];
     }
   }
-  if (threadIdx.x == 0) *p.count_out = (int)(RELEASE ? count + used : count - used);
+  if (threadIdx.x == 0) *p.count_out = (int)(count - used);
+}
+
+template <bool RELEASE, int PER>
+__global__ void __launch_bounds__(kThreads) pages_kernel(const __grid_constant__ Params p) {
+  __shared__ std::conditional_t<RELEASE, Leaving<PER>, Chunk<PER>> c;
+  grid_dependency_wait();
+  grid_dependency_launch();
+  if constexpr (RELEASE) release<PER>(p, c);
+  else reserve<PER>(p, c);
 }
 
 thread_local char g_err[256] = "";

@@ -210,7 +210,8 @@ def release_slots(lens: torch.Tensor, which: torch.Tensor, block_table: torch.Te
                   free_count: torch.Tensor, page_size: int, *, stream=None) -> None:
     """Gives the pages of the requests with ``which[b] != 0`` (int32) back to the end of the list of free pages; their lengths
     become 0 and their entries of the table -1.  A request whose pages the list has no room for keeps them (that, and all later
-    ones).  ``which`` may be ``lens``; nothing else shares memory."""
+    ones that hold any).  Negative entries are no pages: a program may put back pages of a row itself (those that a window has left
+    behind) and write -1 in their places.  ``which`` may be ``lens``; nothing else shares memory."""
     batch = lens.shape[0] if lens.dim() == 1 else -1
     _ints(lens, "lens", (batch,))
     _ints(which, "which", (batch,))

@@ -602,6 +602,41 @@ def test_release_without_room_keeps_the_request():
 
 
 @gpu
+@pytest.mark.parametrize("batch,page,wide,holes", [
+    (1, 16, 3, 1), (40, 16, 8, 30), (600, 4, 20, 4000), (1100, 8, 5, 1500), (3, 1, 20000, 9000), (2100, 2, 3, 0)])
+def test_release_passes_over_entries_that_are_no_page(batch, page, wide, holes):
+    """Pages that a program took out of a request's row itself (negative entries) are not put on the list of free pages; the others
+    go back in their order, and room is needed for them alone."""
+    lens, new, table, free, count = _state(batch, page, wide, 1, batch)
+    rng = random.Random(holes)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    held = [min(wide, -(-n // page)) for n in lens]
+    for _ in range(holes):
+        b = rng.randrange(batch)
+        if held[b]:
+            table[b][rng.randrange(held[b])] = rng.choice((-1, -7, -(2 ** 31)))
+    which = [b % 3 != 1 for b in range(batch)]
+    free = free[:count]
+    back = [table[b][i] for b in range(batch) if which[b] for i in range(held[b]) if table[b][i] >= 0]
+    free_t, lens_t, table_t, count_t = i32(free + [-5] * len(back)), i32(lens), i32(table), i32([count])
+    P.release_slots(lens_t, i32([int(w) for w in which]), table_t, free_t, count_t, page)
+    assert count_t.tolist() == [count + len(back)]
+    assert free_t.tolist() == free + back
+    assert lens_t.tolist() == [0 if w else n for n, w in zip(lens, which)]
+    assert table_t.tolist() == [[-1] * wide if w else r for r, w in zip(table, which)]
+
+
+@gpu
+def test_release_without_room_counts_pages_alone():
+    """A row without pages needs no room, also behind a request that finds none."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    lens, table, free, count = i32([8, 8, 8, 8]), i32([[1, -1], [-1, 4], [5, 6], [-3, -3]]), i32([0, 9, 9, 9]), i32([1])
+    P.release_slots(lens, i32([1, 1, 1, 1]), table, free, count, 4)
+    assert lens.tolist() == [0, 0, 8, 0] and count.tolist() == [3] and free.tolist() == [0, 1, 4, 9]
+    assert table.tolist() == [[-1, -1], [-1, -1], [5, 6], [-1, -1]]
+
+
+@gpu
 def test_cache_lives_through_requests():
     """Requests that come, grow and go for many steps: no page is ever held twice, and none is lost."""
     rng = random.Random(3)
