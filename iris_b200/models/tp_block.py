@@ -16,9 +16,10 @@ The reference has no model code; its fused kernels are the ingredients (``docs/F
 describes the row-parallel and column-parallel splits).  ``TPDecoderBaseline`` is the same network with cuBLAS GEMMs
 and NCCL ``all_gather_into_tensor`` / ``all_reduce``; ``reference_forward`` is the unsharded fp32 oracle.
 The attention core of the fused stack is this repository's tcgen05 kernel (``iris_b200/ops/attention.py``) whenever
-the head dimension is 128 and the sequence length a multiple of 128; the baseline stack (and the fused one for other
-shapes, or with ``attention="sdpa"``) calls ``torch.nn.functional.scaled_dot_product_attention``.  Grouped heads and sliding
-windows (``attention_window_fwd``, any sequence length) need the own kernel.
+the head dimension is 128 and the sequence length a multiple of 128 (with positions, head norms or a cache: any length); the
+baseline stack (and the fused one for other shapes, or with ``attention="sdpa"``) calls
+``torch.nn.functional.scaled_dot_product_attention``.  Grouped heads and sliding windows (``attention_window_fwd``, any sequence
+length), and single tokens over a cache (``paged_attention``), need the own kernels.
 
 Serving: a decoder of whole prompts (``seq`` rows to a sequence) and one of single tokens (``seq=1``, ``weights=`` the first one's)
 share a paged cache (``iris_b200/ops/paged.py``, :meth:`TPDecoder.make_cache`).  ``forward(x, cache=..., new_lens=...)`` takes the
@@ -173,7 +174,8 @@ class TPDecoder:
             op = G.all_gather_gemm(self.ctxs, T, bt, ag_slices=ag_slices, **kw)
             return op, op.a_full
         self.heads_local = cfg.n_heads // W
-        self.own_attention = attention == "iris" and cfg.head_dim == A.HEAD_DIM and cfg.seq % 128 == 0
+        self.own_ragged = attention == "iris" and cfg.head_dim == A.HEAD_DIM      # any length, with positions, norms or a cache
+        self.own_attention = self.own_ragged and cfg.seq % 128 == 0
         self.ts = T // W
         nl = len(self.ctxs)
         # one rank: the gate / up projection applies the SwiGLU on its way out (its own kernel otherwise)
@@ -303,7 +305,7 @@ class TPDecoder:
             q, out = (t[:, :hl * d].unflatten(1, (hl, d)) for t in (qkv, self.attn[l]))
             P.paged_attention(q, cache[l].k(layer), cache[l].v(layer), cache[l].block_table, cache[l].lens, out,
                               window=cfg.window, sinks=cfg.sinks, status=status)
-        elif self.windowed or (cfg.seq % 128 and d == A.HEAD_DIM):
+        elif self.windowed or (self.own_ragged and cfg.seq % 128):
             A.attention_window_fwd(qkv, self.attn[l], cfg.batch, cfg.seq, hl, kl, window=cfg.window or cfg.seq, sinks=cfg.sinks,
                                    status=status)
         elif self.own_attention:

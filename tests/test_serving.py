@@ -181,6 +181,31 @@ def test_rows_of_no_token_reach_nothing(kind, seq, attention, rubbish):
     prefill.close(), decode.close(), ctx.close()
 
 
+@pytest.mark.parametrize("kind", [dict(rope_theta=10000.0), dict(qk_norm=True), dict()])
+@pytest.mark.parametrize("with_cache", [False, True])
+def test_the_librarys_attention_where_it_is_asked_for(kind, with_cache, monkeypatch):
+    """``attention="sdpa"`` goes for configurations with positions or head norms and for calls with a cache too, at any length."""
+    from iris_b200.ops import attention as A
+    cfg = TPConfig(batch=2, seq=96, **SIZES, **kind)
+    ctx = iris.iris(192 << 20)
+    model = TPDecoder(ctx, cfg, attention="sdpa")
+    x = _inputs(2, 96).view(192, -1)
+
+    def never(*a, **k):
+        raise AssertionError("the own kernel was called")
+    monkeypatch.setattr(A, "attention_window_fwd", never)
+    monkeypatch.setattr(A, "attention_fwd", never)
+    shards = [x.clone()]
+    if with_cache:
+        got = _forward(model, x, model.make_cache(12, 16, 2, 96), [96, 96])
+    else:
+        model.forward(shards)
+        got = shards[0]
+    model.check()
+    _near(got, reference_forward(x, cfg))
+    model.close(), ctx.close()
+
+
 def test_refusals():
     ctx = iris.iris(192 << 20)
     cfg = TPConfig(batch=2, seq=64, **SIZES, **KINDS["grouped"])
