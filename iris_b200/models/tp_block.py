@@ -239,6 +239,8 @@ class TPDecoder:
                 raise ValueError("the cache does not fit this decoder (make_cache)")
             if self.rotation is not None and any(c.max_len > self.rotation.shape[0] for c in cache):
                 raise ValueError("the cache holds more positions than there are angles for (TPConfig.positions)")
+            if cfg.seq == 1 and cfg.head_dim not in P.HEAD_DIMS:
+                raise ValueError(f"single tokens over a cache need heads of 64, 128 or 256, not {cfg.head_dim}")
             tick("reserve")
             for l in range(nl):
                 cache[l].reserve(new_lens, self.slots, self.cache_positions, row_stride=cfg.seq, fresh=cfg.seq > 1)

@@ -17,6 +17,7 @@ import torch
 
 from .. import _native
 
+HEAD_DIMS = (64, 128, 256)   # of paged_attention
 _DT = {torch.bfloat16: 0, torch.float16: 1}
 _P, _L, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 _ATTENTION, _RESERVE, _LIMITS = struct.Struct("@34qd"), struct.Struct("@17q"), struct.Struct("@2q")
@@ -82,7 +83,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError("expected q and out [batch, heads, head_dim] and a cache [pages, page_size, kv_heads, head_dim]")
     batch, heads, dim = shape
     pages, size, kv_heads, cache_dim = cache_shape
-    if cache_dim != dim or kv_heads < 1 or heads < 1 or heads % kv_heads or dim not in (64, 128, 256):
+    if cache_dim != dim or kv_heads < 1 or heads < 1 or heads % kv_heads or dim not in HEAD_DIMS:
         raise ValueError(f"{heads} query heads of {dim} do not go with {kv_heads} key heads of {cache_dim} (64, 128 or 256)")
     q_batch, q_head, q_one = q.stride()
     out_batch, out_head, out_one = out.stride()

@@ -206,6 +206,20 @@ def test_the_librarys_attention_where_it_is_asked_for(kind, with_cache, monkeypa
     model.close(), ctx.close()
 
 
+def test_heads_that_cannot_be_decoded_are_refused_before_pages_are_taken():
+    more = dict(SIZES, hidden=512, rope_theta=10000.0, positions=40)
+    more.update(n_heads=16, head_dim=32)
+    ctx = iris.iris(192 << 20)
+    prefill = TPDecoder(ctx, TPConfig(batch=2, seq=32, **more))
+    decode = TPDecoder(ctx, TPConfig(batch=2, seq=1, **more), weights=prefill)
+    cache = prefill.make_cache(8, 16, 2, 40)
+    _forward(prefill, _inputs(2, 32).view(64, -1), cache, [20, 3])
+    with pytest.raises(ValueError, match="64, 128 or 256"):
+        _forward(decode, _inputs(2, 1).view(2, -1), cache, [1, 1])
+    assert cache[0].lens.tolist() == [20, 3] and cache[0].free_count.item() == 5
+    prefill.close(), decode.close(), ctx.close()
+
+
 def test_refusals():
     ctx = iris.iris(192 << 20)
     cfg = TPConfig(batch=2, seq=64, **SIZES, **KINDS["grouped"])
