@@ -445,7 +445,8 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
 #pragma unroll
         for (int b = 0; b < kTB; ++b) {
           const bool good = got[b] && (uint32_t)page[b] < (uint32_t)p.pages;
-          if (got[b] && !good) record_status(p.status, kBadPointer, kSitePage, l.b, b, (uint64_t)(int64_t)page[b]);
+          const int key = __shfl_sync(0xffffffffu, now.key, first_lane + b) + (lane & 15);
+          if (got[b] && !good) record_status(p.status, kBadPointer, kSitePage, l.b, key, (uint64_t)(int64_t)page[b]);
           got[b] = __ballot_sync(0xffffffffu, good) & 0xffffu;
           if (lane == 0) masks[stage * kTB + b] = got[b];
           for (int j = 0; j < kBlock; j += size)

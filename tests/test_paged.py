@@ -183,6 +183,19 @@ def test_attention_leaves_out_and_reports_bad_pages(wide):
 
 
 @gpu
+@pytest.mark.parametrize("page", [1, 2, 4, 8, 16, 64])
+@pytest.mark.parametrize("wide", [None, 5000])
+def test_attention_reports_the_key_of_a_bad_page(page, wide):
+    """The record names the sequence and a key of the page, whatever the pages' size."""
+    case = Case([5, 16 * 23 + 1], 4, 2, 128, page, torch.bfloat16, wide=wide)
+    status = torch.zeros(16, dtype=torch.int32, device="cuda")
+    case.table[1, 16 * 23 // page] = -3                                     # that of the last key
+    case.run(status=status)
+    first = 16 * 23 // page * page
+    assert status[:3].tolist() == [2, 95, 1] and first <= status[3].item() <= 16 * 23 and status[4].item() == -3
+
+
+@gpu
 def test_attention_lengths_outside_the_table_are_cut():
     case = Case([64, 64], 2, 1, 64, 16, torch.bfloat16)
     case.run()
