@@ -87,7 +87,7 @@ def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: 
     if rows == 0:
         return out
     qkv_ptr, out_ptr = qkv.data_ptr(), out.data_ptr()
-    if rows > 1 and ld_out < heads * HEAD_DIM or not (out_ptr == qkv_ptr and ld_out == ld_in) and may_overlap(
+    if rows > 1 and ld_out < heads * HEAD_DIM or not (out_ptr == qkv_ptr and (ld_out == ld_in or rows == 1)) and may_overlap(
             rows, qkv_ptr, ld_in, (heads + 2 * kv_heads) * HEAD_DIM, out_ptr, ld_out, heads * HEAD_DIM):
         raise ValueError("rows of out must not overlap, nor lie over qkv but for the query columns themselves")
     if device != _native.current_device(device):

@@ -133,7 +133,7 @@ def qk_norm_rope(qkv: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, 
     if tokens == 0:
         return out
     qkv_ptr, out_ptr = qkv.data_ptr(), out.data_ptr()
-    in_place = out_ptr == qkv_ptr and ld_out == ld_in
+    in_place = out_ptr == qkv_ptr and (ld_out == ld_in or tokens == 1)
     if tokens > 1 and ld_out < out_width:
         raise ValueError("rows of out must not overlap")
     if not in_place and may_overlap(tokens, qkv_ptr, ld_in, width, out_ptr, ld_out, out_width):

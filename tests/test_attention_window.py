@@ -251,6 +251,13 @@ def test_refusals():
             A.attention_window_fwd(**{**ok, "qkv": wide[:, :1024], "out": fine})
 
 
+def test_one_token_over_its_queries_whatever_its_strides():
+    """Along one row a stride says nothing."""
+    qkv, _, _ = _inputs(1, 1, 4, 2, torch.bfloat16, device="cpu")
+    with pytest.raises(ValueError, match="CUDA device"):
+        A.attention_window_fwd(qkv, torch.as_strided(qkv, (1, 512), (0, 1)), 1, 1, 4, 2, window=4)
+
+
 def test_a_status_that_is_no_block_is_refused():
     """A record has 32 bytes; what is smaller, strided or misaligned would be written past."""
     qkv, _, out = _inputs(2, 10, 4, 2, torch.bfloat16, device="cpu")

@@ -277,6 +277,15 @@ def test_refusals():
             R.rotary_table(**{**dict(positions=4, rotary_dim=32), **bad})
 
 
+def test_one_token_in_place_whatever_its_strides():
+    """Along one row a stride says nothing."""
+    c = Case(1, 2, 1, 32, 16, torch.bfloat16, device="cpu")
+    over = torch.as_strided(c.qkv, c.qkv.shape, (0, 1))
+    for out in (over, over[:, :64]):
+        with pytest.raises(ValueError, match="CUDA device"):
+            R.qk_norm_rope(c.qkv, out, c.pos, c.table, 2, 1, 32, **c.kw(), **c.cache())
+
+
 def test_a_status_that_is_no_block_is_refused():
     """A record has 32 bytes; what is smaller, strided or misaligned would be written past."""
     c = Case(3, 2, 1, 32, 16, torch.bfloat16, device="cpu")
