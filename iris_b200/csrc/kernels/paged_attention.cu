@@ -1149,19 +1149,18 @@ int iris_k_paged_attention(const IrisPagedAttentionArgs* args) {
     if (!apart) return refuse("out must be q itself, or share no memory with it");
   }
   using namespace iris::overlap;
-  const Rows to = {out, dim * 2, {{batch, out_batch * 2}, {heads, out_head * 2}, {1, 0}}}, sums = matrix(lse, heads * 4, batch, lse_batch * 4);
-  const Rows from = {q, dim * 2, {{batch, q_batch * 2}, {heads, q_head * 2}, {1, 0}}};
-  const Rows keys = {k, dim * 2, {{pages, page_pitch * 2}, {page_size, slot_pitch * 2}, {kv_heads, head_pitch * 2}}};
-  Rows values = keys;
-  values.at = v;
+  const Rows to(out, dim * 2, {batch, out_batch * 2}, {heads, out_head * 2}), sums(lse, heads * 4, {batch, lse_batch * 4});
+  const Rows from(q, dim * 2, {batch, q_batch * 2}, {heads, q_head * 2});
+  const Rows keys(k, dim * 2, {pages, page_pitch * 2}, {page_size, slot_pitch * 2}, {kv_heads, head_pitch * 2});
+  const Rows values(v, dim * 2, {pages, page_pitch * 2}, {page_size, slot_pitch * 2}, {kv_heads, head_pitch * 2});
   if (!apart(to) || !apart(sums)) return refuse("rows of out, or of lse, must not overlap");
   if (meet(sums, to) || meet(sums, from) || meet(sums, keys) || meet(sums, values))
     return refuse("lse must share no memory with q, out or the cache");
   const int sms = sms_of((int)device);
   if (sms < 1) return refuse("no device");
-  const Rows pages_of = matrix(table, wide * 4, batch, table_pitch * 4), lengths = one_row(lens, batch * 4);
-  for (const Rows& w : {to, sums})
-    if (meet(w, pages_of) || meet(w, lengths)) return refuse("out and lse must share no memory with the block table or the lengths");
+  const Rows pages_of(table, wide * 4, {batch, table_pitch * 4}), lengths(lens, batch * 4);
+  if (meet(to, pages_of) || meet(to, lengths) || meet(sums, pages_of) || meet(sums, lengths))
+    return refuse("out and lse must share no memory with the block table or the lengths");
   Params p;
   memset(&p, 0, sizeof(p));
   p.batch = (int)batch;

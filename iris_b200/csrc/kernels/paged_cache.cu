@@ -405,13 +405,13 @@ int refuse(const char* what) {
 struct Array {
   iris::overlap::Rows rows;
   bool written;
-  const void* in_place[2];
+  uintptr_t in_place[2];
 };
 Array ints(const void* at, int64_t n, bool written = false, const void* in_place = nullptr, const void* or_in_place = nullptr) {
-  return {iris::overlap::one_row(at, n * 4), written, {in_place, or_in_place}};
+  return {{at, n * 4}, written, {reinterpret_cast<uintptr_t>(in_place), reinterpret_cast<uintptr_t>(or_in_place)}};
 }
 Array rows_of(const void* table, int64_t batch, int64_t wide, int64_t pitch) {
-  return {iris::overlap::matrix(table, wide * 4, batch, pitch * 4), true, {nullptr, nullptr}};
+  return {{table, wide * 4, {batch, pitch * 4}}, true, {0, 0}};
 }
 // Whether what is written shares memory with anything else, but for what may be updated in place.
 template <int N>
@@ -420,8 +420,9 @@ bool share_memory(const Array (&arrays)[N]) {
     for (int j = 0; j < i; ++j) {
       const Array &a = arrays[i], &b = arrays[j];
       if (!a.written && !b.written) continue;
-      if (a.rows.at == b.rows.at && a.rows.bytes == b.rows.bytes && (a.in_place[0] == b.rows.at || a.in_place[1] == b.rows.at)) continue;
-      if (meet(a.rows, b.rows)) return true;
+      if (meet(a.rows, b.rows) && !(a.rows.at == b.rows.at && a.rows.end == b.rows.end &&
+                                    (a.in_place[0] == b.rows.at || a.in_place[1] == b.rows.at)))
+        return true;
     }
   return false;
 }

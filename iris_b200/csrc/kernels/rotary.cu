@@ -307,18 +307,17 @@ int iris_k_qk_norm_rope(const IrisQkNormRopeArgs* args) {
   {
     // what is written shares no memory with anything else, but for out in the place of qkv, which the caller looks after
     using namespace iris::overlap;
-    const Rows in = matrix(qkv, (heads + 2 * kv_heads) * dim * 2, tokens, ld_in * 2);
-    const Rows to = matrix(out, out_heads * dim * 2, tokens, ld_out * 2);
-    Rows keys = {k_cache, k_cache ? dim * 2 : 0, {{pages, page_pitch * 2}, {page_size, slot_pitch * 2}, {kv_heads, head_pitch * 2}}};
-    Rows values = keys;
-    values.at = v_cache;
-    if (!apart(to) || (k_cache && (!apart(keys) || meet(keys, values)))) return refuse("rows of the cache, or of out, must not overlap");
-    if (k_cache && (meet(keys, in) || meet(values, in) || meet(keys, to) || meet(values, to)))
+    const Rows in(qkv, (heads + 2 * kv_heads) * dim * 2, {tokens, ld_in * 2});
+    const Rows to(out, out_heads * dim * 2, {tokens, ld_out * 2});
+    const Rows keys(k_cache, dim * 2, {pages, page_pitch * 2}, {page_size, slot_pitch * 2}, {kv_heads, head_pitch * 2});
+    const Rows values(v_cache, dim * 2, {pages, page_pitch * 2}, {page_size, slot_pitch * 2}, {kv_heads, head_pitch * 2});
+    if (!apart(to) || !apart(keys) || meet(keys, values)) return refuse("rows of the cache, or of out, must not overlap");
+    if (meet(keys, in) || meet(values, in) || meet(keys, to) || meet(values, to))
       return refuse("the cache must share no memory with qkv or out");
-    const Rows read[] = {one_row(positions, tokens * 4), one_row(slots, tokens * 4), one_row(q_weight, dim * 2),
-                         one_row(k_weight, dim * 2), matrix(table, rotary * 4, positions_in_table, ld_table * 4)};
+    const Rows read[] = {Rows(positions, tokens * 4), Rows(slots, tokens * 4), Rows(q_weight, dim * 2),
+                         Rows(k_weight, dim * 2), Rows(table, rotary * 4, {positions_in_table, ld_table * 4})};
     for (const Rows& r : read)
-      if (meet(to, r) || (k_cache && (meet(keys, r) || meet(values, r))))
+      if (meet(to, r) || meet(keys, r) || meet(values, r))
         return refuse("out and the cache must share no memory with positions, slots, weights or the table");
   }
   Params p;

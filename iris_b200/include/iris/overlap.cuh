@@ -9,16 +9,19 @@
 namespace iris {
 namespace overlap {
 
-struct Rows {
-  const void* at;
-  int64_t bytes;
-  struct {
-    int64_t n, pitch;      // pitch in bytes
-  } dim[3];
+struct Dim {
+  int64_t n, pitch;        // pitch in bytes
 };
-
-inline Rows one_row(const void* at, int64_t bytes) { return {at, at ? bytes : 0, {{1, 0}, {1, 0}, {1, 0}}}; }
-inline Rows matrix(const void* at, int64_t bytes, int64_t n, int64_t pitch) { return {at, at ? bytes : 0, {{n, pitch}, {1, 0}, {1, 0}}}; }
+struct Rows {
+  uintptr_t at, end;       // first byte, and the one behind the last
+  int64_t bytes;
+  Dim dim[3];
+  Rows(const void* p, int64_t row, Dim a = {1, 0}, Dim b = {1, 0}, Dim c = {1, 0})
+      : at(reinterpret_cast<uintptr_t>(p)), bytes(p ? row : 0), dim{a, b, c} {
+    end = at;
+    if (bytes > 0 && a.n > 0 && b.n > 0 && c.n > 0) end += bytes + (a.n - 1) * a.pitch + (b.n - 1) * b.pitch + (c.n - 1) * c.pitch;
+  }
+};
 
 // The dimensions of more than one, largest pitch first.
 inline Rows sorted(Rows r) {
@@ -59,27 +62,23 @@ inline bool reaches(const Rows& r, int i, int back, int64_t lo, int64_t hi) {
   return false;
 }
 
-// Whether a and b share memory: exactly, if both are laid out alike or one is a single row (and the pitches nest); else whether the
-// memory from the first to the last byte of the one meets that of the other.
-inline bool meet(const Rows& a0, const Rows& b0) {
-  if (a0.bytes <= 0 || b0.bytes <= 0) return false;
+inline bool meet_within(const Rows& a0, const Rows& b0) {   // (those whose first to last bytes meet)
+  const int64_t off = (int64_t)(b0.at - a0.at);
   const Rows a = sorted(a0), b = sorted(b0);
-  int64_t a_span = a.bytes, b_span = b.bytes;
   bool alike = true, a_one = true, b_one = true;
   for (int i = 0; i < 3; ++i) {
-    if (a.dim[i].n < 1 || b.dim[i].n < 1) return false;
-    a_span += (a.dim[i].n - 1) * a.dim[i].pitch, b_span += (b.dim[i].n - 1) * b.dim[i].pitch;
     alike = alike && a.dim[i].n == b.dim[i].n && a.dim[i].pitch == b.dim[i].pitch;
     a_one = a_one && a.dim[i].n == 1, b_one = b_one && b.dim[i].n == 1;
   }
-  const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(b.at) - reinterpret_cast<uintptr_t>(a.at));
-  if (off >= a_span || off <= -b_span) return false;
   // a row of a at off_a and one of b at off + off_b meet if off - a.bytes < off_a - off_b < off + b.bytes
   if (b_one && apart(a)) return reaches(a, 0, 0, off - a.bytes, off + b.bytes);
   if (a_one && apart(b)) return reaches(b, 0, 0, -off - b.bytes, -off + a.bytes);
   if (alike && apart(a)) return reaches(a, 0, 1, off - a.bytes, off + b.bytes);
   return true;
 }
+// Whether a and b share memory: exactly, if both are laid out alike or one is a single row (and the pitches nest); else whether the
+// memory from the first to the last byte of the one meets that of the other.
+inline bool meet(const Rows& a, const Rows& b) { return a.at < b.end && b.at < a.end && a.at < a.end && b.at < b.end && meet_within(a, b); }
 
 }  // namespace overlap
 }  // namespace iris
