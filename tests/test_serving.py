@@ -220,6 +220,36 @@ def test_heads_that_cannot_be_decoded_are_refused_before_pages_are_taken():
     prefill.close(), decode.close(), ctx.close()
 
 
+def test_captured_prompts():
+    """Prompts recorded once and replayed with other rows and lengths: requests that hold tokens and padding of NaN included."""
+    more = dict(SIZES, **KINDS["window"], positions=64)
+    ctx = iris.iris(192 << 20)
+    prefill = TPDecoder(ctx, TPConfig(batch=3, seq=40, **more))
+    cache = prefill.make_cache(9, 16, 3, 64)
+    x = _inputs(3, 40)
+    want = reference_forward(x.view(120, -1), TPConfig(batch=3, seq=40, **more)).view(3, 40, -1)
+    rows, new = torch.empty((120, 512), dtype=torch.bfloat16, device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda")
+    graph = prefill.capture([rows], cache=cache, new_lens=new)
+    held = [0, 0, 0]
+    for lens in ([40, 3, 0], [5, 0, 20], [0, 0, 1], [12, 33, 0]):
+        padded = x.clone()
+        for b, n in enumerate(lens):
+            padded[b, n:] = float("nan")
+        rows.copy_(padded.view(120, -1))
+        new.copy_(torch.tensor(lens))
+        graph.replay()
+        prefill.check()
+        given = [b for b in range(3) if lens[b] and not held[b]]
+        held = [lens[b] if b in given else held[b] for b in range(3)]
+        assert cache[0].lens.tolist() == held
+        for b in given:
+            _near(rows.view(3, 40, -1)[b, :lens[b]], want[b, :lens[b]])
+        if lens[2] == 1:
+            cache[0].release(torch.tensor([1, 1, 0], dtype=torch.int32, device="cuda"))
+            held[:2] = [0, 0]
+    prefill.close(), ctx.close()
+
+
 def test_refusals():
     ctx = iris.iris(192 << 20)
     cfg = TPConfig(batch=2, seq=64, **SIZES, **KINDS["grouped"])
