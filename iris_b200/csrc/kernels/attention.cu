@@ -85,11 +85,12 @@ constexpr int kPolyEvery = 4;
 // words of bits and rows of the output written 64 bytes at a time 266,000 -> 244,700 cycles of half the case, 8 % less.)
 constexpr float kGrowth = 8.f;
 
-// fp16 with windows: weights are made 2^kLift times as large, since fp16 has no numbers below 2^-24 (8190 keys that weigh 2^-26 of
-// the largest each, 1.2e-4 of the sum, were left out of the output).  Below 2^-14 of 2^kLift they lose bits; the largest is
-// 2^(kGrowth + kLift) but for a score's rounding, half of what fp16 holds.
+// What the exponents of the weights are counted from, for a row's maximum m.  fp16 with windows: weights are made 2^7 times as
+// large, since fp16 has no numbers below 2^-24 (8190 keys that weigh 2^-26 of the largest each, 1.2e-4 of the sum, were left out of
+// the output).  Below 2^-21 of the maximum they lose bits; the largest is 2^(kGrowth + 7) but for a score's rounding, half of what
+// fp16 holds.  Not where m is so large that its own rounding would take a weight out of that.
 template <bool F16, bool WIN>
-constexpr float kLift = F16 && WIN ? 7.f : 0.f;
+__device__ __forceinline__ float origin(float m) { return F16 && WIN && fabsf(m) < 4194304.f ? m - 7.f : m; }
 
 // Up to so many first keys make a tile of their own width instead of a whole one (2 x 8192 tokens, 32 heads, window 1024, 4 first
 // keys: with whole tiles, and with side B going through the tile that it sees nothing of, 400 us).
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
 #pragma unroll
           for (int i = 0; i < kNarrow; i += 2) mx = max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
           m_run = mx * p.scale_log2;
-          const float shift = m_run == -INFINITY ? 0.f : kLift<F16, WIN> - m_run;
+          const float shift = m_run == -INFINITY ? 0.f : -origin<F16, WIN>(m_run);
           const float2 neg = make_float2(shift, shift);
           float2 sum = make_float2(0.f, 0.f);
           uint32_t pk[kNarrow / 2];
@@ -630,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
           // 16 at a time 328, one to an instruction 322, between the exponentials 336, two loads in flight 328.)
           // (each row by itself, so that none depends on what its neighbours in the warp see)
           const float m_new = WIN && !(mx > m_run + kGrowth) ? m_run : fmaxf(m_run, mx);
-          const float alpha = m_new == m_run ? 1.f : fast_exp2(m_run - m_new);
+          const float alpha = m_new == m_run ? 1.f : fast_exp2(origin<F16, WIN>(m_run) - origin<F16, WIN>(m_new));
           const float2 alpha2 = make_float2(alpha, alpha);
           l_run *= alpha;
           m_run = m_new;
@@ -650,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
           }
         }
         // (a row that has seen scores of minus infinity only: they weigh 0, and not the NaN of their difference)
-        const float shift = m_run == -INFINITY ? 0.f : kLift<F16, WIN> - m_run;
+        const float shift = m_run == -INFINITY ? 0.f : -origin<F16, WIN>(m_run);
         const float2 neg = make_float2(shift, shift);
         float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -758,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_kernel(const __grid
       } else {
         // the two sides' maxima and sums, in buffers that alternate from item to item
         volatile float* mine = merge + (dn & 1) * 512;
-        mine[x * 256 + row] = m_run;
+        mine[x * 256 + row] = origin<F16, WIN>(m_run);
         mine[x * 256 + 128 + row] = l_run;
         __syncwarp();
         if (lane == 0) mbar_arrive(merge_bar);

@@ -21,8 +21,8 @@
 //     to 8 heads.  (A tcgen05 tile is 128 rows; the rate asked for here is 1 % of what those do.)
 //   * A step that raises no running maximum, which a vote finds out, needs no reduction over lanes.
 //   * The weights enter the second product as two 16-bit numbers, the rounded value and what it lost, so that the output has
-//     one rounding to 16 bits, its own.  fp16 has no numbers below 2^-24, so there the largest weight is 2^14 instead of 1
-//     (kLift): what is lost of a weight is at most 2^-39 of the largest.
+//     one rounding to 16 bits, its own.  fp16 has no numbers below 2^-24, so there the largest weight is 2^14 instead of 1:
+//     what is lost of a weight is at most 2^-39 of the largest.
 // Two ways to share out the keys:
 //   cluster  the CTAs of a cluster take equal parts of one sequence and key head and add up through distributed shared
 //            memory: one launch, no workspace.  For sequences of few tiles.
@@ -61,10 +61,11 @@ constexpr int kBlock = 16;                       // keys of a product
 constexpr int kHalfBlock = kBlock * 128;         // bytes of a block's keys (or values) in a panel
 constexpr int kJoinThreads = 512;
 constexpr int64_t kMostKeys = 0x7fffffff - 1023;   // of a sequence: positions are looked at up to a batch of blocks behind the last
-// fp16: weights are made 2^kLift times as large.  (At 0, 20000 keys that weigh 2^-26 of the largest each, 3e-4 of the sum, were
-// left out of the output; 14 and not 15, as a score's rounding may put a weight above the maximum's.)
+// What the exponents of the weights are counted from, for a maximum m.  fp16: weights are made 2^14 times as large.  (At 1, 20000
+// keys that weigh 2^-26 of the largest each, 3e-4 of the sum, were left out of the output; 14 and not 15, as a score's rounding may
+// put a weight above the maximum's.)  Not where m is so large that its own rounding would take a weight out of what fp16 holds.
 template <bool F16>
-constexpr float kLift = F16 ? 14.f : 0.f;
+__device__ __forceinline__ float origin(float m) { return F16 && fabsf(m) < 4194304.f ? m - 14.f : m; }
 constexpr uint32_t kSitePage = 95, kSiteLoad = 98, kSiteTile = 99;
 
 template <int D, int COLS = 8>
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
         x += __shfl_xor_sync(0xffffffffu, x, 16);
         const int row = 8 * n + 2 * t + e;
         if (g == 0) {
-          stat_m[warp * kRows + row] = m[n][e] - kLift<F16>;   // (what the weights and their sum are scaled by)
+          stat_m[warp * kRows + row] = origin<F16>(m[n][e]);
           stat_l[warp * kRows + row] = x;
         }
 #pragma unroll
@@ -664,7 +665,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             const float m_new = fmaxf(m[n][e], x);
-            const float f = m_new == m[n][e] ? 1.f : exp2_fast(m[n][e] - m_new);
+            const float f = m_new == m[n][e] ? 1.f : exp2_fast(origin<F16>(m[n][e]) - origin<F16>(m_new));
             m[n][e] = m_new;
             sum[n][e] *= f;
 #pragma unroll
@@ -674,7 +675,7 @@ __global__ void __launch_bounds__(Shape<D, COLS>::kThreads, Shape<D, COLS>::kPer
       uint32_t hi[kB][kN][2], lo[kB][kN][2];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        const float s0 = m[n][0] == -INFINITY ? 0.f : kLift<F16> - m[n][0], s1 = m[n][1] == -INFINITY ? 0.f : kLift<F16> - m[n][1];
+        const float s0 = m[n][0] == -INFINITY ? 0.f : -origin<F16>(m[n][0]), s1 = m[n][1] == -INFINITY ? 0.f : -origin<F16>(m[n][1]);
 #pragma unroll
         for (int j = 0; j < kB; ++j)
 #pragma unroll

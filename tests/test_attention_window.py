@@ -157,6 +157,32 @@ def test_weights_far_below_the_largest_count(first, heads, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("heads", [1, 40])                  # keys of a query tile shared out; pairs of query tiles
+@pytest.mark.parametrize("sign", [1, -1])
+def test_huge_scores_stay_finite(sign, heads):
+    """fp16, scores of up to 2^27 (in powers of two) of either sign, each off by as much as 4: every 50th key is far above the
+    others, so that the values of the largest one that a row sees are its output, to the rounding of its weight and its own."""
+    seq, window = 900, 130
+    qkv, _, out = _inputs(1, seq, heads, heads, torch.float16)
+    x = qkv.unflatten(1, (3, heads, 128))
+    g = torch.Generator().manual_seed(3)
+    size = torch.randint(20, 50, (seq // 50,), generator=g).unique().flip(0).repeat(18)[:18] * 600.0
+    x[:, :2] = 0.0
+    x[:, 0, :, 0] = 20000.0
+    x[:, 1, :, 0] = 3000.0 if sign > 0 else -60000.0
+    x[::50, 1, :, 0] = (size if sign > 0 else size - 59000.0)[:, None].to("cuda", torch.float16)
+    A.attention_window_fwd(qkv, out, 1, seq, heads, window=window)
+    k, v = x[:, 1, 0, 0].double(), x[:, 2].double()
+    for row in range(0, seq, 7):
+        seen = torch.arange(max(0, row - window + 1), row + 1, device="cuda")
+        best = k[seen] == k[seen].max()
+        if best.sum() > 1:                                   # (rows that see none of the large ones, or two alike)
+            continue
+        want = v[seen[best]][0].flatten()
+        assert bool(((out[row].double() - want).abs() <= 2 * HALF[torch.float16] * want.abs() + 2.0 ** -24).all()), row
+
+
+@gpu
 def test_in_a_graph_and_on_another_stream():
     qkv, _, out = _inputs(2, 300, 4, 2, torch.bfloat16)
     st = torch.cuda.Stream()

@@ -490,6 +490,31 @@ def test_attention_weights_far_below_the_largest_count(dtype, wide):
     assert bool(((case.lse[0].double() - (18.0 + math.log1p(others))).abs() <= 2.0 ** -22 * 20 + rel * others).all())
 
 
+@gpu
+@pytest.mark.parametrize("wide", [None, 5000])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_of_huge_scores_stays_finite(sign, wide):
+    """fp16, scores of up to 2^27 (in powers of two) of either sign, each off by as much as 4: one key of each sequence is
+    far above the others, so that its values are the output (to a weight's 2^-16 and the output's rounding)."""
+    lens = [200 + 37 * i for i in range(12)]
+    case = Case(lens, 4, 2, 64, 16, torch.float16, wide=wide, seed=5)
+    g = torch.Generator().manual_seed(11)
+    want = torch.empty((12, 4, 64), dtype=torch.float64, device="cuda")
+    case.q.zero_()
+    for b, n in enumerate(lens):
+        j = torch.arange(n, device="cuda")
+        at = case.table[b].long()[j // 16], j % 16
+        size = float(torch.randint(4000, 30000, (1,), generator=g))
+        case.q[b, :, 0] = 2000.0 + 97 * b
+        case.k[at] = 0.0
+        case.k[at[0], at[1], :, 0] = size / 2 if sign > 0 else -2 * size
+        top = int(torch.randint(0, n, (1,), generator=g))
+        case.k[at[0][top], at[1][top], :, 0] = size * sign
+        want[b] = case.v[at[0][top], at[1][top]].double().repeat_interleave(2, 0)
+    case.run(scale=1.0)
+    assert bool(((case.out.double() - want).abs() <= (HALF[torch.float16] + 2.0 ** -15) * want.abs()).all())
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------
 
 def _plain_reserve(lens, new, table, free, count, page, rows, row_stride):
