@@ -25,7 +25,7 @@
 //                   product starts when the first half of P is there
 // What bounds it: the chain of one side, scores -> softmax -> product: 4100 - 4700 cycles per step of a pair for 2048 of MMAs
 // and 2048 of ex2; in a long run the GPU's power limit takes the clock besides.  8 x 2048 tokens x 32 heads bf16, causal /
-// without a mask: from a rest, 1965 MHz, 298 / 499 us (317 / 524 with output rows written 16 bytes at a time); a run of seconds,
+// without a mask: from a rest, 1965 MHz, 298 / 499 us (314 / 522 with output rows written 16 bytes at a time); a run of seconds,
 // 1582 MHz at 990 W, 338 / 575 us.  A scale that is renewed only after a growth of 2^8 saved another 30 / 57 us from a rest, but
 // then a row's largest weight is rounded like the others and the error against 64 bits grows by 2 to 4 % (2.034e-3 -> 2.071e-3,
 // 2.256e-3 -> 2.337e-3, both bf16).

@@ -6,8 +6,8 @@
 // the first `sinks`.  Key j lies in slot j % page_size of page block_table[b, j / page_size]; query head h reads key head
 // h / (heads / kv_heads).  16-bit elements, fp32 sums, head dimension 64, 128 or 256.  No counterpart in the reference.
 //
-// Every key and value is read once and used for 2 * group products: HBM bounds it, and the work goes into an even share of
-// the bytes for every SM, enough of them in flight, and few instructions per byte.
+// Every key and value is read once (once for every 16 query heads that share it) and used for 2 * group products: HBM bounds it,
+// and the work goes into an even share of the bytes for every SM, enough of them in flight, and few instructions per byte.
 //   * The keys that are seen are counted through in blocks of 16 (first keys, then the window), so a mask costs nothing but at
 //     the blocks' edges: a position in that count gives the key, the key its page.
 //   * One warp loads: it looks the pages of 32 blocks up at a time, a batch ahead, and has the TMA unit copy the blocks (a 4-D

@@ -60,9 +60,9 @@ def attention_window_fwd(qkv: torch.Tensor, out: torch.Tensor, batch: int, seq: 
 
     ``qkv`` is ``[batch * seq, (heads + 2 * kv_heads) * 128]`` with the Q, K and V column blocks side by side, query head ``h``
     reading key head ``h // (heads // kv_heads)``; ``out`` is ``[batch * seq, heads * 128]``; rows may be strided views.
-    ``seq``: any length.  ``out`` may be the query columns of ``qkv`` themselves.  ``status``: as for :func:`attention_fwd`.  A masked key weighs exactly nothing; a masked *value* that
-    is infinite or NaN still reaches the queries of its sequence whose window shares its tile of 128 keys (zero times it), so
-    the rows of padding have to be finite.
+    ``seq``: any length.  ``out`` may be the query columns of ``qkv`` themselves.  ``status``: as for :func:`attention_fwd`, at
+    least 32 bytes.  A masked key weighs exactly nothing; a masked *value* that is infinite or NaN still reaches the queries of its
+    sequence whose window shares its tile of 128 keys (zero times it), so the rows of padding have to be finite.
     """
     kv_heads = heads if kv_heads is None else kv_heads
     dtype, shape = qkv.dtype, qkv.shape

@@ -202,7 +202,7 @@ def reserve_slots(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     if max_len is None and not fresh:
         rc = _native.entry("iris_k_reserve_slots")(args)
     else:
-        rc = _native.entry("iris_k_reserve_slots_within")(args + _LIMITS.pack(0x7fffffff if max_len is None else max_len, fresh))
+        rc = _native.entry("iris_k_reserve_slots_within")(args + _LIMITS.pack(0x7fffffff if max_len is None else min(max_len, 0x7fffffff), fresh))
     if rc:
         _raise("reserve_slots", rc)
 
